@@ -31,7 +31,9 @@ enum {
     SB200_ERR_UNSUPPORTED = 3,   /* valid request this build cannot run              */
     SB200_ERR_DEVICE_TIMEOUT = 4,/* a bounded wait inside a kernel expired           */
     SB200_ERR_ALLOC = 5,         /* device or host allocation failed                 */
-    SB200_ERR_TOO_LARGE = 6      /* size beyond a documented limit                   */
+    SB200_ERR_TOO_LARGE = 6,     /* size beyond a documented limit                   */
+    SB200_ERR_TOKEN_RANGE = 7    /* a token number beyond the vocabulary (found on the
+                                    device: sb200_check_device_status)               */
 };
 
 /* Arithmetic of the dense GEMM.
@@ -44,6 +46,10 @@ enum {
  *            to about 1e-6 relative.
  */
 enum { SB200_MODE_TF32 = 0, SB200_MODE_TF32X3 = 1 };
+
+/* Element types of the operators of token models further down (the GEMM and the
+ * elementwise steps of an MLP are fp32). */
+enum { SB200_F32 = 0, SB200_BF16 = 1, SB200_F16 = 2 };
 
 /* Which kernel family ran; for tests and profiling. */
 enum { SB200_PATH_AUTO = 0, SB200_PATH_TCGEN05 = 1, SB200_PATH_SIMT = 2 };
@@ -135,8 +141,10 @@ enum { SB200_OPT_SPLIT_EXPLICIT_HI = 1, SB200_OPT_MERGE_MN_BOXES = 2, SB200_OPT_
 int sb200_ctx_set_option(sb200_ctx* ctx, int option, int value);
 
 /* Reads (and clears) the device status word after synchronising the stream.
- * Non-zero means a bounded wait in a kernel gave up; the results of that
- * launch are undefined but the context stays usable. */
+ * SB200_ERR_DEVICE_TIMEOUT means a bounded wait in a kernel gave up: the results of
+ * that launch are undefined.  SB200_ERR_TOKEN_RANGE means an embedding call met a
+ * token number beyond the vocabulary and treated it as padding.  The word keeps the
+ * first of several events; the context stays usable. */
 int sb200_check_device_status(sb200_ctx* ctx, sb200_stream stream);
 
 /*
@@ -553,6 +561,103 @@ int sb200_sgd_update(sb200_ctx* ctx, float* z, const float* dz, float lr, int64_
  * (Sources/Sapphire/compute/dense/cuda/kernels/BasicKernel.cu:115-125). */
 int sb200_scale(sb200_ctx* ctx, float* out, const float* in, float factor, int64_t n,
                 sb200_stream stream);
+
+/* ---- operators of token models -------------------------------------------
+ * What a stack of Linear layers needs around it to be trained on tokens: the
+ * embedding at its front, layer norm between the layers, and the orthogonalised
+ * update of its matrix weights (beside sb200_sgd_update).  The reference has no
+ * counterpart (its units are the Linear, convolution and elementwise ones).
+ *
+ * Matrices are row-major with a leading dimension (row pitch) in elements; any
+ * pointer aligned to its element is accepted, and 16-byte aligned rows whose width
+ * is a multiple of 16 bytes are the fast case.  Scratch memory is the caller's: a
+ * call that needs some has a *_workspace function that returns its size in bytes
+ * (-1: arguments the call would refuse), and takes a 16-byte aligned device buffer
+ * of at least that size, whose content before the call does not matter.  So nothing
+ * is allocated, the calls can be captured into CUDA graphs as they are, and two of
+ * them may run at the same time if their workspaces and outputs differ.  Results
+ * are the same bits run to run.
+ */
+
+/*
+ * out[t, :] = scale * table[ids[t], :] for n tokens; table is [vocab, cols] of
+ * table_type, out [n, cols] of type.  ids: n numbers of index_bits (32 or 64) bits.
+ * A negative number is padding: its row of out is zero.  A number >= vocab gives a
+ * row of zeros too and is reported as SB200_ERR_TOKEN_RANGE by
+ * sb200_check_device_status.  The two types are equal or one of them is SB200_F32
+ * (SB200_ERR_UNSUPPORTED otherwise); the product is rounded once.
+ * Limits (SB200_ERR_TOO_LARGE): n <= 2^30, vocab <= 2^31 - 2, cols <= 2^20.
+ */
+int sb200_embedding(sb200_ctx* ctx, void* out, int64_t ldo, const void* table, int64_t ldt,
+                    const void* ids, int index_bits, int64_t n, int64_t vocab, int64_t cols,
+                    float scale, int table_type, int type, sb200_stream stream);
+
+/*
+ * The table's gradient: dtable[v, :] = scale * sum of dout[t, :] over the tokens t
+ * with ids[t] == v, in an order that depends on the token numbers alone; sums in
+ * fp32, rounded once.  accumulate = 0: every row of dtable is written, with zeros
+ * where no token names it.  accumulate != 0: the sums are added to dtable and the
+ * other rows are neither read nor written; with dtable the table itself and scale
+ * times -lr this is the SGD step of the rows in use.  Padding and out-of-range
+ * numbers contribute nothing (the latter are reported as by sb200_embedding).
+ * table_type is dtable's type, type dout's; limits as above.
+ */
+int64_t sb200_embedding_backward_workspace(const sb200_ctx* ctx, int64_t n, int64_t vocab, int64_t cols);
+int sb200_embedding_backward(sb200_ctx* ctx, void* dtable, int64_t ldt, const void* dout, int64_t ldo,
+                             const void* ids, int index_bits, int64_t n, int64_t vocab, int64_t cols,
+                             float scale, int table_type, int type, int accumulate,
+                             void* workspace, int64_t workspace_bytes, sb200_stream stream);
+
+/*
+ * Layer norm of `rows` rows of `cols` elements:
+ *     mean = sum x / cols,  rstd = 1 / sqrt(sum (x - mean)^2 / cols + eps),
+ *     y = (x - mean) * rstd * weight + bias
+ * x and y of `type`, weight and bias [cols] of weight_type, which is `type` or
+ * SB200_F32; weight NULL is 1, bias NULL is 0.  mean and rstd ([rows], fp32, each may
+ * be NULL) are what the backward pass wants.  y may be x itself (same pointer and
+ * pitch).  Statistics in fp32 from differences to the mean; y is rounded once.
+ */
+int sb200_layer_norm(sb200_ctx* ctx, void* y, int64_t ldy, float* mean, float* rstd,
+                     const void* x, int64_t ldx, const void* weight, const void* bias,
+                     int64_t rows, int64_t cols, float eps, int type, int weight_type,
+                     sb200_stream stream);
+
+/*
+ * With h = (x - mean) * rstd and g = dy * weight:
+ *     dx = rstd * (g - sum g / cols - h * sum (g h) / cols)      (dx may be NULL)
+ *     dweight = sum over rows of dy * h, dbias = sum over rows of dy   (each may be NULL)
+ * accumulate_dx / accumulate_weight != 0 add to what the buffers hold (dx, as a
+ * residual branch wants it; dweight and dbias, over several micro-batches).  dx may
+ * be dy itself.  The workspace is needed when dweight or dbias is asked for.  With
+ * no rows dweight and dbias are zero (or stay as they are when they accumulate).
+ */
+int64_t sb200_layer_norm_backward_workspace(const sb200_ctx* ctx, int64_t rows, int64_t cols);
+int sb200_layer_norm_backward(sb200_ctx* ctx, void* dx, int64_t lddx, void* dweight, void* dbias,
+                              const void* dy, int64_t lddy, const void* x, int64_t ldx,
+                              const void* weight, const float* mean, const float* rstd,
+                              int64_t rows, int64_t cols, int type, int weight_type,
+                              int accumulate_dx, int accumulate_weight,
+                              void* workspace, int64_t workspace_bytes, sb200_stream stream);
+
+/*
+ * The orthogonalised update of `batch` matrices g [rows, cols] (gradients or their
+ * momentum), as the Muon optimizer takes it in the place of the gradient itself:
+ *     X = g / (|g| + eps)  (Frobenius norm),  then `steps` times
+ *     A = X X^T,  X = a X + (b A + c A A) X   (with X^T X on the right for a tall g),
+ * out = X.  The usual coefficients 3.4445, -4.7750, 2.0315 and five steps bring the
+ * singular values near one.  g and out are of `type` and may be the same matrix.
+ * SB200_F32 and SB200_F16 are computed to about fp32 accuracy (operands in two fp16
+ * parts, 22 bits); SB200_BF16 with operands of 11 bits, its own result having 8.
+ * Coefficients that let a singular value, or |b s^2 + c s^4|, pass about 7 on the
+ * way are refused (SB200_ERR_UNSUPPORTED).  Limits (SB200_ERR_TOO_LARGE): sides
+ * <= 2^20, batch <= 65535, steps <= 64.  The waits inside the kernels are bounded like those of the GEMM.
+ */
+int64_t sb200_orthogonalize_workspace(int64_t rows, int64_t cols, int64_t batch, int type);
+int sb200_orthogonalize(sb200_ctx* ctx, void* out, int64_t ldo, int64_t stride_out,
+                        const void* g, int64_t ldg, int64_t stride_g,
+                        int64_t rows, int64_t cols, int64_t batch, int steps,
+                        float a, float b, float c, float eps, int type,
+                        void* workspace, int64_t workspace_bytes, sb200_stream stream);
 
 #ifdef __cplusplus
 }

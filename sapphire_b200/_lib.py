@@ -12,8 +12,9 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libsapphire_b200.so")
 
 OK = 0
-ERR_INVALID_ARG, ERR_CUDA, ERR_UNSUPPORTED, ERR_DEVICE_TIMEOUT, ERR_ALLOC, ERR_TOO_LARGE = range(1, 7)
+ERR_INVALID_ARG, ERR_CUDA, ERR_UNSUPPORTED, ERR_DEVICE_TIMEOUT, ERR_ALLOC, ERR_TOO_LARGE, ERR_TOKEN_RANGE = range(1, 8)
 MODE_TF32, MODE_TF32X3 = 0, 1
+F32, BF16, F16 = 0, 1, 2
 PATH_AUTO, PATH_TCGEN05, PATH_SIMT = 0, 1, 2
 OPT_SPLIT_EXPLICIT_HI = 1
 OPT_MERGE_MN_BOXES = 2
@@ -144,6 +145,27 @@ SIGNATURES = {
     "sb200_sgd_update": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_float, C.c_int64,
                                    C.c_void_p]),
     "sb200_scale": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_float, C.c_int64, C.c_void_p]),
+    "sb200_embedding": (C.c_int, [
+        C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int,
+        C.c_int64, C.c_int64, C.c_int64, C.c_float, C.c_int, C.c_int, C.c_void_p]),
+    "sb200_embedding_backward_workspace": (C.c_int64, [C.c_void_p, C.c_int64, C.c_int64, C.c_int64]),
+    "sb200_embedding_backward": (C.c_int, [
+        C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int,
+        C.c_int64, C.c_int64, C.c_int64, C.c_float, C.c_int, C.c_int, C.c_int,
+        C.c_void_p, C.c_int64, C.c_void_p]),
+    "sb200_layer_norm": (C.c_int, [
+        C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p,
+        C.c_void_p, C.c_int64, C.c_int64, C.c_float, C.c_int, C.c_int, C.c_void_p]),
+    "sb200_layer_norm_backward_workspace": (C.c_int64, [C.c_void_p, C.c_int64, C.c_int64]),
+    "sb200_layer_norm_backward": (C.c_int, [
+        C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p,
+        C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_int, C.c_int,
+        C.c_int, C.c_int, C.c_void_p, C.c_int64, C.c_void_p]),
+    "sb200_orthogonalize_workspace": (C.c_int64, [C.c_int64, C.c_int64, C.c_int64, C.c_int]),
+    "sb200_orthogonalize": (C.c_int, [
+        C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_int64,
+        C.c_int64, C.c_int64, C.c_int64, C.c_int, C.c_float, C.c_float, C.c_float, C.c_float, C.c_int,
+        C.c_void_p, C.c_int64, C.c_void_p]),
     # Sapphire-signature shims (include/sapphire_b200_compat.h)
     "sb200_compat_set_mode": (C.c_int, [C.c_int]),
     "sb200_compat_dense_gemm": (C.c_int, [C.c_uint, C.c_void_p, C.c_void_p, C.c_void_p,

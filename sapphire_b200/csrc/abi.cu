@@ -120,6 +120,7 @@ extern "C" const char* sb200_status_string(int status)
         case SB200_ERR_DEVICE_TIMEOUT: return "a bounded wait inside a kernel expired";
         case SB200_ERR_ALLOC: return "allocation failed";
         case SB200_ERR_TOO_LARGE: return "size beyond a documented limit";
+        case SB200_ERR_TOKEN_RANGE: return "a token number beyond the vocabulary";
         default: return "unknown status";
     }
 }
@@ -195,7 +196,7 @@ extern "C" int sb200_check_device_status(sb200_ctx* ctx, sb200_stream stream_)
         return SB200_OK;
     cudaMemsetAsync(ctx->d_status, 0, sizeof(unsigned), stream);
     cudaStreamSynchronize(stream);
-    return SB200_ERR_DEVICE_TIMEOUT;
+    return word == FAULT_TOKEN_RANGE ? SB200_ERR_TOKEN_RANGE : SB200_ERR_DEVICE_TIMEOUT;
 }
 
 namespace {

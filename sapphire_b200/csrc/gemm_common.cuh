@@ -117,6 +117,31 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, const A
     return true;
 }
 
+// The same for barriers that the peer CTA of a pair arrives on: cluster-scope acquire.
+__device__ __forceinline__ bool wait_bar_cluster(uint64_t* bar, uint32_t parity, const Abort& ab,
+                                                 unsigned code)
+{
+    // The global timer is slow to read: the clock of a wait starts at its 64th failed
+    // try, so the waits of the steady state (a few tries) never read it.
+    uint64_t t0 = 0;
+    uint32_t spins = 0;
+    while (!ptx::mbar_try_wait_cluster(bar, parity)) {
+        if ((++spins & 63u) == 0) {
+            if (*ab.flag)
+                return false;
+            const uint64_t now = ptx::globaltimer_ns();
+            if (t0 == 0) {
+                t0 = now;
+            } else if (now - t0 > ab.limit_ns) {
+                *ab.flag = 1;
+                atomicCAS(ab.status, 0u, code);
+                return false;
+            }
+        }
+    }
+    return true;
+}
+
 // One thread's 32 consecutive output columns of one row: D = post((C + bias) + acc);
 // mrow is the row of the gate matrix or null.
 __device__ __forceinline__ void store_row_chunk(const uint32_t (&v)[32], float* drow,

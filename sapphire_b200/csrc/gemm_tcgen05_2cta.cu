@@ -39,31 +39,6 @@ constexpr int PAIR_TILES_BYTES = PAIR_STAGE_BYTES * PAIR_STAGES;
 constexpr int PAIR_BAR_BYTES = ((2 * PAIR_STAGES + 4) * 8 + 16 + 15) & ~15;
 constexpr int PAIR_SMEM = PAIR_TILES_BYTES + PAIR_BAR_BYTES + 4 * EPI_STAGE_BYTES_PER_WARP + 1024;
 
-// waits of this kernel see arrivals from the peer CTA: cluster-scope acquire
-__device__ __forceinline__ bool wait_bar_cluster(uint64_t* bar, uint32_t parity, const Abort& ab,
-                                                 unsigned code)
-{
-    // The global timer is slow to read: the clock of a wait starts at its 64th failed
-    // try, so the waits of the steady state (a few tries) never read it.
-    uint64_t t0 = 0;
-    uint32_t spins = 0;
-    while (!ptx::mbar_try_wait_cluster(bar, parity)) {
-        if ((++spins & 63u) == 0) {
-            if (*ab.flag)
-                return false;
-            const uint64_t now = ptx::globaltimer_ns();
-            if (t0 == 0) {
-                t0 = now;
-            } else if (now - t0 > ab.limit_ns) {
-                *ab.flag = 1;
-                atomicCAS(ab.status, 0u, code);
-                return false;
-            }
-        }
-    }
-    return true;
-}
-
 template <bool A_MN, bool B_MN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
 gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap mapA,

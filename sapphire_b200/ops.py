@@ -391,3 +391,219 @@ def scale(ctx, x, factor, out=None):
     out = x if out is None else out
     _ew("sb200_scale", ctx, out.data_ptr(), x.data_ptr(), float(factor), x.numel())
     return out
+
+
+# ---------------------------------------------------- operators of token models
+
+_TYPE = {torch.float32: L.F32, torch.bfloat16: L.BF16, torch.float16: L.F16}
+_INDEX_BITS = {torch.int32: 32, torch.int64: 64}
+
+
+def _type_code(t: torch.Tensor, what: str) -> int:
+    code = _TYPE.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{what}: float32, bfloat16 or float16, got {t.dtype}")
+    return code
+
+
+def _on_device(ctx: Context, t: torch.Tensor, what: str) -> None:
+    if not t.is_cuda or t.device.index != ctx.device:
+        raise ValueError(f"{what} must be on cuda:{ctx.device}, got {t.device}")
+
+
+def _rows(ctx: Context, t: torch.Tensor, what: str):
+    """(rows, cols, row pitch) of a tensor seen as rows of its contiguous last dimension;
+    the leading dimensions must be equally spaced rows."""
+    _on_device(ctx, t, what)
+    if t.dim() < 1:
+        raise ValueError(f"{what} needs a last dimension")
+    cols = t.shape[-1]
+    if t.dim() == 2:
+        rows, pitch, inner = t.shape[0], t.stride(0), t.stride(1)
+    elif t.is_contiguous():
+        rows, pitch, inner = (t.numel() // cols if cols else 0), cols, 1
+    else:
+        inner, rows, pitch = t.stride(-1), 1, None
+        for size, step in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+            if size == 1:
+                continue
+            if pitch is None:
+                pitch = step
+            elif step != pitch * rows:
+                raise ValueError(f"{what}: the rows must be equally spaced")
+            rows *= size
+    if cols > 1 and inner != 1:
+        raise ValueError(f"{what}: the last dimension must be contiguous")
+    if rows <= 1 or pitch is None:
+        pitch = cols if pitch is None or pitch < cols else pitch
+    elif pitch < cols:
+        raise ValueError(f"{what}: rows overlap")
+    return rows, cols, pitch
+
+
+def _vector(ctx: Context, t: torch.Tensor, n: int, what: str) -> int:
+    _on_device(ctx, t, what)
+    if t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous vector of {n} elements")
+    return t.data_ptr()
+
+
+def _scratch(name: str, nbytes: int, ctx: Context):
+    """A workspace from torch's allocator: it belongs to the current stream, and inside a
+    graph capture to the graph."""
+    if nbytes < 0:
+        raise L.Sb200Error(name, L.ERR_TOO_LARGE)
+    return torch.empty(max(nbytes, 1), dtype=torch.uint8, device=torch.device("cuda", ctx.device))
+
+
+def _ids(ctx: Context, ids: torch.Tensor):
+    _on_device(ctx, ids, "ids")
+    bits = _INDEX_BITS.get(ids.dtype)
+    if bits is None:
+        raise TypeError(f"ids: int32 or int64, got {ids.dtype}")
+    return (ids if ids.is_contiguous() else ids.contiguous()), bits
+
+
+def embedding(ctx: Context, table: torch.Tensor, ids: torch.Tensor, *, scale: float = 1.0,
+              out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """out[..., :] = scale * table[ids[...], :].  A negative id is padding (a row of zeros);
+    an id beyond the table gives zeros and is reported by ``ctx.check_device_status()``.
+    ``out_dtype`` (default: the table's) may differ from the table's if one of the two is
+    float32."""
+    if table.dim() != 2:
+        raise ValueError("table must be [vocab, cols]")
+    vocab, cols, ldt = _rows(ctx, table, "table")
+    ids, bits = _ids(ctx, ids)
+    if out is None:
+        out = torch.empty(*ids.shape, cols, dtype=out_dtype or table.dtype, device=table.device)
+    elif out_dtype is not None and out.dtype != out_dtype:
+        raise TypeError("out has another dtype than out_dtype")
+    elif out.shape != (*ids.shape, cols):
+        raise ValueError("out must be [*ids.shape, cols]")
+    _, _, ldo = _rows(ctx, out, "out")
+    _ew("sb200_embedding", ctx, out.data_ptr(), ldo, table.data_ptr(), ldt, ids.data_ptr(), bits, ids.numel(), vocab,
+        cols, scale, _type_code(table, "table"), _type_code(out, "out"))
+    return out
+
+
+def embedding_backward(ctx: Context, dtable: torch.Tensor, dout: torch.Tensor, ids: torch.Tensor, *,
+                       scale: float = 1.0, accumulate: bool = False) -> torch.Tensor:
+    """dtable[v, :] = scale * sum of dout over the tokens with id v (0 where there is none);
+    ``accumulate`` adds to dtable instead and leaves the rows without tokens alone.
+    Returns ``dtable``."""
+    if dtable.dim() != 2:
+        raise ValueError("dtable must be [vocab, cols]")
+    vocab, cols, ldt = _rows(ctx, dtable, "dtable")
+    ids, bits = _ids(ctx, ids)
+    if dout.shape != (*ids.shape, cols):
+        raise ValueError("dout must be [*ids.shape, cols]")
+    _, _, ldo = _rows(ctx, dout, "dout")
+    n = ids.numel()
+    ws = _scratch("sb200_embedding_backward",
+                  L.lib().sb200_embedding_backward_workspace(ctx.handle, n, vocab, cols), ctx)
+    _ew("sb200_embedding_backward", ctx, dtable.data_ptr(), ldt, dout.data_ptr(), ldo, ids.data_ptr(), bits, n, vocab,
+        cols, scale, _type_code(dtable, "dtable"), _type_code(dout, "dout"), int(accumulate), ws.data_ptr(), ws.numel())
+    return dtable
+
+
+def layer_norm(ctx: Context, x: torch.Tensor, weight: Optional[torch.Tensor] = None,
+               bias: Optional[torch.Tensor] = None, *, eps: float = 1e-5, out: Optional[torch.Tensor] = None,
+               mean: Optional[torch.Tensor] = None, rstd: Optional[torch.Tensor] = None):
+    """Layer norm over the last dimension; returns (out, mean, rstd), the last two fp32 of
+    the leading shape, as the backward pass wants them.  ``out`` may be ``x``.  weight and
+    bias are of x's dtype or float32."""
+    rows, cols, ldx = _rows(ctx, x, "x")
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    elif out.shape != x.shape or out.dtype != x.dtype:
+        raise ValueError("out must have x's shape and dtype")
+    if mean is None:
+        mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    if rstd is None:
+        rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    if mean.dtype != torch.float32 or rstd.dtype != torch.float32:
+        raise TypeError("mean and rstd are float32")
+    code = _type_code(x, "x")
+    wcode, wptr, bptr = _norm_weights(ctx, cols, code, weight, bias)
+    _, _, ldo = _rows(ctx, out, "out")
+    _ew("sb200_layer_norm", ctx, out.data_ptr(), ldo, _vector(ctx, mean, rows, "mean"), _vector(ctx, rstd, rows, "rstd"),
+        x.data_ptr(), ldx, wptr, bptr, rows, cols, eps, code, wcode)
+    return out, mean, rstd
+
+
+def _norm_weights(ctx, cols, code, weight, bias, names=("weight", "bias")):
+    """(type code, pointer, pointer) of two vectors of one dtype, either of which may be None."""
+    wcode = code
+    for t, what in zip((weight, bias), names):
+        if t is not None:
+            wcode = _type_code(t, what)
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise TypeError(f"{names[0]} and {names[1]} must have one dtype")
+    return (wcode, None if weight is None else _vector(ctx, weight, cols, names[0]),
+            None if bias is None else _vector(ctx, bias, cols, names[1]))
+
+
+def layer_norm_backward(ctx: Context, dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
+                        weight: Optional[torch.Tensor] = None, *, dx: Optional[torch.Tensor] = None,
+                        dweight: Optional[torch.Tensor] = None, dbias: Optional[torch.Tensor] = None,
+                        accumulate_dx: bool = False, accumulate_weight: bool = False):
+    """Returns (dx, dweight, dbias); buffers that are not given are allocated, dweight and
+    dbias with the weight's dtype (x's without one).  ``accumulate_dx`` adds to dx (a
+    residual branch's gradient), ``accumulate_weight`` to dweight and dbias (further
+    micro-batches): the buffers concerned must then be given.  ``dx`` may be ``dy``."""
+    rows, cols, ldx = _rows(ctx, x, "x")
+    if dy.shape != x.shape or dy.dtype != x.dtype:
+        raise ValueError("dy must have x's shape and dtype")
+    _, _, ldy = _rows(ctx, dy, "dy")
+    if (accumulate_dx and dx is None) or (accumulate_weight and (dweight is None or dbias is None)):
+        raise ValueError("accumulating needs the buffers that are added to")
+    if mean.dtype != torch.float32 or rstd.dtype != torch.float32:
+        raise TypeError("mean and rstd are float32")
+    if dx is None:
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    elif dx.shape != x.shape or dx.dtype != x.dtype:
+        raise ValueError("dx must have x's shape and dtype")
+    code = _type_code(x, "x")
+    wdtype = weight.dtype if weight is not None else dweight.dtype if dweight is not None else x.dtype
+    if dweight is None:
+        dweight = torch.empty(cols, dtype=wdtype, device=x.device)
+    if dbias is None:
+        dbias = torch.empty(cols, dtype=wdtype, device=x.device)
+    if dweight.dtype != wdtype or dbias.dtype != wdtype:
+        raise TypeError("dweight and dbias must have the weight's dtype")
+    wcode, dwptr, dbptr = _norm_weights(ctx, cols, code, dweight, dbias, ("dweight", "dbias"))
+    _, _, lddx = _rows(ctx, dx, "dx")
+    ws = _scratch("sb200_layer_norm_backward",
+                  L.lib().sb200_layer_norm_backward_workspace(ctx.handle, rows, cols), ctx)
+    _ew("sb200_layer_norm_backward", ctx, dx.data_ptr(), lddx, dwptr, dbptr, dy.data_ptr(), ldy, x.data_ptr(), ldx,
+        None if weight is None else _vector(ctx, weight, cols, "weight"), _vector(ctx, mean, rows, "mean"),
+        _vector(ctx, rstd, rows, "rstd"), rows, cols, code, wcode, int(accumulate_dx), int(accumulate_weight),
+        ws.data_ptr(), ws.numel())
+    return dx, dweight, dbias
+
+
+def orthogonalize(ctx: Context, g: torch.Tensor, *, steps: int = 5, coefficients=(3.4445, -4.7750, 2.0315),
+                  eps: float = 1e-7, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The orthogonalised update of a matrix [rows, cols], or of each of a batch of them:
+    x = g / (|g| + eps), then ``steps`` Newton-Schulz products
+    x = a x + (b A + c A A) x with A = x x^T.  ``out`` may be ``g``; apply it with
+    ``sgd_update``."""
+    if g.dim() not in (2, 3):
+        raise ValueError("expected [rows, cols] or [batch, rows, cols]")
+    if out is None:
+        out = torch.empty(g.shape, dtype=g.dtype, device=g.device)
+    elif out.shape != g.shape or out.dtype != g.dtype:
+        raise ValueError("out must have g's shape and dtype")
+    code = _type_code(g, "g")
+    batch = g.shape[0] if g.dim() == 3 else 1
+    (rows, cols), geometry = g.shape[-2:], []
+    for t, what in ((out, "out"), (g, "g")):
+        _on_device(ctx, t, what)
+        if cols > 1 and t.stride(-1) != 1:
+            raise ValueError(f"{what}: the last dimension must be contiguous")
+        ld = t.stride(-2) if rows > 1 else max(cols, t.stride(-2))
+        geometry += [t.data_ptr(), ld, t.stride(0) if t.dim() == 3 else 0]
+    a, b, c = coefficients
+    ws = _scratch("sb200_orthogonalize", L.lib().sb200_orthogonalize_workspace(rows, cols, batch, code), ctx)
+    _ew("sb200_orthogonalize", ctx, *geometry, rows, cols, batch, int(steps), a, b, c, eps, code, ws.data_ptr(), ws.numel())
+    return out

@@ -1,0 +1,572 @@
+"""GPU parity of the token-model operators (embedding, layer norm, orthogonalised update)
+with their definitions in 64 bits.
+
+Tolerances are bounds, counted before the kernels ran.  u = 2^-24 is the rounding of an
+fp32 operation, h(T) = finfo(T).eps / 2 the rounding of a result to T.  A sum of which each
+term passes through D additions is off by at most D u times the sum of the absolute values
+(first order; the bounds below count a few operations more than there are)."""
+import math
+
+import pytest
+import torch
+
+from sapphire_b200 import _lib as L
+from sapphire_b200 import ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+U = 2.0 ** -24
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+def half_step(t):
+    return torch.finfo(t).eps / 2
+
+
+def tiny(t):
+    """Half the spacing of T's subnormal numbers."""
+    return torch.finfo(t).smallest_normal * torch.finfo(t).eps / 2
+
+
+def gen(seed):
+    g = torch.Generator()
+    g.manual_seed(seed)
+    return g
+
+
+def randn(g, *shape, dtype=F32, pitch=None, offset=0):
+    """Normal values on the device, as rows of `pitch` elements starting `offset` elements in."""
+    x = torch.randn(*shape, generator=g).to(dtype)
+    if pitch is None and not offset:
+        return x.to(DEV)
+    rows, cols = shape
+    pitch = pitch or cols
+    flat = torch.full((rows * pitch + offset + 16,), float("nan"), dtype=dtype, device=DEV)
+    view = flat[offset:offset + rows * pitch].view(rows, pitch)[:, :cols]
+    view.copy_(x.to(DEV))
+    return view
+
+
+def check(got, want, tol):
+    got, want = got.double().cpu(), want.double().cpu()
+    assert got.shape == want.shape
+    off = (got - want).abs()
+    bad = ~(off <= tol.double().cpu() if torch.is_tensor(tol) else off <= tol)
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} values off, the worst by {float(off[bad].max()):.3g}"
+
+
+# --------------------------------------------------------------------- embedding
+
+COMBOS = [(F32, F32), (BF16, BF16), (F16, F16), (F32, BF16), (F32, F16), (BF16, F32), (F16, F32)]
+
+
+def token_ids(g, n, vocab, dtype, pad=True):
+    ids = (torch.rand(n, generator=g) ** 3 * vocab).long().clamp_(0, max(vocab - 1, 0))
+    if pad and n > 2:
+        ids[torch.randperm(n, generator=g)[: n // 5]] = -1
+        ids[n // 2] = -100
+    return ids.to(dtype)
+
+
+@pytest.mark.parametrize("tt,ta", COMBOS)
+@pytest.mark.parametrize("n,vocab,cols,index", [(1, 1, 1, torch.int64), (5, 10, 7, torch.int32), (64, 100, 512, torch.int64),
+                                                (333, 1000, 264, torch.int32), (1025, 77, 1000, torch.int64), (3, 5, 8200, torch.int64)])
+def test_embedding(ctx, tt, ta, n, vocab, cols, index):
+    g = gen(n + cols)
+    table = randn(g, vocab, cols, dtype=tt)
+    ids = token_ids(g, n, vocab, index)
+    scale = math.sqrt(cols)
+    out = ops.embedding(ctx, table, ids.to(DEV), scale=scale, out_dtype=ta)
+    assert out.dtype == ta and out.shape == (n, cols)
+    s32 = float(torch.tensor(scale, dtype=F32))
+    want = torch.where((ids >= 0)[:, None], table.cpu().double()[ids.long().clamp_min(0)] * s32, 0.0)
+    check(out, want, want.abs() * (half_step(ta) + U) * 1.0001 + tiny(ta))
+    ctx.check_device_status()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("pitch,offset", [(24, 0), (19, 0), (24, 1), (17, 3)])
+def test_embedding_strides(ctx, dtype, pitch, offset):
+    """Row pitches and base addresses that 16-byte accesses do not fit."""
+    g = gen(3)
+    table = randn(g, 40, 16, dtype=dtype, pitch=pitch, offset=offset)
+    ids = token_ids(g, 100, 40, torch.int64).to(DEV)
+    buf = torch.full((100, pitch), 7.0, dtype=dtype, device=DEV)
+    out = ops.embedding(ctx, table, ids, scale=1.0, out=buf[:, :16])
+    want = torch.where((ids >= 0)[:, None], table[ids.clamp_min(0)], 0.0)
+    assert torch.equal(out, want)
+    assert (buf[:, 16:] == 7.0).all()                      # what lies between the rows stays
+    dt = torch.full((40, pitch), 5.0, dtype=dtype, device=DEV)
+    ops.embedding_backward(ctx, dt[:, :16], out, ids)
+    assert (dt[:, 16:] == 5.0).all()
+    full = ops.embedding_backward(ctx, torch.empty(40, 16, dtype=dtype, device=DEV), out.contiguous(), ids)
+    assert torch.equal(dt[:, :16], full)
+
+
+def test_embedding_out_of_range_is_reported(ctx):
+    table = torch.ones(10, 8, device=DEV)
+    ids = torch.tensor([0, 9, 10, 1 << 40, -1], device=DEV)
+    out = ops.embedding(ctx, table, ids)
+    with pytest.raises(L.Sb200Error) as e:
+        ctx.check_device_status()
+    assert e.value.status == L.ERR_TOKEN_RANGE
+    assert out.sum(1).tolist() == [8, 8, 0, 0, 0]
+    ctx.check_device_status()                              # read once, then clear
+    dt = ops.embedding_backward(ctx, torch.empty(10, 8, device=DEV), torch.ones(5, 8, device=DEV), ids)
+    with pytest.raises(L.Sb200Error):
+        ctx.check_device_status()
+    assert dt.sum().item() == 16 and dt[0, 0] == 1 and dt[9, 0] == 1
+
+
+def grad_reference(dout, ids, vocab, scale):
+    keep = ids >= 0
+    want = torch.zeros(vocab, dout.shape[1], dtype=torch.float64)
+    size = torch.zeros(vocab, dout.shape[1], dtype=torch.float64)
+    count = torch.zeros(vocab, dtype=torch.float64)
+    at, d = ids[keep].long(), dout.cpu().double()[keep]
+    want.index_add_(0, at, d)
+    size.index_add_(0, at, d.abs())
+    count.index_add_(0, at, torch.ones(len(at), dtype=torch.float64))
+    return want * scale, size * abs(scale), count[:, None]
+
+
+@pytest.mark.parametrize("tt,ta", COMBOS)
+@pytest.mark.parametrize("n,vocab,cols,index", [(1, 1, 1, torch.int64), (7, 600, 7, torch.int32), (64, 100, 512, torch.int64),
+                                                (2049, 1000, 264, torch.int32), (5000, 513, 33, torch.int64),
+                                                (4100, 300000, 16, torch.int64), (700, 3, 2056, torch.int32)])
+def test_embedding_backward(ctx, tt, ta, n, vocab, cols, index):
+    g = gen(n + cols)
+    dout = randn(g, n, cols, dtype=ta)
+    ids = token_ids(g, n, vocab, index)
+    dt = torch.full((vocab, cols), float("nan"), dtype=tt, device=DEV)
+    ops.embedding_backward(ctx, dt, dout, ids.to(DEV), scale=0.5)
+    want, size, count = grad_reference(dout, ids, vocab, 0.5)
+    check(dt, want, (count + 2) * U * size + half_step(tt) * want.abs() * 1.001 + tiny(tt))
+    again = ops.embedding_backward(ctx, torch.empty_like(dt), dout, ids.to(DEV), scale=0.5)
+    assert torch.equal(again, dt)                          # fixed order of the sums
+    # accumulating: rows in use are added to, the others not written
+    before = randn(g, vocab, cols, dtype=tt)
+    acc = ops.embedding_backward(ctx, before.clone(), dout, ids.to(DEV), scale=-0.25, accumulate=True)
+    want, size, count = grad_reference(dout, ids, vocab, -0.25)
+    total = before.cpu().double() + want
+    check(acc, total, (count + 2) * U * (size + total.abs()) + half_step(tt) * total.abs() * 1.001 + tiny(tt))
+    idle = (count[:, 0] == 0).to(DEV)
+    assert torch.equal(acc[idle], before[idle])
+
+
+@pytest.mark.parametrize("n,distinct", [(20000, 1), (20000, 2), (70001, 3), (33000, 33000)])
+def test_embedding_backward_long_runs(ctx, n, distinct):
+    """Runs over many pieces, and none: one token number, a few, all different."""
+    g = gen(n)
+    ids = torch.randint(0, distinct, (n,), generator=g) if distinct < n else torch.randperm(n, generator=g)
+    dout = randn(g, n, 24)
+    dt = ops.embedding_backward(ctx, torch.empty(distinct, 24, device=DEV), dout, ids.to(DEV))
+    want, size, count = grad_reference(dout, ids, distinct, 1.0)
+    check(dt, want, (count + 2) * U * size)
+
+
+def test_embedding_backward_all_padding(ctx):
+    dt = torch.full((33, 12), float("nan"), device=DEV)
+    ids = torch.full((100,), -1, dtype=torch.int32, device=DEV)
+    ops.embedding_backward(ctx, dt, torch.full((100, 12), float("nan"), device=DEV), ids)
+    assert (dt == 0).all()
+    ops.embedding_backward(ctx, dt.fill_(3.0), torch.ones(0, 12, device=DEV), ids[:0])
+    assert (dt == 0).all()
+
+
+def test_embedding_padding_rows_are_not_read_into_sums(ctx):
+    """What stands in the gradient rows of padding (NaN, infinities) reaches nothing."""
+    ids = torch.tensor([0, -1, 1, -1, 0, 1, -7], device=DEV)
+    dout = torch.ones(7, 20, device=DEV)
+    dout[ids < 0] = torch.tensor([float("nan"), float("inf"), -float("inf")], device=DEV)[:, None]
+    dt = ops.embedding_backward(ctx, torch.empty(4, 20, device=DEV), dout, ids)
+    assert torch.equal(dt.cpu(), torch.tensor([2.0, 2.0, 0.0, 0.0])[:, None].expand(4, 20))
+
+
+# -------------------------------------------------------------------- layer norm
+
+LN_TYPES = [(F32, F32), (BF16, F32), (BF16, BF16), (F16, F32), (F16, F16)]
+LN_SHAPES = [(1, 1), (3, 2), (64, 512), (1000, 8), (37, 40), (17, 1000), (300, 4096), (5, 4001), (9, 8192), (4, 8200),
+             (3, 20000), (2500, 129)]
+
+
+def depth(cols):
+    """Additions a term of a row sum passes through: a thread's own, lanes, warps."""
+    return 16 + 5 + 16 + cols // 512
+
+
+def ln_reference(x, w, b, eps):
+    x = x.cpu().double()
+    mean = x.mean(-1, keepdim=True)
+    rstd = 1.0 / (x.var(-1, correction=0, keepdim=True) + eps).sqrt()
+    h = (x - mean) * rstd
+    w = torch.ones(x.shape[-1], dtype=torch.float64) if w is None else w.cpu().double()
+    b = torch.zeros(x.shape[-1], dtype=torch.float64) if b is None else b.cpu().double()
+    return x, mean, rstd, h, w, b
+
+
+@pytest.mark.parametrize("t,wt", LN_TYPES)
+@pytest.mark.parametrize("rows,cols", LN_SHAPES)
+def test_layer_norm(ctx, t, wt, rows, cols):
+    g = gen(rows * 31 + cols)
+    x = (randn(g, rows, cols) + 3.0 * randn(g, rows, 1)).to(t)
+    w, b = randn(g, cols, dtype=wt), randn(g, cols, dtype=wt)
+    eps = 1e-3
+    y, mean, rstd = ops.layer_norm(ctx, x, w, b, eps=eps)
+    x, m, r, h, w, b = ln_reference(x, w, b, eps)
+    D = depth(cols) + 8
+    dm = D * U * x.abs().mean(-1, keepdim=True)            # of the mean; enters the differences whole
+    check(mean, m[:, 0], dm[:, 0])
+    dr = (D * U + dm ** 2 * r ** 2) * r                    # the variance moves by the mean's error squared
+    check(rstd, r[:, 0], dr[:, 0])
+    want = h * w + b
+    tol = w.abs() * (r * dm + h.abs() * (dr / r + 4 * U)) + 4 * U * (b.abs() + want.abs())
+    check(y, want, tol + half_step(t) * (want.abs() + tol) * 1.001 + tiny(t))
+
+
+@pytest.mark.parametrize("t,wt", LN_TYPES)
+@pytest.mark.parametrize("rows,cols", LN_SHAPES)
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_layer_norm_backward(ctx, t, wt, rows, cols, accumulate):
+    g = gen(rows * 31 + cols)
+    x = (randn(g, rows, cols) + randn(g, rows, 1)).to(t)
+    dy, w = randn(g, rows, cols, dtype=t), randn(g, cols, dtype=wt)
+    _, mean, rstd = ops.layer_norm(ctx, x, w, None, eps=1e-3)
+    kw, dx0, dw0, db0 = {}, 0.0, 0.0, 0.0
+    if accumulate:
+        dx0, dw0, db0 = randn(g, rows, cols, dtype=t), randn(g, cols, dtype=wt), randn(g, cols, dtype=wt)
+        kw = dict(dx=dx0.clone(), dweight=dw0.clone(), dbias=db0.clone(), accumulate_dx=True, accumulate_weight=True)
+        dx0, dw0, db0 = dx0.cpu().double(), dw0.cpu().double(), db0.cpu().double()
+    dx, dw, db = ops.layer_norm_backward(ctx, dy, x, mean, rstd, w, **kw)
+    m, r = mean.cpu().double()[:, None], rstd.cpu().double()[:, None]       # the call's own inputs
+    dy, w = dy.cpu().double(), w.cpu().double()
+    h = (x.cpu().double() - m) * r
+    gw = dy * w
+    m1, m2 = gw.mean(-1, keepdim=True), (gw * h).mean(-1, keepdim=True)
+    want = r * (gw - m1 - h * m2) + dx0
+    D = (depth(cols) + 10) * U
+    size = r * (gw.abs() * 6 * U + D * gw.abs().mean(-1, keepdim=True) + h.abs() * (D * (gw * h).abs().mean(-1, keepdim=True)) +
+                6 * U * (m1.abs() + (h * m2).abs())) + 2 * U * want.abs()
+    check(dx, want, size + half_step(t) * (want.abs() + size) * 1.001 + tiny(t))
+    R = (rows + 70) * U
+    for got, terms, start in ((dw, dy * h, dw0), (db, dy, db0)):
+        total = terms.sum(0) + start
+        tol = (R + 4 * U) * terms.abs().sum(0) + 2 * U * total.abs()
+        check(got, total, tol + half_step(wt) * (total.abs() + tol) * 1.001 + tiny(wt))
+
+
+def test_layer_norm_backward_against_differences(ctx):
+    """sum(dy * y) has the gradients dx, dweight, dbias: central differences of the 64-bit definition."""
+    g = gen(5)
+    x, w, b, dy = randn(g, 6, 24), randn(g, 24), randn(g, 24), randn(g, 6, 24)
+    _, mean, rstd = ops.layer_norm(ctx, x, w, b)
+    grads = ops.layer_norm_backward(ctx, dy, x, mean, rstd, w)
+
+    def loss(x, w, b):
+        m = x.mean(-1, keepdim=True)
+        v = ((x - m) ** 2).mean(-1, keepdim=True)
+        return (dy.cpu().double() * ((x - m) / (v + 1e-5).sqrt() * w + b)).sum()
+
+    args = [t.cpu().double() for t in (x, w, b)]
+    step = 1e-5
+    for k, got in enumerate(grads):
+        want = torch.zeros_like(args[k]).reshape(-1)
+        for i in range(want.numel()):
+            moved = [[t.clone() for t in args] for _ in range(2)]
+            for sign, m in zip((1, -1), moved):
+                m[k].view(-1)[i] += sign * step
+            want[i] = (loss(*moved[0]) - loss(*moved[1])) / (2 * step)
+        # differences: step^2 times a third derivative (values here are of order 10) and 1e-16 / step of rounding
+        check(got.reshape(-1), want, 1e-5 * (1 + want.abs().max()))
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("cols,pitch,offset", [(16, 24, 0), (16, 19, 0), (512, 520, 1), (4096, 4104, 0), (4000, 4003, 2), (8200, 8208, 0)])
+def test_layer_norm_strides_and_in_place(ctx, t, cols, pitch, offset):
+    g = gen(cols)
+    x = randn(g, 21, cols, dtype=t, pitch=pitch, offset=offset)
+    dy = randn(g, 21, cols, dtype=t, pitch=pitch, offset=offset)
+    w, b = randn(g, cols), randn(g, cols)
+    y, mean, rstd = ops.layer_norm(ctx, x.contiguous(), w, b)
+    buf = torch.full((21, pitch), 7.0, dtype=t, device=DEV)
+    y2, mean2, rstd2 = ops.layer_norm(ctx, x, w, b, out=buf[:, :cols])
+    # another access width adds in another order: both are within the bound of the definition
+    D = depth(cols) + 8
+    off = 2 * D * U * (1 + x.double().abs().mean(-1, keepdim=True) * rstd[:, None].double())
+    wy = w.double().abs() * off * (1 + ((y.double() - b.double()) / w.double()).abs()) + 4 * U * (b.abs() + y.abs().double())
+    check(y2, y, wy + 2 * half_step(t) * y.double().abs() * 1.01 + tiny(t))
+    assert (buf[:, cols:] == 7.0).all()
+    x3 = x.contiguous()
+    y3, _, _ = ops.layer_norm(ctx, x3, w, b, out=x3)
+    assert y3.data_ptr() == x3.data_ptr() and torch.equal(y3, y)
+    dx, dw, db = ops.layer_norm_backward(ctx, dy.contiguous(), x.contiguous(), mean, rstd, w)
+    dy3 = dy.contiguous()
+    dx3, dw3, db3 = ops.layer_norm_backward(ctx, dy3, x.contiguous(), mean, rstd, w, dx=dy3)
+    assert torch.equal(dx3, dx) and torch.equal(dw3, dw) and torch.equal(db3, db)
+    buf.fill_(9.0)
+    ops.layer_norm_backward(ctx, dy, x, mean, rstd, w, dx=buf[:, :cols])
+    assert (buf[:, cols:] == 9.0).all()
+    scale = rstd.double()[:, None] * (w.double().abs() * dy.double().abs()).mean(-1, keepdim=True)
+    check(buf[:, :cols], dx, 64 * D * U * scale * (1 + ((x.double() - mean.double()[:, None]) * rstd.double()[:, None]).abs()) +
+          2 * half_step(t) * dx.double().abs() * 1.01 + 4 * U * dx.double().abs() + tiny(t))
+
+
+def test_layer_norm_without_weights_and_leading_dimensions(ctx):
+    g = gen(8)
+    x = randn(g, 12, 96).view(3, 4, 96)
+    y, mean, rstd = ops.layer_norm(ctx, x)
+    assert y.shape == x.shape and mean.shape == (3, 4)
+    one, zero = torch.ones(96, device=DEV), torch.zeros(96, device=DEV)
+    y1, _, _ = ops.layer_norm(ctx, x, one, zero)
+    assert torch.equal(y, y1)
+    a = ops.layer_norm_backward(ctx, y, x, mean, rstd)
+    b = ops.layer_norm_backward(ctx, y, x, mean, rstd, one)
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_layer_norm_constant_rows_and_bad_values(ctx):
+    """A row without variance gives the bias; a row with NaN or infinity stays its own affair."""
+    x = torch.full((4, 64), 5.0, device=DEV)
+    x[1] = torch.arange(64, device=DEV)
+    x[2, 7] = float("nan")
+    x[3, 9] = float("inf")
+    b = torch.arange(64, dtype=F32, device=DEV)
+    y, mean, rstd = ops.layer_norm(ctx, x, None, b)
+    assert torch.equal(y[0], b)
+    assert torch.isfinite(y[1]).all() and torch.isnan(y[2]).all() and torch.isnan(y[3]).all()
+    alone, _, _ = ops.layer_norm(ctx, x[1:2].contiguous(), None, b)
+    assert torch.equal(alone[0], y[1])
+
+
+def test_layer_norm_large_offsets(ctx):
+    """Rows far from zero: the variance comes from differences to the mean."""
+    g = gen(2)
+    x = randn(g, 16, 1024) * 0.5 + 1000.0
+    y, _, rstd = ops.layer_norm(ctx, x, eps=0.0)
+    _, m, r, h, _, _ = ln_reference(x, None, None, 0.0)
+    # the mean's error (depth x u x 1000) against a deviation of 0.5
+    tol = (depth(1024) + 8) * U * 1000.0 * r
+    check(y, h, tol * (1 + h.abs()) + 8 * U * h.abs())
+
+
+def test_layer_norm_no_rows(ctx):
+    dw, db = torch.full((16,), 3.0, device=DEV), torch.full((16,), 3.0, device=DEV)
+    empty, stat = torch.empty(0, 16, device=DEV), torch.empty(0, device=DEV)
+    ops.layer_norm(ctx, empty)
+    ops.layer_norm_backward(ctx, empty, empty, stat, stat, dweight=dw, dbias=db, dx=empty, accumulate_weight=True)
+    assert (dw == 3).all() and (db == 3).all()
+    ops.layer_norm_backward(ctx, empty, empty, stat, stat, dweight=dw, dbias=db)
+    assert (dw == 0).all() and (db == 0).all()
+
+
+# ----------------------------------------------------------------- orthogonalize
+
+COEF = (3.4445, -4.7750, 2.0315)
+
+
+def ns_reference(g, steps=5, coef=COEF, eps=1e-7):
+    a, b, c = coef
+    x = g.cpu().double()
+    tall = x.shape[-2] > x.shape[-1]
+    x = x.mT if tall else x
+    x = x / (x.square().sum((-2, -1), keepdim=True).sqrt() + eps)
+    for _ in range(steps):
+        m = x @ x.mT
+        x = a * x + (b * m + c * (m @ m)) @ x
+    return x.mT if tall else x
+
+
+def ns_tolerance(t, steps=5):
+    """Relative, 2-norm.  The operands' roundings, three matrices a step, carried along
+    (a step multiplies an error in a direction by no more than it multiplies the direction
+    itself, about), then the result's own.  Two parts: 22 bits and chains of 24 cut
+    additions, a few u each: 1e-5 is the bar of the library's other fp32-accurate products."""
+    if t == BF16:
+        return steps * 3 * 2.0 ** -12 + half_step(t)
+    return 1e-5 + (half_step(t) if t == F16 else 0.0)
+
+
+def rel(got, want):
+    got, want = got.cpu().double(), want.cpu().double()
+    return float((got - want).norm() / want.norm())
+
+
+def gradient(g, *shape, dtype=F32):
+    """A few strong directions over noise, small values as gradients have them."""
+    rows, cols = shape[-2:]
+    rank = max(1, min(rows, cols) // 8)
+    x = torch.randn(*shape[:-1], rank, generator=g) @ torch.randn(*shape[:-2], rank, cols, generator=g) / rank ** 0.5
+    return ((x + 0.3 * torch.randn(*shape, generator=g)) * 1e-3).to(dtype).to(DEV)
+
+
+NS_SHAPES = [(1, 1), (1, 7), (5, 3), (10, 256), (64, 64), (65, 127), (128, 128), (129, 300), (784, 512), (256, 1000),
+             (640, 640), (1, 5000), (1300, 260)]
+
+
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+@pytest.mark.parametrize("rows,cols", NS_SHAPES)
+def test_orthogonalize(ctx, t, rows, cols):
+    g = gradient(gen(rows + 7 * cols), rows, cols, dtype=t)
+    out = ops.orthogonalize(ctx, g)
+    ctx.check_device_status()
+    assert rel(out, ns_reference(g)) <= ns_tolerance(t)
+    assert torch.equal(ops.orthogonalize(ctx, g), out)
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("batch,rows,cols", [(3, 100, 60), (2, 300, 700), (9, 512, 512), (5, 33, 33), (3, 1300, 1024)])
+def test_orthogonalize_batches(ctx, t, batch, rows, cols):
+    """Every matrix of a batch as alone; the larger ones take tiles of 256 on pairs of SMs."""
+    g = gradient(gen(batch), batch, rows, cols, dtype=t)
+    out = ops.orthogonalize(ctx, g)
+    ctx.check_device_status()
+    for k in range(batch):
+        assert rel(out[k], ns_reference(g[k])) <= ns_tolerance(t)
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("rows,cols", [(2500, 2300), (2048, 4096)])
+def test_orthogonalize_large(ctx, t, rows, cols):
+    g = gradient(gen(rows), rows, cols, dtype=t)
+    out = ops.orthogonalize(ctx, g)
+    ctx.check_device_status()
+    want = g.double()
+    x = want.mT if rows > cols else want
+    x = x / (x.norm() + 1e-7)
+    for _ in range(5):
+        m = x @ x.mT
+        x = COEF[0] * x + (COEF[1] * m + COEF[2] * (m @ m)) @ x
+    assert rel(out, x.mT if rows > cols else x) <= ns_tolerance(t)
+
+
+def test_orthogonalize_strides_steps_and_in_place(ctx):
+    g = gen(4)
+    wide = gradient(g, 90, 200)
+    for view in (wide[:, :120], wide[:, 3:124], wide[:60, 5:]):
+        out = torch.full((view.shape[0], 211), 2.0, device=DEV)
+        got = ops.orthogonalize(ctx, view, out=out[:, 1:1 + view.shape[1]])
+        assert rel(got, ns_reference(view)) <= ns_tolerance(F32)
+        assert (out[:, 0] == 2).all() and (out[:, 1 + view.shape[1]:] == 2).all()
+    for steps, coef in ((1, COEF), (2, COEF), (12, (1.5, -0.5, 0.0))):
+        got = ops.orthogonalize(ctx, wide, steps=steps, coefficients=coef)
+        assert rel(got, ns_reference(wide, steps, coef)) <= ns_tolerance(F32, steps)
+    want = ops.orthogonalize(ctx, wide)
+    same = wide.clone()
+    assert torch.equal(ops.orthogonalize(ctx, same, out=same), want)
+    batch = gradient(g, 4, 50, 70)
+    got = ops.orthogonalize(ctx, batch[::2])
+    assert torch.equal(got[1], ops.orthogonalize(ctx, batch[2]))
+
+
+def test_orthogonalize_range_of_inputs(ctx):
+    """Magnitudes at both ends of fp32, zero, and values that are not finite."""
+    g = gradient(gen(6), 40, 70)
+    want = ops.orthogonalize(ctx, g, eps=0.0)
+    for power in (-90, 100):                               # a power of two changes nothing
+        assert torch.equal(ops.orthogonalize(ctx, g * 2.0 ** power, eps=0.0), want)
+    assert (ops.orthogonalize(ctx, torch.zeros(30, 20, device=DEV)) == 0).all()
+    bad = g.clone()
+    bad[3, 5] = float("nan")
+    assert torch.isnan(ops.orthogonalize(ctx, bad)).all()
+
+
+def test_orthogonalize_bounded_waits(ctx):
+    """The waits of both kernels run out, the status says so and the context goes on."""
+    small, large = gradient(gen(1), 130, 300), gradient(gen(2), 2300, 2300)
+    want = ops.orthogonalize(ctx, small)
+    ctx.check_device_status()
+    ctx.set_option(L.OPT_WAIT_LIMIT_US, 2000)
+    ctx.set_option(L.OPT_TEST_STALL_KBLOCKS, 1)
+    try:
+        for g in (small, large):
+            ops.orthogonalize(ctx, g, steps=1)
+            with pytest.raises(L.Sb200Error) as e:
+                ctx.check_device_status()
+            assert e.value.status == L.ERR_DEVICE_TIMEOUT
+    finally:
+        ctx.set_option(L.OPT_TEST_STALL_KBLOCKS, -1)
+        ctx.set_option(L.OPT_WAIT_LIMIT_US, 2000000)
+    assert torch.equal(ops.orthogonalize(ctx, small), want)
+
+
+# ----------------------------------------------------------- streams and graphs
+
+def test_other_streams_and_captured_graphs(ctx):
+    """The calls on another stream than the tensors', and two captured graphs that share
+    one context, replayed in turn after larger calls have run."""
+    g = gen(11)
+    table, ids = randn(g, 50, 64), token_ids(g, 200, 50, torch.int64).to(DEV)
+    dout, x, w, b = randn(g, 200, 64), randn(g, 200, 64), randn(g, 64), randn(g, 64)
+    m = gradient(g, 70, 40)
+
+    def step(k):
+        e = ops.embedding(ctx, table, ids, scale=2.0)
+        y, mean, rstd = ops.layer_norm(ctx, e + x * k, w, b)
+        dx, dw, db = ops.layer_norm_backward(ctx, dout, e + x * k, mean, rstd, w)
+        dt = ops.embedding_backward(ctx, torch.empty_like(table), dx, ids, scale=2.0)
+        return [e, y, dx, dw, db, dt, ops.orthogonalize(ctx, m * k)]
+
+    want = {k: [t.clone() for t in step(k)] for k in (1, 3)}
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = step(1)
+    side.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(got, want[1]))
+    graphs, outs = {}, {}
+    for k in (1, 3):
+        graphs[k] = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graphs[k]):
+            outs[k] = step(k)
+    big = randn(g, 3000, 512)
+    ops.layer_norm_backward(ctx, big, big, torch.zeros(3000, device=DEV), torch.ones(3000, device=DEV))
+    ops.orthogonalize(ctx, big)
+    for k in (3, 1, 3, 1):
+        for t in outs[k]:
+            t.fill_(float("nan"))
+        graphs[k].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(outs[k], want[k]))
+
+
+# ------------------------------------------------------------ a run of them together
+
+def test_training_step_of_a_token_model(ctx):
+    """Embedding, layer norm, Linear, softmax cross-entropy, and back: every gradient and
+    the updated parameters against autograd in 64 bits.  The matrix weight takes the
+    orthogonalised update, the vectors and the table SGD."""
+    g = gen(21)
+    vocab, width, classes, n, lr = 300, 96, 52, 257, 0.02
+    table, W = randn(g, vocab, width) * 0.1, randn(g, width, classes) * 0.1
+    bias, lw, lb = randn(g, classes) * 0.1, 1 + 0.1 * randn(g, width), 0.1 * randn(g, width)
+    ids = token_ids(g, n, vocab, torch.int64).to(DEV)
+    target = torch.randint(0, classes, (n,), generator=g).to(DEV)
+    onehot = torch.nn.functional.one_hot(target, classes).float()
+    scale = width ** 0.5
+
+    e = ops.embedding(ctx, table, ids, scale=scale)
+    y, mean, rstd = ops.layer_norm(ctx, e, lw, lb)
+    logits = ops.gemm(ctx, y, W, bias=bias, mode=L.MODE_TF32X3)
+    _, loss, dlogits = ops.softmax_cross_entropy(ctx, logits, onehot)
+    dy = ops.gemm(ctx, dlogits, W, trans_b=True, mode=L.MODE_TF32X3)
+    dbias = torch.empty(classes, device=DEV)
+    dW = ops.gemm(ctx, y, dlogits, trans_a=True, mode=L.MODE_TF32X3, colsum_out=dbias)
+    de, dlw, dlb = ops.layer_norm_backward(ctx, dy, e, mean, rstd, lw)
+    dtable = ops.embedding_backward(ctx, torch.empty_like(table), de, ids, scale=scale)
+
+    p = [t.cpu().double().requires_grad_() for t in (table, lw, lb, W, bias)]
+    rows = p[0][ids.cpu().clamp_min(0)] * (ids.cpu() >= 0)[:, None] * scale
+    out = torch.nn.functional.layer_norm(rows, (width,), p[1], p[2], 1e-5) @ p[3] + p[4]
+    want_loss = torch.nn.functional.cross_entropy(out, target.cpu(), reduction="none")
+    want_loss.sum().backward()
+    # the products are good to 1e-5, the sums around them to a few u: one bar for all
+    assert rel(loss, want_loss.detach()) <= 3e-5
+    for got, want in zip((dtable, dlw, dlb, dW, dbias), p):
+        assert rel(got, want.grad) <= 3e-5
+    # padding rows are constant (zero): their layer norm has rstd = eps^-1/2 and their gradient goes nowhere
+
+    new_W = ops.sgd_update(ctx, W.clone(), ops.orthogonalize(ctx, dW), lr)
+    want_W = p[3].detach() - lr * ns_reference(p[3].grad)
+    assert rel(new_W, want_W) <= 3e-5
+    new_table = ops.embedding_backward(ctx, table.clone(), de, ids, scale=-lr * scale, accumulate=True)
+    assert rel(new_table, p[0].detach() - lr * p[0].grad) <= 3e-5
