@@ -1,0 +1,1043 @@
+// Orthogonalised update of a matrix (Newton-Schulz products):
+//
+//   X = G / (|G|_F + eps), then `steps` times
+//   A = X X^T,   B = b A + c A A,   X = a X + B X
+//
+// on the shorter side of G (a tall G is worked on transposed, so X is R x C with R <= C).
+//
+// All products run on the tensor cores with fp16 operands and fp32 accumulators.  The
+// singular values of every matrix in the iteration are bounded (the host checks the
+// bound for the given coefficients), so the matrices are kept as fp16 numbers scaled by
+// 2^13, which cannot overflow and keeps small entries out of the subnormal range.
+//
+//   fp32 and fp16 input: every matrix is a sum of two fp16 parts, hi = fp16(x) and
+//     lo = fp16(x - hi), 22 bits of mantissa.  A product is hi.lo + lo.hi + hi.hi, three
+//     tensor-core products at the fp16 rate (a product of two TF32 parts would run at half
+//     of it).  The tensor core cuts its fp32 accumulation short instead of rounding it,
+//     so a chain of accumulations ends after CHUNK_KB k-blocks and the chains are added
+//     in registers.
+//   bf16 input: the products take the hi parts alone (11 bits; the result keeps 8).
+//     X still has both parts and the a X term uses both: rounding X itself every step
+//     would feed the small singular directions, which a step multiplies by a, with the
+//     rounding errors of the large ones.
+//
+// A and A A are symmetric: only tiles on and above the diagonal are computed, and a tile
+// above it is also stored transposed.  X X^T and A A read both operands along k; B X reads
+// X in rows of k ("MN-major"), so no matrix is ever transposed in memory.
+#include <cmath>
+#include <type_traits>
+
+#include "/root/repo/sapphire_b200/csrc/gemm_common.cuh"
+#include "/root/repo/sapphire_b200/csrc/typed.cuh"
+
+__device__ unsigned long long dbg_t[4096*16];
+__device__ unsigned dbg_n;
+namespace sb200 {
+
+using namespace gemm;
+
+namespace {
+#define STAMP(k) do{ if(blockIdx.x==0 && p.launch_no<4096) dbg_t[p.launch_no*16+(k)]=ptx::globaltimer_ns(); }while(0)
+constexpr int KB = 64;                           // fp16 elements of k per block: one 128-byte swizzle row
+constexpr int MMA_K = 16;
+constexpr int TILE_BYTES = 128 * KB * 2;         // 128 rows (or columns) x 64 k
+constexpr int MN_CHUNK_BYTES = 64 * KB * 2;      // MN-major: 64 k rows x 64 columns
+constexpr int CHUNK_KB = 2;                      // k-blocks per accumulation chain with two parts
+constexpr float SCALE = 8192.0f;                 // 2^13
+constexpr float INV_SCALE = 1.0f / 8192.0f;
+constexpr double LARGEST = 7.5;                  // of a singular value: 7.5 * 2^13 < 65504
+constexpr int EPI_WARPS = 8;
+constexpr int THREADS = 64 + EPI_WARPS * 32;
+constexpr int NORM_BLOCKS = 512;                 // partial sums of squares per matrix
+constexpr int ORTH_PANEL = 8;
+constexpr int MAX_SLICES = 8;
+constexpr int PART_LD = 132;                     // floats per row of a partial tile in shared memory
+
+enum Product { GRAM, POLY, APPLY };
+
+// A matrix of the iteration: [parts][batch][rows][ld] fp16, part 0 = hi, 1 = lo.
+struct Split {
+    f16* p;
+    int64_t ld, batch_stride, part_stride;
+};
+
+struct OrthParams {
+    int R, C, batch;
+    int rows, cols, num_kb;                      // of the product
+    int tiles_m, tiles_n, tiles;                 // per matrix
+    int chunk_kb, slices;
+    Split prev, out;                             // prev: added with `coef`; out: the result
+    int out_parts, prev_parts;
+    float coef, alpha;                           // result = coef * prev + alpha * accumulator (scaled by 2^13)
+    void* final_out;                             // APPLY, last step: the caller's matrix
+    int64_t final_ld, final_stride;
+    int final_type, tall, final_vec;
+    unsigned* status;
+    unsigned long long wait_limit_ns;
+    int test_stall_kb;
+    int launch_no;
+};
+
+// The epilogue of the pair kernel moves 32 x 32 blocks of both parts through shared memory
+// (rows of 64 bytes, their 16-byte pieces permuted against bank conflicts): a thread owns a
+// row of the accumulator, and 32 rows a warp touched with plain 16-byte accesses cost 32
+// cycles of the load/store unit each (an epilogue of 24 us where the products take 5);
+// through shared memory four lanes share a row.  TMA would do the same, but it is what
+// feeds the tensor core: blocks moved by TMA made the operand tiles late (9.6 us a tile).
+constexpr int EPI_PART_BYTES = 32 * 32 * 2;
+constexpr int EPI_BUF_BYTES = 2 * EPI_PART_BYTES;
+
+template <bool SPLIT>
+struct OrthSmem {
+    static constexpr int PARTS = SPLIT ? 2 : 1;
+    static constexpr int STAGE = 2 * PARTS * TILE_BYTES;
+    static constexpr int STAGES = SPLIT ? 3 : 5;
+    static constexpr int TILES = STAGE * STAGES;
+    static constexpr int BUFS = SPLIT ? 1 : 2;   // epilogue buffers per warp
+    static constexpr int EPI = EPI_WARPS * BUFS * EPI_BUF_BYTES;
+    static constexpr int BARS = ((2 * STAGES + 4) * 8 + 16 + 15) & ~15;
+    static constexpr int TOTAL = TILES + EPI + BARS + 1024;
+    static_assert(TOTAL <= 227 * 1024, "shared memory per CTA");
+    static_assert(TILES >= 128 * PART_LD * 4 + 128 * 129 * 4, "what the sliced kernel keeps in the place of the stages");
+};
+
+// Tile t of a matrix; symmetric products walk over the tiles with tn >= tm only.
+__device__ __forceinline__ void orth_tile(int t, const OrthParams& p, bool symmetric, int& tm, int& tn)
+{
+    if (!symmetric) {
+        tile_coords(t, p.tiles_m, p.tiles_n, ORTH_PANEL, tm, tn);
+        return;
+    }
+    int row = 0, len = p.tiles_n;
+    while (t >= len) {
+        t -= len;
+        ++row;
+        --len;
+    }
+    tm = row;
+    tn = row + t;
+}
+
+__device__ __forceinline__ void split_f16(const float (&v)[8], Raw<f16, 8>& hi, Raw<f16, 8>& lo)
+{
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        hi.e[e] = __float2half_rn(v[e]);
+        lo.e[e] = __float2half_rn(v[e] - __half2float(hi.e[e]));
+    }
+}
+
+__device__ __forceinline__ void store_transposed(const Raw<f16, 8>& hi, const Raw<f16, 8>& lo, f16* out, const Split& m,
+                                                 int parts, int row, int col, int cols)
+{
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        if (col + e < cols) {                    // lanes hold neighbouring rows: contiguous in the output
+            f16* o = out + static_cast<int64_t>(col + e) * m.ld + row;
+            *o = hi.e[e];
+            if (parts == 2) o[m.part_stride] = lo.e[e];
+        }
+    }
+}
+
+template <typename F>
+__device__ __forceinline__ void with_final_type(const OrthParams& p, int b, F f)
+{
+    const int64_t at = b * p.final_stride;
+    if (p.final_type == SB200_F32) f(static_cast<float*>(p.final_out) + at);
+    else if (p.final_type == SB200_BF16) f(static_cast<bf16*>(p.final_out) + at);
+    else f(static_cast<f16*>(p.final_out) + at);
+}
+
+// One warp's 32 x 32 block of the caller's matrix, stored by rows.  v: this lane's row.
+// buf: 4 KB of shared memory nobody else uses; 16-byte pieces of a row are permuted so that
+// neither side has bank conflicts.
+template <typename T>
+__device__ __forceinline__ void final_block(T* out, const OrthParams& p, uint8_t* buf, int row0, int col0,
+                                            const float (&v)[32])
+{
+    constexpr int PER = 16 / static_cast<int>(sizeof(T));        // elements of a piece
+    constexpr int PIECES = 32 / PER;                             // pieces of a row
+    const int lane = threadIdx.x & 31;
+    auto place = [](int r, int piece) { return PIECES == 8 ? piece ^ (r & 7) : piece ^ ((r >> 1) & 3); };
+    __syncwarp();
+#pragma unroll
+    for (int c = 0; c < PIECES; ++c) {
+        Raw<T, PER> x;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) x.e[e] = from_f<T>(v[c * PER + e]);
+        store_raw<false>(reinterpret_cast<T*>(buf) + lane * 32 + place(lane, c) * PER, x);
+    }
+    __syncwarp();
+    if (p.final_vec && col0 + 32 <= p.C) {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int r = i * (32 / PIECES) + lane / PIECES, c = lane % PIECES;
+            Raw<T, PER> x;
+            load_raw<false>(x, reinterpret_cast<const T*>(buf) + r * 32 + place(r, c) * PER);
+            if (row0 + r < p.R) store_raw<true>(out + static_cast<int64_t>(row0 + r) * p.final_ld + col0 + c * PER, x);
+        }
+    } else {
+        for (int r = 0; r < 32 && row0 + r < p.R; ++r)
+            if (col0 + lane < p.C)
+                out[static_cast<int64_t>(row0 + r) * p.final_ld + col0 + lane] =
+                    reinterpret_cast<const T*>(buf)[r * 32 + place(r, lane / PER) * PER + lane % PER];
+    }
+    __syncwarp();
+}
+
+// PAIR: a cluster of two CTAs per 256 x 256 tile (cta_group::2), clusters walk over the
+// tiles.  Otherwise: a cluster of p.slices CTAs per 128 x 128 tile, each with its slice of
+// the k-blocks; the partial tiles meet in shared memory, and each CTA finishes its share
+// of the columns.
+template <int WHAT, bool PAIR, bool SPLIT>
+__global__ void __launch_bounds__(THREADS, 1)
+orth_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                    const OrthParams p)
+{
+    using S = OrthSmem<SPLIT>;
+    constexpr bool SYMMETRIC = WHAT != APPLY;
+    constexpr bool B_MN = WHAT == APPLY;
+    constexpr int CTAS = PAIR ? 2 : 1;
+    constexpr int BM = 128 * CTAS, BN = 128 * CTAS;
+    constexpr int COLS = BN / 2;                 // accumulator columns of an epilogue warp
+    constexpr uint32_t TMEM_COLS = 2 * BN;
+
+    if(threadIdx.x==0) STAMP(0);
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>(
+        (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    uint8_t* epi = smem + S::TILES;
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(epi + S::EPI);
+    uint64_t* empty_bar = full_bar + S::STAGES;
+    uint64_t* tmem_full = empty_bar + S::STAGES;
+    uint64_t* tmem_empty = tmem_full + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_empty + 2);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const uint32_t rank = ptx::cluster_ctarank();
+    const Abort ab{abort_flag, p.status, p.wait_limit_ns};
+
+    auto wait = [&](uint64_t* bar, uint32_t parity, unsigned code) {
+        if (!PAIR) return wait_bar(bar, parity, ab, code);
+        return wait_bar_cluster(bar, parity, ab, code);
+    };
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S::STAGES; ++s) {
+            ptx::mbar_init(&full_bar[s], 1);
+            ptx::mbar_init(&empty_bar[s], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            ptx::mbar_init(&tmem_full[i], 1);
+            ptx::mbar_init(&tmem_empty[i], EPI_WARPS * CTAS);
+        }
+        *abort_flag = 0;
+        ptx::fence_mbar_init();
+        ptx::prefetch_tensormap(&map_a);
+        ptx::prefetch_tensormap(&map_b);
+    }
+    if (warp == 1) {
+        if (PAIR) {
+            ptx::tmem_alloc_pair(tmem_slot, TMEM_COLS);
+            ptx::tmem_relinquish_pair();
+        } else {
+            ptx::tmem_alloc(tmem_slot, TMEM_COLS);
+            ptx::tmem_relinquish();
+        }
+    }
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    if (PAIR) ptx::cluster_sync();
+    ptx::tc_fence_after_sync();
+    const uint32_t tmem_base = *tmem_slot;
+    if(threadIdx.x==0) STAMP(1);
+    ptx::griddep_launch_dependents();
+    ptx::griddep_wait();
+    if(threadIdx.x==0) STAMP(2);
+
+    const int group = PAIR ? 2 : p.slices;       // CTAs of the cluster
+    const int unit = blockIdx.x / group;
+    const int units = gridDim.x / group;
+    const int total = p.tiles * p.batch;
+    // this CTA's k-blocks
+    const int per_slice = PAIR ? p.num_kb : (p.num_kb + p.slices - 1) / p.slices;
+    const int kb_first = PAIR ? 0 : min(p.num_kb, static_cast<int>(rank) * per_slice);
+    const int kb_last = PAIR ? p.num_kb : min(p.num_kb, kb_first + per_slice);
+    const uint32_t pair_rank = PAIR ? rank : 0u;
+
+    if (warp == 0) {
+        // ------------------------------------------------------ TMA producer
+        if (lane == 0) {
+            int s = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            int issued = 0;
+            for (int t = unit; ok && t < total; t += units) {
+                const int b = t / p.tiles;
+                int tm, tn;
+                orth_tile(t % p.tiles, p, SYMMETRIC, tm, tn);
+                const int m0 = tm * BM + static_cast<int>(pair_rank) * 128;
+                const int n0 = tn * BN + static_cast<int>(pair_rank) * 128;
+                for (int kb = kb_first; kb < kb_last; ++kb) {
+                    if (p.test_stall_kb >= 0 && issued++ >= p.test_stall_kb) {
+                        ok = false;              // test hook: the other roles' waits run out
+                        break;
+                    }
+                    if (!(ok = wait(&empty_bar[s], ph ^ 1u, FAULT_PRODUCER_WAIT))) break;
+                    uint8_t* st = smem + s * S::STAGE;
+                    const int k0 = kb * KB;
+                    if (pair_rank == 0) ptx::mbar_arrive_expect_tx(&full_bar[s], CTAS * S::STAGE);
+                    const uint32_t lead = PAIR ? ptx::map_to_cta(ptx::smem_u32(&full_bar[s]), 0) : 0u;
+                    auto load = [&](uint8_t* dst, const CUtensorMap* map, int x, int y, int z) {
+                        if (PAIR) ptx::tma_load_3d_pair(dst, map, lead, x, y, z);
+                        else ptx::tma_load_3d(dst, map, &full_bar[s], x, y, z);
+                    };
+#pragma unroll
+                    for (int part = 0; part < S::PARTS; ++part) {
+                        const int z = part * p.batch + b;
+                        uint8_t* sa = st + part * TILE_BYTES;
+                        uint8_t* sb = st + (S::PARTS + part) * TILE_BYTES;
+                        load(sa, &map_a, k0, m0, z);
+                        if (B_MN) {
+                            load(sb, &map_b, n0, k0, z);
+                            load(sb + MN_CHUNK_BYTES, &map_b, n0 + 64, k0, z);
+                        } else {
+                            load(sb, &map_b, k0, n0, z);
+                        }
+                    }
+                    if (++s == S::STAGES) {
+                        s = 0;
+                        ph ^= 1u;
+                    }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // ------------------------------------- MMA issuer (a pair's leader only)
+        if (lane == 0 && pair_rank == 0) {
+            constexpr uint32_t idesc = ptx::make_idesc_f16(BM, BN, 0, B_MN);
+            constexpr uint32_t A_STEP = MMA_K * 2, B_STEP = B_MN ? MMA_K * 128u : MMA_K * 2u;
+            constexpr uint32_t B_LBO = B_MN ? MN_CHUNK_BYTES : 16u;
+            int s = 0;
+            uint32_t ph = 0;
+            int acc = 0;
+            uint32_t acc_ph = 0;
+            bool ok = true;
+            for (int t = unit; ok && t < total; t += units) {
+                for (int kb0 = kb_first; ok && kb0 < kb_last; kb0 += p.chunk_kb) {
+                    if (!(ok = wait(&tmem_empty[acc], acc_ph ^ 1u, FAULT_MMA_WAIT_TMEM))) break;
+                    ptx::tc_fence_after_sync();
+                    const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BN);
+                    const int kb1 = min(kb0 + p.chunk_kb, kb_last);
+                    for (int kb = kb0; kb < kb1; ++kb) {
+                        if (!(ok = wait(&full_bar[s], ph, FAULT_MMA_WAIT_FULL))) break;
+                        if(kb==kb_first) STAMP(3);
+                        ptx::tc_fence_after_sync();
+                        const uint32_t sa = ptx::smem_u32(smem + s * S::STAGE);
+                        const uint32_t sb = sa + S::PARTS * TILE_BYTES;
+#pragma unroll
+                        for (int pass = 0; pass < (SPLIT ? 3 : 1); ++pass) {
+                            // hi.lo, lo.hi, hi.hi: small terms first
+                            const uint32_t pa = sa + (SPLIT && pass == 1 ? TILE_BYTES : 0);
+                            const uint32_t pb = sb + (SPLIT && pass == 0 ? TILE_BYTES : 0);
+#pragma unroll
+                            for (int k = 0; k < KB / MMA_K; ++k) {
+                                const uint64_t da = ptx::make_smem_desc(pa + k * A_STEP, 16u, 1024u, ptx::LAYOUT_SW128);
+                                const uint64_t db = ptx::make_smem_desc(pb + k * B_STEP, B_LBO, 1024u, ptx::LAYOUT_SW128);
+                                const uint32_t more = (kb > kb0 || pass > 0 || k > 0) ? 1u : 0u;
+                                if (PAIR) ptx::mma_f16_pair(d, da, db, idesc, more);
+                                else ptx::mma_f16(d, da, db, idesc, more);
+                            }
+                        }
+                        if (PAIR) ptx::mma_commit_pair(&empty_bar[s], 3);
+                        else ptx::mma_commit(&empty_bar[s]);
+                        if (++s == S::STAGES) {
+                            s = 0;
+                            ph ^= 1u;
+                        }
+                    }
+                    if (!ok) break;
+                    if (PAIR) ptx::mma_commit_pair(&tmem_full[acc], 3);
+                    else ptx::mma_commit(&tmem_full[acc]);
+                    acc ^= 1;
+                    if (acc == 0) acc_ph ^= 1u;
+                }
+            }
+        }
+    } else {
+        // ---------------------------------------------------------- epilogue
+        // warp w reads TMEM lanes 32 (w % 4) .. + 31 and one half of the columns
+        const int q = warp & 3, half = (warp - 2) >> 2;
+        const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(half * COLS);
+        uint8_t* bufs = epi + (warp - 2) * S::BUFS * EPI_BUF_BYTES;
+        int acc = 0;
+        uint32_t acc_ph = 0;
+        bool ok = true;
+        auto release = [&]() {                   // this accumulator is read: on to the other
+            ptx::tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) {
+                if (PAIR) ptx::mbar_arrive_cluster(ptx::map_to_cta(ptx::smem_u32(&tmem_empty[acc]), 0));
+                else ptx::mbar_arrive(&tmem_empty[acc]);
+            }
+            acc ^= 1;
+            if (acc == 0) acc_ph ^= 1u;
+        };
+        for (int t = unit; ok && t < total; t += units) {
+            const int b = t / p.tiles;
+            int tm, tn;
+            orth_tile(t % p.tiles, p, SYMMETRIC, tm, tn);
+            const int row0 = tm * BM + static_cast<int>(pair_rank) * 128 + q * 32;
+            const int col0 = tn * BN + half * COLS;
+            // blocks of 32 columns this warp has to finish; none where its rows or columns are beyond the matrix
+            const int blocks = row0 < p.rows && col0 < p.cols ? min(COLS, p.cols - col0 + 31) / 32 : 0;
+            // 16-byte piece c of row r of a block
+            auto place = [&](int k, int part, int r, int c) {
+                return reinterpret_cast<f16*>(bufs + k * EPI_BUF_BYTES + part * EPI_PART_BYTES + r * 64 +
+                                              ((c ^ ((r >> 1) & 3)) << 4));
+            };
+            auto fetch = [&](int i) {            // block i of prev into its buffer: four lanes a row
+                const f16* src = p.prev.p + b * p.prev.batch_stride + col0 + i * 32 + (lane & 3) * 8;
+                for (int part = 0; part < p.prev_parts; ++part) {
+#pragma unroll
+                    for (int it = 0; it < 4; ++it) {
+                        const int r = it * 8 + (lane >> 2);
+                        const bool in = row0 + r < p.rows;       // (the pitch covers whole blocks of columns)
+                        ptx::cp_async_16(place(i % S::BUFS, part, r, lane & 3),
+                                         in ? src + part * p.prev.part_stride + static_cast<int64_t>(row0 + r) * p.prev.ld : src,
+                                         in ? 16 : 0);
+                    }
+                }
+            };
+            if constexpr (PAIR && WHAT != GRAM) {
+                // the first blocks of prev travel while the products run; one group a block
+#pragma unroll
+                for (int i = 0; i < S::BUFS; ++i) {
+                    if (i < blocks) fetch(i);
+                    ptx::cp_async_commit();
+                }
+            }
+            if (SPLIT || !PAIR) {
+                // chains of accumulations are added here, rounded to nearest
+                float sum[COLS];
+#pragma unroll
+                for (int j = 0; j < COLS; ++j) sum[j] = 0.0f;
+                for (int kb0 = kb_first; kb0 < kb_last; kb0 += p.chunk_kb) {
+                    if (!(ok = wait(&tmem_full[acc], acc_ph, FAULT_EPI_WAIT))) break;
+                if(threadIdx.x==64) STAMP(4);
+                    ptx::tc_fence_after_sync();
+#pragma unroll
+                    for (int c = 0; c < COLS / 32; ++c) {
+                        uint32_t v[32];
+                        ptx::tmem_ld_32x32(lane_base + static_cast<uint32_t>(acc * BN + c * 32), v);
+                        ptx::tmem_ld_wait();
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) sum[c * 32 + j] = __fadd_rn(sum[c * 32 + j], __uint_as_float(v[j]));
+                    }
+                    if (PAIR && kb0 + p.chunk_kb >= kb_last) break;
+                    release();
+                }
+                if (!ok) break;
+                if constexpr (PAIR) {
+                    // the total goes back into the last accumulator, for the loop over the blocks:
+                    // unrolled over 128 registers that loop spilled, and its code, run once a tile,
+                    // came from beyond the instruction cache
+#pragma unroll
+                    for (int c = 0; c < COLS / 32; ++c) {
+                        uint32_t v[32];
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(sum[c * 32 + j]);
+                        ptx::tmem_st_32x32(lane_base + static_cast<uint32_t>(acc * BN + c * 32), v);
+                    }
+                    ptx::tmem_st_wait();
+                } else {
+                    // every role of this CTA is done with the stages (the last product has read
+                    // them): the partial tile goes there
+                    float* part = reinterpret_cast<float*>(smem) + (q * 32 + lane) * PART_LD + half * COLS;
+#pragma unroll
+                    for (int j = 0; j < COLS; j += 4)
+                        *reinterpret_cast<float4*>(part + j) = make_float4(sum[j], sum[j + 1], sum[j + 2], sum[j + 3]);
+                }
+            } else {
+                if (!(ok = wait(&tmem_full[acc], acc_ph, FAULT_EPI_WAIT))) break;
+                ptx::tc_fence_after_sync();
+            }
+            if constexpr (!PAIR) continue;       // (one tile a cluster: the rest is below)
+            f16* out = p.out.p + b * p.out.batch_stride;
+            const bool mirror = SYMMETRIC && tn > tm;            // (all rows of such a tile are in the matrix)
+#pragma unroll 1
+            for (int i = 0; i < blocks; ++i) {
+                const int k = i % S::BUFS;
+                const int col = col0 + i * 32;
+                uint32_t a[32];
+                ptx::tmem_ld_32x32(lane_base + static_cast<uint32_t>(acc * BN + i * 32), a);
+                if (WHAT != GRAM) {
+                    ptx::cp_async_wait<S::BUFS - 1>();
+                    __syncwarp();
+                }
+                ptx::tmem_ld_wait();
+                float v[32];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    float h[8];
+                    if (WHAT != GRAM) {
+                        load_f<false>(h, place(k, 0, lane, c));
+                        if (p.prev_parts == 2) {
+                            float l[8];
+                            load_f<false>(l, place(k, 1, lane, c));
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) h[e] += l[e];
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float x = __uint_as_float(a[c * 8 + e]) * p.alpha;
+                        v[c * 8 + e] = WHAT != GRAM ? fmaf(p.coef, h[e], x) : x;
+                    }
+                }
+                if (WHAT == APPLY && p.final_out) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) v[e] *= INV_SCALE;
+                    with_final_type(p, b, [&](auto* o) {
+                        if (p.tall) {
+                            if (row0 + lane < p.R) {
+#pragma unroll
+                                for (int e = 0; e < 32; ++e)
+                                    if (col + e < p.C)
+                                        o[static_cast<int64_t>(col + e) * p.final_ld + row0 + lane] =
+                                            from_f<std::remove_pointer_t<decltype(o)>>(v[e]);
+                            }
+                        } else {
+                            final_block(o, p, bufs + k * EPI_BUF_BYTES, row0, col, v);
+                        }
+                    });
+                } else {
+                    // in place (a lane reads and writes its own row), then out by rows
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        Raw<f16, 8> hi, lo;
+                        float x[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) x[e] = v[c * 8 + e];
+                        split_f16(x, hi, lo);
+                        store_raw<false>(place(k, 0, lane, c), hi);
+                        if (p.out_parts == 2) store_raw<false>(place(k, 1, lane, c), lo);
+                        if (SYMMETRIC && mirror) store_transposed(hi, lo, out, p.out, p.out_parts, row0 + lane, col + c * 8, p.cols);
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (int part = 0; part < 2; ++part) {
+                        if (part >= p.out_parts) break;
+#pragma unroll
+                        for (int it = 0; it < 4; ++it) {
+                            const int r = it * 8 + (lane >> 2);
+                            Raw<f16, 8> x;
+                            load_raw<false>(x, place(k, part, r, lane & 3));
+                            if (row0 + r < p.rows)
+                                store_raw<false>(out + part * p.out.part_stride + static_cast<int64_t>(row0 + r) * p.out.ld + col +
+                                                     (lane & 3) * 8, x);
+                        }
+                    }
+                }
+                __syncwarp();
+                if (WHAT != GRAM) {
+                    if (i + S::BUFS < blocks) fetch(i + S::BUFS);
+                    ptx::cp_async_commit();
+                }
+            }
+            if (WHAT != GRAM) ptx::cp_async_wait<0>();
+            release();
+        }
+    }
+
+    if constexpr (!PAIR) {
+        // The slices of a tile meet: CTA r adds its share of the rows of all of them, in slice
+        // order.  A warp takes whole rows, so that what crosses between the SMs and what goes
+        // to memory are runs of 512 and 256 bytes (a thread a row took 8 us for 64 KB).
+        if(threadIdx.x==64) STAMP(5);
+        __syncthreads();
+        ptx::cluster_sync();
+        if(threadIdx.x==64) STAMP(6);
+        if (warp >= 2 && *abort_flag == 0) {
+            const int b = unit / p.tiles;
+            int tm, tn;
+            orth_tile(unit % p.tiles, p, SYMMETRIC, tm, tn);
+            const int share = 128 / p.slices;
+            const int first = static_cast<int>(rank) * share;    // of this CTA's rows
+            const int col = tn * BN + lane * 4;
+            const bool mirror = SYMMETRIC && tn > tm;
+            const bool last = WHAT == APPLY && p.final_out;
+            const f16* prev = p.prev.p + b * p.prev.batch_stride + col;
+            f16* out = p.out.p + b * p.out.batch_stride;
+            // for results that are stored transposed: [128 columns][share rows] of fp32 behind the partial tile
+            float* turned = reinterpret_cast<float*>(smem) + 128 * PART_LD;
+            const int turned_ld = share + 1;
+#pragma unroll 2
+            for (int r = warp - 2; r < share; r += EPI_WARPS) {
+                const int row = tm * BM + first + r;
+                const bool in = row < p.rows && col < p.cols;
+                Raw<f16, 4> ph, pl;
+                if (WHAT != GRAM && in) {        // rows have a pitch of a multiple of 64: whole vectors fit
+                    load_raw<false>(ph, prev + static_cast<int64_t>(row) * p.prev.ld);
+                    if (p.prev_parts == 2) load_raw<false>(pl, prev + p.prev.part_stride + static_cast<int64_t>(row) * p.prev.ld);
+                }
+                const uint32_t at = ptx::smem_u32(smem) + static_cast<uint32_t>(((first + r) * PART_LD + lane * 4) * 4);
+                float4 x[MAX_SLICES];
+#pragma unroll
+                for (int s = 0; s < MAX_SLICES; ++s)
+                    if (s < p.slices) x[s] = ptx::ld_cluster_f4(ptx::map_to_cta(at, s));
+                float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int s = 0; s < MAX_SLICES; ++s) {
+                    if (s < p.slices) {          // (a slice without work wrote zeros)
+                        v[0] += x[s].x; v[1] += x[s].y; v[2] += x[s].z; v[3] += x[s].w;
+                    }
+                }
+                Raw<f16, 4> hi, lo;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    v[e] *= p.alpha;
+                    if (WHAT != GRAM && in) {
+                        const float h = to_f(ph.e[e]);
+                        v[e] = fmaf(p.coef, p.prev_parts == 2 ? h + to_f(pl.e[e]) : h, v[e]);
+                    }
+                    if (last) v[e] *= INV_SCALE;
+                    hi.e[e] = __float2half_rn(v[e]);
+                    lo.e[e] = __float2half_rn(v[e] - __half2float(hi.e[e]));
+                }
+                if (mirror || (last && p.tall)) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) turned[(lane * 4 + e) * turned_ld + r] = v[e];
+                }
+                if (!in) continue;
+                if (last) {
+                    if (!p.tall)
+                        with_final_type(p, b, [&](auto* o) {
+                            o += static_cast<int64_t>(row) * p.final_ld + col;
+                            if (p.final_vec && col + 4 <= p.cols) {
+                                store_f<false>(o, v);
+                            } else {
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    if (col + e < p.cols) o[e] = from_f<std::remove_pointer_t<decltype(o)>>(v[e]);
+                            }
+                        });
+                    continue;
+                }
+                f16* o = out + static_cast<int64_t>(row) * p.out.ld + col;
+                store_raw<false>(o, hi);
+                if (p.out_parts == 2) store_raw<false>(o + p.out.part_stride, lo);
+            }
+            if (mirror || (last && p.tall)) {
+                asm volatile("bar.sync 1, 256;" ::: "memory");   // the eight warps here
+                for (int i = threadIdx.x - 64; i < 128 * share; i += EPI_WARPS * 32) {
+                    const int c = i / share, r = i % share;
+                    const int at_col = tn * BN + c, at_row = tm * BM + first + r;
+                    if (at_col >= p.cols || at_row >= p.rows) continue;
+                    const float x = turned[c * turned_ld + r];
+                    if (last) {
+                        with_final_type(p, b, [&](auto* o) {
+                            o[static_cast<int64_t>(at_col) * p.final_ld + at_row] = from_f<std::remove_pointer_t<decltype(o)>>(x);
+                        });
+                    } else {
+                        f16* o = out + static_cast<int64_t>(at_col) * p.out.ld + at_row;
+                        const f16 hi = __float2half_rn(x);
+                        *o = hi;
+                        if (p.out_parts == 2) o[p.out.part_stride] = __float2half_rn(x - __half2float(hi));
+                    }
+                }
+            }
+        }
+    }
+
+    if(threadIdx.x==64) STAMP(7);
+    // common exit, also after an abort; a CTA of a cluster stays while a peer may touch its memory
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    ptx::cluster_sync_relaxed();
+    if (warp == 1) {
+        __syncwarp();
+        ptx::tc_fence_after_sync();
+        if (PAIR) ptx::tmem_dealloc_pair(tmem_base, TMEM_COLS);
+        else ptx::tmem_dealloc(tmem_base, TMEM_COLS);
+    }
+    if(threadIdx.x==32) STAMP(9);
+}
+
+// ------------------------------------------------------- norm and first split
+
+// partial[matrix][block]: sums of squares, in fp64 (squares of fp32 numbers leave the fp32
+// range).  Threads walk over whole accesses of VEC elements, eight of them in flight.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256)
+orth_norm_kernel(double* __restrict__ partial, const T* __restrict__ g, int64_t ld, int64_t stride, int64_t rows,
+                 int64_t cols)
+{
+    constexpr int DEEP = 8;
+    __shared__ double sh[8];
+    const T* m = g + blockIdx.y * stride;
+    const int64_t nvec = cols / VEC, total = rows * nvec;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
+    double s = 0.0;
+    for (int64_t i0 = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i0 < total; i0 += step * DEEP) {
+        Raw<T, VEC> r[DEEP];
+#pragma unroll
+        for (int k = 0; k < DEEP; ++k) {
+            const int64_t i = i0 + k * step;
+            if (i < total) load_raw<false>(r[k], m + (i / nvec) * ld + (i % nvec) * VEC);
+        }
+#pragma unroll
+        for (int k = 0; k < DEEP; ++k) {
+            if (i0 + k * step < total) {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const double x = static_cast<double>(to_f(r[k].e[e]));
+                    s = fma(x, x, s);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double t = 0.0;
+        for (int i = 0; i < 8; ++i) t += sh[i];
+        partial[blockIdx.y * gridDim.x + blockIdx.x] = t;
+    }
+}
+
+// X0 = G / (|G| + eps) (transposed when TALL) as scaled fp16 parts; 64 x 64 tiles, a thread
+// holds 4 x 4 elements: rows of a tile are read and written 4 columns a lane.
+template <typename T, bool VEC, bool TALL>
+__global__ void __launch_bounds__(256)
+orth_split_kernel(Split x, const double* __restrict__ partial, int parts, const T* __restrict__ g, int64_t ld,
+                  int64_t stride, int64_t rows, int64_t cols, float eps)
+{
+    __shared__ float tile[TALL ? 64 : 1][65];
+    __shared__ float inv_sh;
+    const T* m = g + blockIdx.z * stride;
+    const int64_t r0 = static_cast<int64_t>(blockIdx.y) * 64, c0 = static_cast<int64_t>(blockIdx.x) * 64;
+    const int tx = (threadIdx.x & 15) * 4, ty = threadIdx.x >> 4;
+    Raw<T, 4> in[4];                             // requested before the norm is known
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int64_t r = r0 + ty + k * 16, c = c0 + tx;
+        const T* src = m + r * ld + c;
+        if (VEC && r < rows && c < cols) {       // (the width is a multiple of 4)
+            load_raw<false>(in[k], src);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) in[k].e[e] = r < rows && c + e < cols ? src[e] : from_f<T>(0.0f);
+        }
+    }
+    if (threadIdx.x < 32) {
+        double s = 0.0;
+        for (int i = threadIdx.x; i < parts; i += 32) s += partial[blockIdx.z * parts + i];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if (threadIdx.x == 0) inv_sh = static_cast<float>(static_cast<double>(SCALE) / (sqrt(s) + static_cast<double>(eps)));
+    }
+    __syncthreads();
+    const float inv = inv_sh;
+    f16* out = x.p + blockIdx.z * x.batch_stride;
+    const int64_t xr0 = TALL ? c0 : r0, xc0 = TALL ? r0 : c0, xrows = TALL ? cols : rows;
+    if (TALL) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) tile[ty + k * 16][tx + e] = to_f(in[k].e[e]);
+        __syncthreads();
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int64_t r = xr0 + ty + k * 16;
+        if (r >= xrows) continue;
+        Raw<f16, 4> hi, lo;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float v = (TALL ? tile[tx + e][ty + k * 16] : to_f(in[k].e[e])) * inv;
+            hi.e[e] = __float2half_rn(v);
+            lo.e[e] = __float2half_rn(v - __half2float(hi.e[e]));
+        }
+        f16* o = out + r * x.ld + xc0 + tx;      // the pitch is a multiple of 64: the columns fit
+        store_raw<false>(o, hi);
+        store_raw<false>(o + x.part_stride, lo);
+    }
+}
+
+// ------------------------------------------------------------------------- host
+
+struct OrthPlan {
+    int64_t R, C, batch, ldx, lda;
+    bool split;
+    int64_t x[2], a, b, norm, total;             // byte offsets
+};
+
+OrthPlan plan_orth(int64_t rows, int64_t cols, int64_t batch, int type)
+{
+    OrthPlan q{};
+    q.R = rows < cols ? rows : cols;
+    q.C = rows < cols ? cols : rows;
+    q.batch = batch;
+    q.ldx = (q.C + 63) / 64 * 64;
+    q.lda = (q.R + 63) / 64 * 64;
+    q.split = type != SB200_BF16;
+    int64_t at = 0;
+    auto take = [&](int64_t bytes) { const int64_t o = at; at += (bytes + 255) / 256 * 256; return o; };
+    for (int i = 0; i < 2; ++i) q.x[i] = take(2 * batch * q.R * q.ldx * 2);
+    q.a = take((q.split ? 2 : 1) * batch * q.R * q.lda * 2);
+    q.b = take((q.split ? 2 : 1) * batch * q.R * q.lda * 2);
+    q.norm = take(batch * NORM_BLOCKS * 8);
+    q.total = at + 256;                          // the base is rounded up to 256 bytes
+    return q;
+}
+
+// box: 64 elements along the contiguous dimension (a row of the 128-byte swizzle) x box_rows rows
+int orth_map(sb200_ctx* ctx, CUtensorMap* map, const Split& m, int64_t cols, int64_t rows, int64_t matrices, int box_rows)
+{
+    EncodeTiledFn enc = reinterpret_cast<EncodeTiledFn>(ctx->encode_tiled);
+    if (!enc) return SB200_ERR_UNSUPPORTED;
+    const TensorMapKey key{reinterpret_cast<uint64_t>(m.p), cols, rows, m.ld, matrices, m.batch_stride, box_rows, 3};
+    return cached_map(ctx, map, key, [&](CUtensorMap* t) {
+        cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(matrices)};
+        cuuint64_t strides[2] = {static_cast<cuuint64_t>(m.ld) * 2, static_cast<cuuint64_t>(m.batch_stride) * 2};
+        cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_rows), 1};
+        cuuint32_t estr[3] = {1, 1, 1};
+        return enc(t, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, m.p, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    });
+}
+
+int dbg_no=0;
+struct OrthMaps {
+    CUtensorMap a, b;
+};
+
+template <int WHAT, bool PAIR, bool SPLIT>
+int launch_product(sb200_ctx* ctx, const OrthMaps& m, OrthParams p, cudaStream_t stream)
+{
+    auto kern = orth_product_kernel<WHAT, PAIR, SPLIT>;
+    constexpr int SMEM = OrthSmem<SPLIT>::TOTAL;
+    static bool attr_done[16] = {};
+    if (ctx->device >= 16 || !attr_done[ctx->device]) {
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess) return SB200_ERR_CUDA;
+        if (ctx->device < 16) attr_done[ctx->device] = true;
+    }
+    constexpr int TILE = PAIR ? 256 : 128;
+    p.tiles_m = (p.rows + TILE - 1) / TILE;
+    p.tiles_n = (p.cols + TILE - 1) / TILE;
+    p.tiles = WHAT == APPLY ? p.tiles_m * p.tiles_n : p.tiles_m * (p.tiles_m + 1) / 2;
+    const long long total = static_cast<long long>(p.tiles) * p.batch;
+    const int group = PAIR ? 2 : p.slices;
+    const long long most = PAIR ? ctx->sm_count / 2 : total;     // pairs walk over the tiles
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(group * (total < most ? total : most)));
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = SMEM;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(group);
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    static int no=0; p.launch_no = (dbg_no++);
+    const cudaError_t err = cudaLaunchKernelEx(&cfg, kern, m.a, m.b, p);
+    ctx->launches += 1;
+    return err == cudaSuccess && cudaGetLastError() == cudaSuccess ? SB200_OK : SB200_ERR_CUDA;
+}
+
+// Pairs or slices.  A 256 x 256 tile on a pair and a 128 x 128 tile on one SM take about
+// the same time per k-block (the tensor core of the latter waits for shared memory: 128
+// bytes a cycle feed it and take in the tiles), so a pair does four times the work on
+// twice the SMs; slices win where the tiles do not fill the device.  Returns 0 for pairs,
+// else the number of slices.
+int slices_for(const sb200_ctx* ctx, int64_t rows, int64_t cols, int64_t batch, int num_kb, bool symmetric, bool split)
+{
+    auto tiles = [&](int64_t t) {
+        const int64_t tm = (rows + t - 1) / t, tn = (cols + t - 1) / t;
+        return (symmetric ? tm * (tm + 1) / 2 : tm * tn) * batch;
+    };
+    const int64_t pairs = ctx->sm_count / 2, t1 = tiles(128), t2 = tiles(256);
+    int s = 1;
+    while (s < MAX_SLICES && 2 * s <= num_kb && t1 * 2 * s <= ctx->sm_count) s *= 2;
+    const double sliced = static_cast<double>((t1 * s + ctx->sm_count - 1) / ctx->sm_count) *
+                          ((num_kb + s - 1) / s * (split ? 0.8 : 1.2) + 4.0);
+    const double paired = static_cast<double>((t2 + pairs - 1) / pairs) * num_kb + (split ? 4.0 : 8.0);
+    return sliced < paired ? s : 0;
+}
+
+template <int WHAT>
+int product(sb200_ctx* ctx, bool split, const OrthMaps& m, OrthParams p, cudaStream_t stream)
+{
+    p.slices = slices_for(ctx, p.rows, p.cols, p.batch, p.num_kb, WHAT != APPLY, split);
+    if (p.slices == 0)
+        return split ? launch_product<WHAT, true, true>(ctx, m, p, stream) : launch_product<WHAT, true, false>(ctx, m, p, stream);
+    return split ? launch_product<WHAT, false, true>(ctx, m, p, stream) : launch_product<WHAT, false, false>(ctx, m, p, stream);
+}
+
+// Largest |f| of an odd or even polynomial over [0, s], by its samples: the polynomials
+// are smooth, 1024 samples are within a thousandth of the maximum.
+template <typename F>
+double largest(F f, double s)
+{
+    double m = 0.0;
+    for (int i = 0; i <= 1024; ++i) {
+        const double v = std::fabs(f(s * i / 1024.0));
+        if (!(v <= m)) m = v;
+    }
+    return m;
+}
+
+// Whether every matrix of the iteration stays inside the range of the scaled fp16 parts.
+bool bounded(double a, double b, double c, int steps)
+{
+    double s = 1.01;
+    for (int k = 0; k < steps; ++k) {
+        const double m = largest([&](double t) { return b * t * t + c * t * t * t * t; }, s);
+        if (!(s * s < LARGEST) || !(m < LARGEST)) return false;
+        s = 1.01 * largest([&](double t) { return t * (a + b * t * t + c * t * t * t * t); }, s);
+    }
+    return true;
+}
+
+constexpr int64_t MAX_SIDE = int64_t(1) << 20;
+constexpr int MAX_STEPS = 64;
+
+}  // namespace
+}  // namespace sb200
+
+using namespace sb200;
+
+extern "C" int64_t sb200_orthogonalize_workspace(int64_t rows, int64_t cols, int64_t batch, int type)
+{
+    if (rows < 0 || cols < 0 || batch < 0 || !known_type(type) || rows > MAX_SIDE || cols > MAX_SIDE || batch > 65535) return -1;
+    return plan_orth(rows, cols, batch, type).total;
+}
+
+extern "C" int sb200_orthogonalize(sb200_ctx* ctx, void* out, int64_t ldo, int64_t stride_out, const void* g, int64_t ldg,
+                                   int64_t stride_g, int64_t rows, int64_t cols, int64_t batch, int steps, float a, float b,
+                                   float c, float eps, int type, void* workspace, int64_t workspace_bytes, sb200_stream stream_)
+{
+    TraceRange trace("sb200_orthogonalize");
+    if (!ctx || rows < 0 || cols < 0 || batch < 0 || ldo < cols || ldg < cols || stride_out < 0 || stride_g < 0 ||
+        !known_type(type) || steps < 1 || !(eps >= 0.0f))
+        return SB200_ERR_INVALID_ARG;
+    if (batch > 1 && stride_out < (rows - 1) * ldo + cols) return SB200_ERR_INVALID_ARG;   // outputs would overlap
+    if (rows > MAX_SIDE || cols > MAX_SIDE || batch > 65535 || steps > MAX_STEPS) return SB200_ERR_TOO_LARGE;
+    if (!bounded(a, b, c, steps)) return SB200_ERR_UNSUPPORTED;
+    if (rows == 0 || cols == 0 || batch == 0) return SB200_OK;
+    if (!out || !g) return SB200_ERR_INVALID_ARG;
+    const OrthPlan q = plan_orth(rows, cols, batch, type);
+    if (!workspace || workspace_bytes < q.total) return SB200_ERR_INVALID_ARG;
+    DeviceGuard dev(ctx->device);
+    if (!dev.ok) return SB200_ERR_CUDA;
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    unsigned char* ws = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~uintptr_t(255));
+    const int tall = rows > cols;
+
+    auto matrix = [&](int64_t at, int64_t ld) {
+        Split m;
+        m.p = reinterpret_cast<f16*>(ws + at);
+        m.ld = ld;
+        m.batch_stride = q.R * ld;
+        m.part_stride = batch * q.R * ld;
+        return m;
+    };
+    const Split X[2] = {matrix(q.x[0], q.ldx), matrix(q.x[1], q.ldx)};
+    const Split A = matrix(q.a, q.lda), B = matrix(q.b, q.lda);
+    double* partial = reinterpret_cast<double*>(ws + q.norm);
+
+    const dim3 split_grid(static_cast<unsigned>((cols + 63) / 64), static_cast<unsigned>((rows + 63) / 64), static_cast<unsigned>(batch));
+    auto start = [&](auto t) {
+        using T = decltype(t);
+        constexpr int WIDE = 16 / sizeof(T);
+        const T* gp = static_cast<const T*>(g);
+        const bool wide = cols % WIDE == 0 && ldg % WIDE == 0 && (batch == 1 || stride_g % WIDE == 0) && aligned_to(g, 16);
+        // about 8 accesses a thread
+        const int64_t accesses = rows * cols / (wide ? WIDE : 1);
+        int64_t blocks = (accesses + 2047) / 2048;
+        const int parts = static_cast<int>(blocks < NORM_BLOCKS ? blocks : NORM_BLOCKS);
+        const dim3 norm_grid(parts, static_cast<unsigned>(batch));
+        if (wide) orth_norm_kernel<T, WIDE><<<norm_grid, 256, 0, stream>>>(partial, gp, ldg, stride_g, rows, cols);
+        else orth_norm_kernel<T, 1><<<norm_grid, 256, 0, stream>>>(partial, gp, ldg, stride_g, rows, cols);
+        auto split = [&](auto kern) { kern<<<split_grid, 256, 0, stream>>>(X[0], partial, parts, gp, ldg, stride_g, rows, cols, eps); };
+        if (tall) { if (wide) split(orth_split_kernel<T, true, true>); else split(orth_split_kernel<T, false, true>); }
+        else { if (wide) split(orth_split_kernel<T, true, false>); else split(orth_split_kernel<T, false, false>); }
+    };
+    if (type == SB200_F32) start(float{});
+    else if (type == SB200_BF16) start(bf16{});
+    else start(f16{});
+    ctx->launches += 2;
+    if (cudaGetLastError() != cudaSuccess) return SB200_ERR_CUDA;
+
+    const int64_t xm = 2 * batch, am = (q.split ? 2 : 1) * batch;
+    CUtensorMap x_rows[2], x_cols[2], a_rows, b_rows;
+    for (int i = 0; i < 2; ++i) {
+        if (const int rc = orth_map(ctx, &x_rows[i], X[i], q.C, q.R, xm, 128)) return rc;
+        if (const int rc = orth_map(ctx, &x_cols[i], X[i], q.C, q.R, xm, KB)) return rc;
+    }
+    if (const int rc = orth_map(ctx, &a_rows, A, q.R, q.R, am, 128)) return rc;
+    if (const int rc = orth_map(ctx, &b_rows, B, q.R, q.R, am, 128)) return rc;
+
+    OrthParams p{};
+    p.R = static_cast<int>(q.R);
+    p.C = static_cast<int>(q.C);
+    p.batch = static_cast<int>(batch);
+    p.status = ctx->d_status;
+    p.wait_limit_ns = ctx->wait_limit_ns;
+    p.test_stall_kb = ctx->test_stall_kb;
+    const int kb_c = static_cast<int>((q.C + KB - 1) / KB), kb_r = static_cast<int>((q.R + KB - 1) / KB);
+    for (int k = 0; k < steps; ++k) {
+        const int from = k & 1, to = from ^ 1;
+        // A = X X^T
+        p.rows = p.cols = p.R;
+        p.num_kb = kb_c;
+        p.chunk_kb = q.split ? CHUNK_KB : kb_c;
+        p.prev = A;
+        p.prev_parts = 0;
+        p.out = A;
+        p.out_parts = q.split ? 2 : 1;
+        p.coef = 0.0f;
+        p.alpha = INV_SCALE;
+        p.final_out = nullptr;
+        if (const int rc = product<GRAM>(ctx, q.split, {x_rows[from], x_rows[from]}, p, stream)) return rc;
+        // B = b A + c A A
+        p.num_kb = kb_r;
+        p.chunk_kb = q.split ? CHUNK_KB : kb_r;
+        p.prev_parts = p.out_parts;
+        p.out = B;
+        p.coef = b;
+        p.alpha = c * INV_SCALE;
+        if (const int rc = product<POLY>(ctx, q.split, {a_rows, a_rows}, p, stream)) return rc;
+        // X = a X + B X
+        p.cols = p.C;
+        p.prev = X[from];
+        p.prev_parts = 2;
+        p.out = X[to];
+        p.out_parts = 2;
+        p.coef = a;
+        p.alpha = INV_SCALE;
+        if (k + 1 == steps) {
+            p.final_out = out;
+            p.final_ld = ldo;
+            p.final_stride = batch > 1 ? stride_out : 0;
+            p.final_type = type;
+            p.tall = tall;
+            p.final_vec = !tall && aligned_to(out, 16) && (ldo * type_bytes(type)) % 16 == 0 &&
+                          (p.final_stride * type_bytes(type)) % 16 == 0;
+        }
+        if (const int rc = product<APPLY>(ctx, q.split, {b_rows, x_cols[from]}, p, stream)) return rc;
+    }
+    return SB200_OK;
+}
+
+extern "C" int dbg_read(unsigned long long* h,int n){ cudaDeviceSynchronize(); sb200::dbg_no=0; return cudaMemcpyFromSymbol(h,dbg_t,n*128);}
