@@ -46,7 +46,7 @@ constexpr int CHUNK_KB = 2;                      // k-blocks per accumulation ch
 constexpr float SCALE = 8192.0f;                 // 2^13
 constexpr float INV_SCALE = 1.0f / 8192.0f;
 constexpr double LARGEST = 7.5;                  // of a singular value: 7.5 * 2^13 < 65504
-constexpr int EPI_WARPS = 8;
+constexpr int EPI_WARPS = 16;
 constexpr int THREADS = 64 + EPI_WARPS * 32;
 constexpr int NORM_BLOCKS = 512;                 // partial sums of squares per matrix
 constexpr int ORTH_PANEL = 8;
@@ -78,28 +78,37 @@ struct OrthParams {
     int launch_no;
 };
 
-// The epilogue of the pair kernel moves 32 x 32 blocks of both parts through shared memory
-// (rows of 64 bytes, their 16-byte pieces permuted against bank conflicts): a thread owns a
-// row of the accumulator, and 32 rows a warp touched with plain 16-byte accesses cost 32
-// cycles of the load/store unit each (an epilogue of 24 us where the products take 5);
-// through shared memory four lanes share a row.  TMA would do the same, but it is what
-// feeds the tensor core: blocks moved by TMA made the operand tiles late (9.6 us a tile).
-constexpr int EPI_PART_BYTES = 32 * 32 * 2;
-constexpr int EPI_BUF_BYTES = 2 * EPI_PART_BYTES;
-
+// The epilogue of the pair kernel moves blocks of 32 rows through shared memory (their
+// 16-byte pieces permuted against bank conflicts): a thread owns a row of the accumulator,
+// and 32 rows a warp touched with plain 16-byte accesses cost 32 cycles of the load/store
+// unit each (an epilogue of 24 us where the products take 5); through shared memory the
+// lanes of a row share it.  TMA would do the same, but it is what feeds the tensor core:
+// blocks moved by TMA made the operand tiles late (9.6 us a tile).  Sixteen warps, because
+// the work is a chain of short latencies (eight took twice as long), in a loop that is not
+// unrolled over the blocks, because code that runs once a tile misses the instruction cache.
 template <bool SPLIT>
 struct OrthSmem {
     static constexpr int PARTS = SPLIT ? 2 : 1;
     static constexpr int STAGE = 2 * PARTS * TILE_BYTES;
     static constexpr int STAGES = SPLIT ? 3 : 5;
     static constexpr int TILES = STAGE * STAGES;
-    static constexpr int BUFS = SPLIT ? 1 : 2;   // epilogue buffers per warp
-    static constexpr int EPI = EPI_WARPS * BUFS * EPI_BUF_BYTES;
+    static constexpr int BW = SPLIT ? 16 : 32;   // columns of an epilogue block
+    static constexpr int EPI_PART = 32 * BW * 2; // one part of a block
+    static constexpr int EPI_BUF = 2 * EPI_PART; // one per warp
+    static constexpr int EPI = EPI_WARPS * EPI_BUF;
     static constexpr int BARS = ((2 * STAGES + 4) * 8 + 16 + 15) & ~15;
     static constexpr int TOTAL = TILES + EPI + BARS + 1024;
     static_assert(TOTAL <= 227 * 1024, "shared memory per CTA");
     static_assert(TILES >= 128 * PART_LD * 4 + 128 * 129 * 4, "what the sliced kernel keeps in the place of the stages");
 };
+
+// 16-byte piece c of row r of a block with `pieces` of them a row
+template <int PIECES>
+__device__ __forceinline__ int piece_at(int r, int c)
+{
+    static_assert(PIECES == 2 || PIECES == 4 || PIECES == 8, "rows of 32, 64 or 128 bytes");
+    return r * PIECES + (PIECES == 8 ? c ^ (r & 7) : PIECES == 4 ? c ^ ((r >> 1) & 3) : c ^ ((r >> 2) & 1));
+}
 
 // Tile t of a matrix; symmetric products walk over the tiles with tn >= tm only.
 __device__ __forceinline__ void orth_tile(int t, const OrthParams& p, bool symmetric, int& tm, int& tn)
@@ -118,12 +127,26 @@ __device__ __forceinline__ void orth_tile(int t, const OrthParams& p, bool symme
     tn = row + t;
 }
 
-__device__ __forceinline__ void split_f16(const float (&v)[8], Raw<f16, 8>& hi, Raw<f16, 8>& lo)
+template <int N>
+__device__ __forceinline__ void split_f16(const float* v, Raw<f16, N>& hi, Raw<f16, N>& lo)
 {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        hi.e[e] = __float2half_rn(v[e]);
-        lo.e[e] = __float2half_rn(v[e] - __half2float(hi.e[e]));
+    for (int e = 0; e < N; e += 2) {
+        const __half2 h = __floats2half2_rn(v[e], v[e + 1]);
+        const float2 f = __half22float2(h);
+        *reinterpret_cast<__half2*>(&hi.e[e]) = h;
+        *reinterpret_cast<__half2*>(&lo.e[e]) = __floats2half2_rn(v[e] - f.x, v[e + 1] - f.y);
+    }
+}
+
+// hi + lo of eight elements
+__device__ __forceinline__ void join_f16(float (&v)[8], const Raw<f16, 8>& hi)
+{
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi.e[e]));
+        v[e] += f.x;
+        v[e + 1] += f.y;
     }
 }
 
@@ -149,39 +172,40 @@ __device__ __forceinline__ void with_final_type(const OrthParams& p, int b, F f)
     else f(static_cast<f16*>(p.final_out) + at);
 }
 
-// One warp's 32 x 32 block of the caller's matrix, stored by rows.  v: this lane's row.
-// buf: 4 KB of shared memory nobody else uses; 16-byte pieces of a row are permuted so that
-// neither side has bank conflicts.
-template <typename T>
+// One warp's block of 32 rows x BW columns of the caller's matrix, stored by rows.  v: this
+// lane's row.  buf: 128 BW bytes of shared memory nobody else uses.
+template <int BW, typename T>
 __device__ __forceinline__ void final_block(T* out, const OrthParams& p, uint8_t* buf, int row0, int col0,
-                                            const float (&v)[32])
+                                            const float (&v)[BW])
 {
     constexpr int PER = 16 / static_cast<int>(sizeof(T));        // elements of a piece
-    constexpr int PIECES = 32 / PER;                             // pieces of a row
+    constexpr int PIECES = BW / PER;                             // pieces of a row
     const int lane = threadIdx.x & 31;
-    auto place = [](int r, int piece) { return PIECES == 8 ? piece ^ (r & 7) : piece ^ ((r >> 1) & 3); };
+    T* b = reinterpret_cast<T*>(buf);
     __syncwarp();
 #pragma unroll
     for (int c = 0; c < PIECES; ++c) {
-        Raw<T, PER> x;
+        float x[PER];
 #pragma unroll
-        for (int e = 0; e < PER; ++e) x.e[e] = from_f<T>(v[c * PER + e]);
-        store_raw<false>(reinterpret_cast<T*>(buf) + lane * 32 + place(lane, c) * PER, x);
+        for (int e = 0; e < PER; ++e) x[e] = v[c * PER + e];
+        store_f<false>(b + piece_at<PIECES>(lane, c) * PER, x);
     }
     __syncwarp();
-    if (p.final_vec && col0 + 32 <= p.C) {
+    if (p.final_vec && col0 + BW <= p.C) {
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
             const int r = i * (32 / PIECES) + lane / PIECES, c = lane % PIECES;
             Raw<T, PER> x;
-            load_raw<false>(x, reinterpret_cast<const T*>(buf) + r * 32 + place(r, c) * PER);
+            load_raw<false>(x, b + piece_at<PIECES>(r, c) * PER);
             if (row0 + r < p.R) store_raw<true>(out + static_cast<int64_t>(row0 + r) * p.final_ld + col0 + c * PER, x);
         }
     } else {
-        for (int r = 0; r < 32 && row0 + r < p.R; ++r)
-            if (col0 + lane < p.C)
-                out[static_cast<int64_t>(row0 + r) * p.final_ld + col0 + lane] =
-                    reinterpret_cast<const T*>(buf)[r * 32 + place(r, lane / PER) * PER + lane % PER];
+#pragma unroll 1
+        for (int i = lane; i < 32 * BW; i += 32) {
+            const int r = i / BW, c = i % BW;
+            if (row0 + r < p.R && col0 + c < p.C)
+                out[static_cast<int64_t>(row0 + r) * p.final_ld + col0 + c] = b[piece_at<PIECES>(r, c / PER) * PER + c % PER];
+        }
     }
     __syncwarp();
 }
@@ -200,7 +224,8 @@ orth_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     constexpr bool B_MN = WHAT == APPLY;
     constexpr int CTAS = PAIR ? 2 : 1;
     constexpr int BM = 128 * CTAS, BN = 128 * CTAS;
-    constexpr int COLS = BN / 2;                 // accumulator columns of an epilogue warp
+    constexpr int COLS = BN / (EPI_WARPS / 4);   // accumulator columns of an epilogue warp
+    constexpr int BW = S::BW, PIECES = BW / 8;
     constexpr uint32_t TMEM_COLS = 2 * BN;
 
     if(threadIdx.x==0) STAMP(0);
@@ -369,10 +394,13 @@ orth_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         }
     } else {
         // ---------------------------------------------------------- epilogue
-        // warp w reads TMEM lanes 32 (w % 4) .. + 31 and one half of the columns
-        const int q = warp & 3, half = (warp - 2) >> 2;
-        const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(half * COLS);
-        uint8_t* bufs = epi + (warp - 2) * S::BUFS * EPI_BUF_BYTES;
+        // warp w reads TMEM lanes 32 (w % 4) .. + 31 and a quarter of the columns
+        const int q = warp & 3, quarter = (warp - 2) >> 2;
+        const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(quarter * COLS);
+        f16* buf = reinterpret_cast<f16*>(epi + (warp - 2) * S::EPI_BUF);
+        f16* buf_lo = buf + S::EPI_PART / 2;
+        // by rows: PIECES lanes share a row of a block
+        const int by_row = lane / PIECES, by_col = lane % PIECES;
         int acc = 0;
         uint32_t acc_ph = 0;
         bool ok = true;
@@ -391,34 +419,22 @@ orth_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             int tm, tn;
             orth_tile(t % p.tiles, p, SYMMETRIC, tm, tn);
             const int row0 = tm * BM + static_cast<int>(pair_rank) * 128 + q * 32;
-            const int col0 = tn * BN + half * COLS;
-            // blocks of 32 columns this warp has to finish; none where its rows or columns are beyond the matrix
-            const int blocks = row0 < p.rows && col0 < p.cols ? min(COLS, p.cols - col0 + 31) / 32 : 0;
-            // 16-byte piece c of row r of a block
-            auto place = [&](int k, int part, int r, int c) {
-                return reinterpret_cast<f16*>(bufs + k * EPI_BUF_BYTES + part * EPI_PART_BYTES + r * 64 +
-                                              ((c ^ ((r >> 1) & 3)) << 4));
-            };
-            auto fetch = [&](int i) {            // block i of prev into its buffer: four lanes a row
-                const f16* src = p.prev.p + b * p.prev.batch_stride + col0 + i * 32 + (lane & 3) * 8;
-                for (int part = 0; part < p.prev_parts; ++part) {
+            const int col0 = tn * BN + quarter * COLS;
+            // blocks of columns this warp has to finish; none where its rows or columns are beyond the matrix
+            const int blocks = row0 < p.rows && col0 < p.cols ? min(COLS, p.cols - col0 + BW - 1) / BW : 0;
+            const f16* prev = p.prev.p + b * p.prev.batch_stride + static_cast<int64_t>(row0 + by_row) * p.prev.ld + col0 + by_col * 8;
+            auto fetch = [&](int i) {            // block i of prev, asynchronously
 #pragma unroll
-                    for (int it = 0; it < 4; ++it) {
-                        const int r = it * 8 + (lane >> 2);
-                        const bool in = row0 + r < p.rows;       // (the pitch covers whole blocks of columns)
-                        ptx::cp_async_16(place(i % S::BUFS, part, r, lane & 3),
-                                         in ? src + part * p.prev.part_stride + static_cast<int64_t>(row0 + r) * p.prev.ld : src,
-                                         in ? 16 : 0);
-                    }
+                for (int it = 0; it < PIECES; ++it) {
+                    const int r = it * (32 / PIECES) + by_row;
+                    const int bytes = row0 + r < p.rows ? 16 : 0;        // (the pitch covers whole blocks of columns)
+                    const f16* src = prev + (bytes ? static_cast<int64_t>(it * (32 / PIECES)) * p.prev.ld + i * BW : 0);
+                    ptx::cp_async_16(buf + piece_at<PIECES>(r, by_col) * 8, src, bytes);
+                    if (p.prev_parts == 2) ptx::cp_async_16(buf_lo + piece_at<PIECES>(r, by_col) * 8, src + p.prev.part_stride, bytes);
                 }
             };
             if constexpr (PAIR && WHAT != GRAM) {
-                // the first blocks of prev travel while the products run; one group a block
-#pragma unroll
-                for (int i = 0; i < S::BUFS; ++i) {
-                    if (i < blocks) fetch(i);
-                    ptx::cp_async_commit();
-                }
+                if (blocks > 0) fetch(0);        // travels while the products run
             }
             if (SPLIT || !PAIR) {
                 // chains of accumulations are added here, rounded to nearest
@@ -430,33 +446,31 @@ orth_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 if(threadIdx.x==64) STAMP(4);
                     ptx::tc_fence_after_sync();
 #pragma unroll
-                    for (int c = 0; c < COLS / 32; ++c) {
-                        uint32_t v[32];
-                        ptx::tmem_ld_32x32(lane_base + static_cast<uint32_t>(acc * BN + c * 32), v);
+                    for (int c = 0; c < COLS / 16; ++c) {
+                        uint32_t v[16];
+                        ptx::tmem_ld_32x16(lane_base + static_cast<uint32_t>(acc * BN + c * 16), v);
                         ptx::tmem_ld_wait();
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) sum[c * 32 + j] = __fadd_rn(sum[c * 32 + j], __uint_as_float(v[j]));
+                        for (int j = 0; j < 16; ++j) sum[c * 16 + j] = __fadd_rn(sum[c * 16 + j], __uint_as_float(v[j]));
                     }
                     if (PAIR && kb0 + p.chunk_kb >= kb_last) break;
                     release();
                 }
                 if (!ok) break;
                 if constexpr (PAIR) {
-                    // the total goes back into the last accumulator, for the loop over the blocks:
-                    // unrolled over 128 registers that loop spilled, and its code, run once a tile,
-                    // came from beyond the instruction cache
+                    // the total goes back into the last accumulator, for the loop over the blocks
 #pragma unroll
-                    for (int c = 0; c < COLS / 32; ++c) {
-                        uint32_t v[32];
+                    for (int c = 0; c < COLS / 16; ++c) {
+                        uint32_t v[16];
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(sum[c * 32 + j]);
-                        ptx::tmem_st_32x32(lane_base + static_cast<uint32_t>(acc * BN + c * 32), v);
+                        for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(sum[c * 16 + j]);
+                        ptx::tmem_st_32x16(lane_base + static_cast<uint32_t>(acc * BN + c * 16), v);
                     }
                     ptx::tmem_st_wait();
                 } else {
                     // every role of this CTA is done with the stages (the last product has read
                     // them): the partial tile goes there
-                    float* part = reinterpret_cast<float*>(smem) + (q * 32 + lane) * PART_LD + half * COLS;
+                    float* part = reinterpret_cast<float*>(smem) + (q * 32 + lane) * PART_LD + quarter * COLS;
 #pragma unroll
                     for (int j = 0; j < COLS; j += 4)
                         *reinterpret_cast<float4*>(part + j) = make_float4(sum[j], sum[j + 1], sum[j + 2], sum[j + 3]);
@@ -467,30 +481,31 @@ orth_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             }
             if constexpr (!PAIR) continue;       // (one tile a cluster: the rest is below)
             f16* out = p.out.p + b * p.out.batch_stride;
+            f16* out_rows = out + static_cast<int64_t>(row0 + by_row) * p.out.ld + col0 + by_col * 8;
             const bool mirror = SYMMETRIC && tn > tm;            // (all rows of such a tile are in the matrix)
 #pragma unroll 1
             for (int i = 0; i < blocks; ++i) {
-                const int k = i % S::BUFS;
-                const int col = col0 + i * 32;
-                uint32_t a[32];
-                ptx::tmem_ld_32x32(lane_base + static_cast<uint32_t>(acc * BN + i * 32), a);
+                const int col = col0 + i * BW;
+                uint32_t a[BW];
+                if constexpr (BW == 32) ptx::tmem_ld_32x32(lane_base + static_cast<uint32_t>(acc * BN + i * BW), a);
+                else ptx::tmem_ld_32x16(lane_base + static_cast<uint32_t>(acc * BN + i * BW), a);
                 if (WHAT != GRAM) {
-                    ptx::cp_async_wait<S::BUFS - 1>();
+                    ptx::cp_async_wait_all();
                     __syncwarp();
                 }
                 ptx::tmem_ld_wait();
-                float v[32];
+                float v[BW];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    float h[8];
+                for (int c = 0; c < PIECES; ++c) {
+                    float h[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
                     if (WHAT != GRAM) {
-                        load_f<false>(h, place(k, 0, lane, c));
+                        Raw<f16, 8> x;
                         if (p.prev_parts == 2) {
-                            float l[8];
-                            load_f<false>(l, place(k, 1, lane, c));
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) h[e] += l[e];
+                            load_raw<false>(x, buf_lo + piece_at<PIECES>(lane, c) * 8);
+                            join_f16(h, x);
                         }
+                        load_raw<false>(x, buf + piece_at<PIECES>(lane, c) * 8);
+                        join_f16(h, x);
                     }
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
@@ -500,55 +515,49 @@ orth_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 }
                 if (WHAT == APPLY && p.final_out) {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) v[e] *= INV_SCALE;
+                    for (int e = 0; e < BW; ++e) v[e] *= INV_SCALE;
                     with_final_type(p, b, [&](auto* o) {
                         if (p.tall) {
                             if (row0 + lane < p.R) {
 #pragma unroll
-                                for (int e = 0; e < 32; ++e)
+                                for (int e = 0; e < BW; ++e)
                                     if (col + e < p.C)
                                         o[static_cast<int64_t>(col + e) * p.final_ld + row0 + lane] =
                                             from_f<std::remove_pointer_t<decltype(o)>>(v[e]);
                             }
                         } else {
-                            final_block(o, p, bufs + k * EPI_BUF_BYTES, row0, col, v);
+                            final_block<BW>(o, p, reinterpret_cast<uint8_t*>(buf), row0, col, v);
                         }
                     });
                 } else {
                     // in place (a lane reads and writes its own row), then out by rows
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
+                    for (int c = 0; c < PIECES; ++c) {
                         Raw<f16, 8> hi, lo;
-                        float x[8];
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) x[e] = v[c * 8 + e];
-                        split_f16(x, hi, lo);
-                        store_raw<false>(place(k, 0, lane, c), hi);
-                        if (p.out_parts == 2) store_raw<false>(place(k, 1, lane, c), lo);
+                        split_f16(v + c * 8, hi, lo);
+                        store_raw<false>(buf + piece_at<PIECES>(lane, c) * 8, hi);
+                        if (p.out_parts == 2) store_raw<false>(buf_lo + piece_at<PIECES>(lane, c) * 8, lo);
                         if (SYMMETRIC && mirror) store_transposed(hi, lo, out, p.out, p.out_parts, row0 + lane, col + c * 8, p.cols);
                     }
                     __syncwarp();
 #pragma unroll
-                    for (int part = 0; part < 2; ++part) {
-                        if (part >= p.out_parts) break;
-#pragma unroll
-                        for (int it = 0; it < 4; ++it) {
-                            const int r = it * 8 + (lane >> 2);
+                    for (int it = 0; it < PIECES; ++it) {
+                        const int r = it * (32 / PIECES) + by_row;
+                        if (row0 + r < p.rows) {
+                            f16* o = out_rows + static_cast<int64_t>(it * (32 / PIECES)) * p.out.ld + i * BW;
                             Raw<f16, 8> x;
-                            load_raw<false>(x, place(k, part, r, lane & 3));
-                            if (row0 + r < p.rows)
-                                store_raw<false>(out + part * p.out.part_stride + static_cast<int64_t>(row0 + r) * p.out.ld + col +
-                                                     (lane & 3) * 8, x);
+                            load_raw<false>(x, buf + piece_at<PIECES>(r, by_col) * 8);
+                            store_raw<false>(o, x);
+                            if (p.out_parts == 2) {
+                                load_raw<false>(x, buf_lo + piece_at<PIECES>(r, by_col) * 8);
+                                store_raw<false>(o + p.out.part_stride, x);
+                            }
                         }
                     }
                 }
                 __syncwarp();
-                if (WHAT != GRAM) {
-                    if (i + S::BUFS < blocks) fetch(i + S::BUFS);
-                    ptx::cp_async_commit();
-                }
+                if (WHAT != GRAM && i + 1 < blocks) fetch(i + 1);
             }
-            if (WHAT != GRAM) ptx::cp_async_wait<0>();
             release();
         }
     }
@@ -596,7 +605,6 @@ orth_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                         v[0] += x[s].x; v[1] += x[s].y; v[2] += x[s].z; v[3] += x[s].w;
                     }
                 }
-                Raw<f16, 4> hi, lo;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     v[e] *= p.alpha;
@@ -605,9 +613,9 @@ orth_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                         v[e] = fmaf(p.coef, p.prev_parts == 2 ? h + to_f(pl.e[e]) : h, v[e]);
                     }
                     if (last) v[e] *= INV_SCALE;
-                    hi.e[e] = __float2half_rn(v[e]);
-                    lo.e[e] = __float2half_rn(v[e] - __half2float(hi.e[e]));
                 }
+                Raw<f16, 4> hi, lo;
+                split_f16(v, hi, lo);
                 if (mirror || (last && p.tall)) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) turned[(lane * 4 + e) * turned_ld + r] = v[e];
@@ -632,7 +640,7 @@ orth_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 if (p.out_parts == 2) store_raw<false>(o + p.out.part_stride, lo);
             }
             if (mirror || (last && p.tall)) {
-                asm volatile("bar.sync 1, 256;" ::: "memory");   // the eight warps here
+                asm volatile("bar.sync 1, %0;" ::"n"(EPI_WARPS * 32) : "memory");
                 for (int i = threadIdx.x - 64; i < 128 * share; i += EPI_WARPS * 32) {
                     const int c = i / share, r = i % share;
                     const int at_col = tn * BN + c, at_row = tm * BM + first + r;
