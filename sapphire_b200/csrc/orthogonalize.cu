@@ -15,11 +15,12 @@
 //     tensor-core products at the fp16 rate (a product of two TF32 parts would run at half
 //     of it).  The tensor core cuts its fp32 accumulation short instead of rounding it,
 //     so a chain of accumulations ends after CHUNK_KB k-blocks and the chains are added
-//     in registers.
-//   bf16 input: the products take the hi parts alone (11 bits; the result keeps 8).
-//     X still has both parts and the a X term uses both: rounding X itself every step
-//     would feed the small singular directions, which a step multiplies by a, with the
-//     rounding errors of the large ones.
+//     in registers.  a X is added in the epilogue: inside the chains it would triple
+//     their error.
+//   bf16 input: the products take the hi parts alone (11 bits; the result keeps 8), with
+//     X = (a + B) hi + a lo: a stands on the diagonal of B, which saves reading hi again.
+//     X has both parts because rounding X itself every step would feed the small singular
+//     directions, which a step multiplies by a, with the rounding errors of the large ones.
 //
 // A and A A are symmetric: only tiles on and above the diagonal are computed, and a tile
 // above it is also stored transposed.  X X^T and A A read both operands along k; B X reads
@@ -65,8 +66,8 @@ struct OrthParams {
     int tiles_m, tiles_n, tiles;                 // per matrix
     int chunk_kb, slices;
     Split prev, out;                             // prev: added with `coef`; out: the result
-    int out_parts, prev_parts;
-    float coef, alpha;                           // result = coef * prev + alpha * accumulator (scaled by 2^13)
+    int out_parts;
+    float coef, alpha, diagonal;                 // result = diagonal + coef * prev + alpha * accumulator (scaled by 2^13)
     void* final_out;                             // APPLY, last step: the caller's matrix
     int64_t final_ld, final_stride;
     int final_type, tall, final_vec;
@@ -224,6 +225,9 @@ orth_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     constexpr int COLS = BN / (EPI_WARPS / 4);   // accumulator columns of an epilogue warp
     constexpr int BW = S::BW, PIECES = BW / 8;
     constexpr uint32_t TMEM_COLS = 2 * BN;
+    // what the epilogue adds to the product: A, and X or its low part alone (see the top)
+    constexpr bool READS_HI = WHAT == POLY || (WHAT == APPLY && SPLIT);
+    constexpr bool READS_LO = WHAT == APPLY || (WHAT == POLY && SPLIT);
 
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>(
@@ -416,17 +420,17 @@ orth_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             // blocks of columns this warp has to finish; none where its rows or columns are beyond the matrix
             const int blocks = row0 < p.rows && col0 < p.cols ? min(COLS, p.cols - col0 + BW - 1) / BW : 0;
             const f16* prev = p.prev.p + b * p.prev.batch_stride + static_cast<int64_t>(row0 + by_row) * p.prev.ld + col0 + by_col * 8;
-            auto fetch = [&](int i) {            // block i of prev, asynchronously
+            auto fetch = [&](int i) {            // block i of it, asynchronously
 #pragma unroll
                 for (int it = 0; it < PIECES; ++it) {
                     const int r = it * (32 / PIECES) + by_row;
                     const int bytes = row0 + r < p.rows ? 16 : 0;        // (the pitch covers whole blocks of columns)
                     const f16* src = prev + (bytes ? static_cast<int64_t>(it * (32 / PIECES)) * p.prev.ld + i * BW : 0);
-                    ptx::cp_async_16(buf + piece_at<PIECES>(r, by_col) * 8, src, bytes);
-                    if (p.prev_parts == 2) ptx::cp_async_16(buf_lo + piece_at<PIECES>(r, by_col) * 8, src + p.prev.part_stride, bytes);
+                    if (READS_HI) ptx::cp_async_16(buf + piece_at<PIECES>(r, by_col) * 8, src, bytes);
+                    if (READS_LO) ptx::cp_async_16(buf_lo + piece_at<PIECES>(r, by_col) * 8, src + p.prev.part_stride, bytes);
                 }
             };
-            if constexpr (PAIR && WHAT != GRAM) {
+            if constexpr (PAIR && (READS_HI || READS_LO)) {
                 if (blocks > 0) fetch(0);        // travels while the products run
             }
             if (SPLIT || !PAIR) {
@@ -481,7 +485,7 @@ orth_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                 uint32_t a[BW];
                 if constexpr (BW == 32) ptx::tmem_ld_32x32(lane_base + static_cast<uint32_t>(acc * BN + i * BW), a);
                 else ptx::tmem_ld_32x16(lane_base + static_cast<uint32_t>(acc * BN + i * BW), a);
-                if (WHAT != GRAM) {
+                if (READS_HI || READS_LO) {
                     ptx::cp_async_wait_all();
                     __syncwarp();
                 }
@@ -490,19 +494,20 @@ orth_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
 #pragma unroll
                 for (int c = 0; c < PIECES; ++c) {
                     float h[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-                    if (WHAT != GRAM) {
-                        Raw<f16, 8> x;
-                        if (p.prev_parts == 2) {
-                            load_raw<false>(x, buf_lo + piece_at<PIECES>(lane, c) * 8);
-                            join_f16(h, x);
-                        }
+                    Raw<f16, 8> x;
+                    if (READS_LO) {
+                        load_raw<false>(x, buf_lo + piece_at<PIECES>(lane, c) * 8);
+                        join_f16(h, x);
+                    }
+                    if (READS_HI) {
                         load_raw<false>(x, buf + piece_at<PIECES>(lane, c) * 8);
                         join_f16(h, x);
                     }
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        const float x = __uint_as_float(a[c * 8 + e]) * p.alpha;
-                        v[c * 8 + e] = WHAT != GRAM ? fmaf(p.coef, h[e], x) : x;
+                        const float y = __uint_as_float(a[c * 8 + e]) * p.alpha;
+                        v[c * 8 + e] = READS_HI || READS_LO ? fmaf(p.coef, h[e], y) : y;
+                        if (WHAT == POLY && !SPLIT && row0 + lane == col + c * 8 + e) v[c * 8 + e] += p.diagonal;
                     }
                 }
                 if (WHAT == APPLY && p.final_out) {
@@ -542,13 +547,13 @@ orth_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
                             store_raw<false>(o, x);
                             if (p.out_parts == 2) {
                                 load_raw<false>(x, buf_lo + piece_at<PIECES>(r, by_col) * 8);
-                                store_raw<false>(o + p.out.part_stride, x);
+                                store_raw<!SPLIT>(o + p.out.part_stride, x);
                             }
                         }
                     }
                 }
                 __syncwarp();
-                if (WHAT != GRAM && i + 1 < blocks) fetch(i + 1);
+                if ((READS_HI || READS_LO) && i + 1 < blocks) fetch(i + 1);
             }
             release();
         }
@@ -578,10 +583,10 @@ orth_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             for (int r = warp - 2; r < share; r += EPI_WARPS) {
                 const int row = tm * BM + first + r;
                 const bool in = row < p.rows && col < p.cols;
-                Raw<f16, 4> ph, pl;
-                if (WHAT != GRAM && in) {        // rows have a pitch of a multiple of 64: whole vectors fit
-                    load_raw<false>(ph, prev + static_cast<int64_t>(row) * p.prev.ld);
-                    if (p.prev_parts == 2) load_raw<false>(pl, prev + p.prev.part_stride + static_cast<int64_t>(row) * p.prev.ld);
+                float h[4] = {0.0f, 0.0f, 0.0f, 0.0f}, l[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                if (in) {                        // rows have a pitch of a multiple of 64: whole vectors fit
+                    if (READS_HI) load_f<false>(h, prev + static_cast<int64_t>(row) * p.prev.ld);
+                    if (READS_LO) load_f<false>(l, prev + p.prev.part_stride + static_cast<int64_t>(row) * p.prev.ld);
                 }
                 const uint32_t at = ptx::smem_u32(smem) + static_cast<uint32_t>(((first + r) * PART_LD + lane * 4) * 4);
                 float4 x[MAX_SLICES];
@@ -598,10 +603,8 @@ orth_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     v[e] *= p.alpha;
-                    if (WHAT != GRAM && in) {
-                        const float h = to_f(ph.e[e]);
-                        v[e] = fmaf(p.coef, p.prev_parts == 2 ? h + to_f(pl.e[e]) : h, v[e]);
-                    }
+                    if (READS_HI || READS_LO) v[e] = fmaf(p.coef, h[e] + l[e], v[e]);
+                    if (WHAT == POLY && !SPLIT && row == col + e) v[e] += p.diagonal;
                     if (last) v[e] *= INV_SCALE;
                 }
                 Raw<f16, 4> hi, lo;
@@ -665,8 +668,9 @@ orth_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
 
 // ------------------------------------------------------- norm and first split
 
-// partial[matrix][block]: sums of squares, in fp64 (squares of fp32 numbers leave the fp32
-// range).  Threads walk over whole accesses of VEC elements, eight of them in flight.
+// partial[matrix][block]: sums of squares.  Threads walk over accesses of VEC elements,
+// eight of them in flight.  The squares of an access are added in fp32 where they stay
+// well inside its range, else in fp64; the accesses are added in fp64.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256)
 orth_norm_kernel(double* __restrict__ partial, const T* __restrict__ g, int64_t ld, int64_t stride, int64_t rows,
@@ -683,11 +687,22 @@ orth_norm_kernel(double* __restrict__ partial, const T* __restrict__ g, int64_t 
 #pragma unroll
         for (int k = 0; k < DEEP; ++k) {
             const int64_t i = i0 + k * step;
-            if (i < total) load_raw<false>(r[k], m + (i / nvec) * ld + (i % nvec) * VEC);
+            const int64_t row = total <= UINT32_MAX ? static_cast<uint32_t>(i) / static_cast<uint32_t>(nvec) : i / nvec;
+            if (i < total) load_raw<false>(r[k], m + row * ld + (i - row * nvec) * VEC);
         }
 #pragma unroll
         for (int k = 0; k < DEEP; ++k) {
-            if (i0 + k * step < total) {
+            if (i0 + k * step >= total) continue;
+            float most = 0.0f, sum = 0.0f;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float x = to_f(r[k].e[e]);
+                most = fmaxf(most, fabsf(x));
+                sum = fmaf(x, x, sum);
+            }
+            if (most == 0.0f || (most > 1e-15f && most < 1e15f)) {
+                s += static_cast<double>(sum);
+            } else {
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
                     const double x = static_cast<double>(to_f(r[k].e[e]));
@@ -708,7 +723,7 @@ orth_norm_kernel(double* __restrict__ partial, const T* __restrict__ g, int64_t 
 }
 
 // X0 = G / (|G| + eps) (transposed when TALL) as scaled fp16 parts; 64 x 64 tiles, a thread
-// holds 4 x 4 elements: rows of a tile are read and written 4 columns a lane.
+// has eight neighbouring elements of two rows.
 template <typename T, bool VEC, bool TALL>
 __global__ void __launch_bounds__(256)
 orth_split_kernel(Split x, const double* __restrict__ partial, int parts, const T* __restrict__ g, int64_t ld,
@@ -718,17 +733,17 @@ orth_split_kernel(Split x, const double* __restrict__ partial, int parts, const 
     __shared__ float inv_sh;
     const T* m = g + blockIdx.z * stride;
     const int64_t r0 = static_cast<int64_t>(blockIdx.y) * 64, c0 = static_cast<int64_t>(blockIdx.x) * 64;
-    const int tx = (threadIdx.x & 15) * 4, ty = threadIdx.x >> 4;
-    Raw<T, 4> in[4];                             // requested before the norm is known
+    const int tx = (threadIdx.x & 7) * 8, ty = threadIdx.x >> 3;
+    Raw<T, 8> in[2];                             // requested before the norm is known
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const int64_t r = r0 + ty + k * 16, c = c0 + tx;
+    for (int k = 0; k < 2; ++k) {
+        const int64_t r = r0 + ty + k * 32, c = c0 + tx;
         const T* src = m + r * ld + c;
-        if (VEC && r < rows && c < cols) {       // (the width is a multiple of 4)
+        if (VEC && r < rows && c + 8 <= cols) {
             load_raw<false>(in[k], src);
         } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) in[k].e[e] = r < rows && c + e < cols ? src[e] : from_f<T>(0.0f);
+            for (int e = 0; e < 8; ++e) in[k].e[e] = r < rows && c + e < cols ? src[e] : from_f<T>(0.0f);
         }
     }
     if (threadIdx.x < 32) {
@@ -744,22 +759,20 @@ orth_split_kernel(Split x, const double* __restrict__ partial, int parts, const 
     const int64_t xr0 = TALL ? c0 : r0, xc0 = TALL ? r0 : c0, xrows = TALL ? cols : rows;
     if (TALL) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+        for (int k = 0; k < 2; ++k)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) tile[ty + k * 16][tx + e] = to_f(in[k].e[e]);
+            for (int e = 0; e < 8; ++e) tile[ty + k * 32][tx + e] = to_f(in[k].e[e]);
         __syncthreads();
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const int64_t r = xr0 + ty + k * 16;
+    for (int k = 0; k < 2; ++k) {
+        const int64_t r = xr0 + ty + k * 32;
         if (r >= xrows) continue;
-        Raw<f16, 4> hi, lo;
+        float v[8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float v = (TALL ? tile[tx + e][ty + k * 16] : to_f(in[k].e[e])) * inv;
-            hi.e[e] = __float2half_rn(v);
-            lo.e[e] = __float2half_rn(v - __half2float(hi.e[e]));
-        }
+        for (int e = 0; e < 8; ++e) v[e] = (TALL ? tile[tx + e][ty + k * 32] : to_f(in[k].e[e])) * inv;
+        Raw<f16, 8> hi, lo;
+        split_f16(v, hi, lo);
         f16* o = out + r * x.ld + xc0 + tx;      // the pitch is a multiple of 64: the columns fit
         store_raw<false>(o, hi);
         store_raw<false>(o + x.part_stride, lo);
@@ -849,23 +862,25 @@ int launch_product(sb200_ctx* ctx, const OrthMaps& m, OrthParams p, cudaStream_t
     return err == cudaSuccess && cudaGetLastError() == cudaSuccess ? SB200_OK : SB200_ERR_CUDA;
 }
 
-// Pairs or slices.  A 256 x 256 tile on a pair and a 128 x 128 tile on one SM take about
-// the same time per k-block (the tensor core of the latter waits for shared memory: 128
-// bytes a cycle feed it and take in the tiles), so a pair does four times the work on
-// twice the SMs; slices win where the tiles do not fill the device.  Returns 0 for pairs,
-// else the number of slices.
+// Pairs or slices.  A k-block of a 256 x 256 tile on a pair of SMs takes hardly longer than
+// one of a 128 x 128 tile on one SM (whose tensor core waits for shared memory: 128 bytes a
+// cycle feed it and take in the tiles), so a pair does four times the work on twice the SMs;
+// slices win where the tiles are too few to fill the device.  Both are estimated from
+// measured parts, in us: a launch up to its first tile 2; a k-block 0.36 (pair) and 0.33,
+// with two parts 0.85 and 0.65; the epilogue of a pair 2.8 and 4.5, of a cluster of s slices
+// 2.2 and 5 / s.  Returns 0 for pairs, else the number of slices.
 int slices_for(const sb200_ctx* ctx, int64_t rows, int64_t cols, int64_t batch, int num_kb, bool symmetric, bool split)
 {
     auto tiles = [&](int64_t t) {
         const int64_t tm = (rows + t - 1) / t, tn = (cols + t - 1) / t;
         return (symmetric ? tm * (tm + 1) / 2 : tm * tn) * batch;
     };
-    const int64_t pairs = ctx->sm_count / 2, t1 = tiles(128), t2 = tiles(256);
+    auto waves = [](int64_t n, int64_t at_once) { return static_cast<double>((n + at_once - 1) / at_once); };
+    const int64_t sms = ctx->sm_count, t1 = tiles(128), t2 = tiles(256);
     int s = 1;
-    while (s < MAX_SLICES && 2 * s <= num_kb && t1 * 2 * s <= ctx->sm_count) s *= 2;
-    const double sliced = static_cast<double>((t1 * s + ctx->sm_count - 1) / ctx->sm_count) *
-                          ((num_kb + s - 1) / s * (split ? 0.8 : 1.2) + 4.0);
-    const double paired = static_cast<double>((t2 + pairs - 1) / pairs) * num_kb + (split ? 4.0 : 8.0);
+    while (s < MAX_SLICES && 2 * s <= num_kb && t1 * 2 * s <= sms) s *= 2;
+    const double sliced = waves(t1 * s, sms) * (2.0 + (num_kb + s - 1) / s * (split ? 0.65 : 0.33) + 2.2 + 5.0 / s);
+    const double paired = 2.0 + waves(t2, sms / 2) * num_kb * (split ? 0.85 : 0.36) + (split ? 4.5 : 2.8);
     return sliced < paired ? s : 0;
 }
 
@@ -895,9 +910,11 @@ double largest(F f, double s)
 bool bounded(double a, double b, double c, int steps)
 {
     double s = 1.01;
+    // b s^2 + c s^4 is B's norm, with a in front what stands in its place for bf16
     for (int k = 0; k < steps; ++k) {
         const double m = largest([&](double t) { return b * t * t + c * t * t * t * t; }, s);
-        if (!(s * s < LARGEST) || !(m < LARGEST)) return false;
+        const double d = largest([&](double t) { return a + b * t * t + c * t * t * t * t; }, s);
+        if (!(s * s < LARGEST) || !(m < LARGEST) || !(d < LARGEST)) return false;
         s = 1.01 * largest([&](double t) { return t * (a + b * t * t + c * t * t * t * t); }, s);
     }
     return true;
@@ -996,26 +1013,22 @@ extern "C" int sb200_orthogonalize(sb200_ctx* ctx, void* out, int64_t ldo, int64
         p.rows = p.cols = p.R;
         p.num_kb = kb_c;
         p.chunk_kb = q.split ? CHUNK_KB : kb_c;
-        p.prev = A;
-        p.prev_parts = 0;
-        p.out = A;
+        p.prev = p.out = A;
         p.out_parts = q.split ? 2 : 1;
-        p.coef = 0.0f;
         p.alpha = INV_SCALE;
         p.final_out = nullptr;
         if (const int rc = product<GRAM>(ctx, q.split, {x_rows[from], x_rows[from]}, p, stream)) return rc;
-        // B = b A + c A A
+        // B = b A + c A A (+ a on the diagonal)
         p.num_kb = kb_r;
         p.chunk_kb = q.split ? CHUNK_KB : kb_r;
-        p.prev_parts = p.out_parts;
         p.out = B;
         p.coef = b;
         p.alpha = c * INV_SCALE;
+        p.diagonal = a * SCALE;
         if (const int rc = product<POLY>(ctx, q.split, {a_rows, a_rows}, p, stream)) return rc;
         // X = a X + B X
         p.cols = p.C;
         p.prev = X[from];
-        p.prev_parts = 2;
         p.out = X[to];
         p.out_parts = 2;
         p.coef = a;
