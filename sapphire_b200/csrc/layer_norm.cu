@@ -9,11 +9,21 @@
 // x and dy and write dx.  A row is read once, held in the registers of the threads that
 // share it (a group of 1 to 32 lanes, or a block of up to 512 threads, 16 elements a
 // thread), and its sums are taken over those registers, so the variance is the mean of
-// squared differences from the mean, not a difference of large sums.  All sums are
-// fp32.  The blocks walk over rows; in the backward pass every thread therefore keeps
-// the column sums of its own columns in registers over all the rows its block sees,
-// writes one partial sum a block, and a second kernel adds the partials in block order:
-// no atomics, the same bits run to run.
+// squared differences from a mean, not a difference of large sums.  All sums are fp32.
+// The blocks walk over rows; each thread keeps its columns' weights in registers and has
+// its pieces of the next rows on the way into shared memory (its own slots, so nothing
+// but the thread itself waits for them): the memory system always has several rows a
+// block to work on, which one row at a time in registers does not give it (65536 x 4096
+// bf16 forward: 291 us).  In the backward pass every thread keeps the column sums of its
+// columns in registers over all the rows its block sees, writes one partial sum a block,
+// and a second kernel adds the partials in block order: no atomics, the same bits run to
+// run.  Rows that 16-byte accesses do not fit take 4-byte ones, odd rows of 16-bit
+// elements 2-byte ones.
+#include <initializer_list>
+#include <type_traits>
+#include <utility>
+
+#include "ptx.cuh"
 #include "typed.cuh"
 
 namespace sb200 {
@@ -21,28 +31,68 @@ namespace {
 
 constexpr int EPT = 16;                 // elements of a row per thread
 constexpr int MAX_THREADS = 512;        // threads per row at most
+constexpr int MAX_WARPS = MAX_THREADS / 32;
 constexpr int REGISTER_COLS = EPT * MAX_THREADS;
 constexpr int GROUP_BLOCK = 256;        // block size when a row belongs to a warp or less
 
-// Sum over the threads that share a row.  WARP: the `lanes` (power of two) neighbouring
-// lanes; otherwise the block, through one barrier: callers alternate between two
-// buffers, so that a buffer is written again only after a later barrier.
-template <bool WARP>
-__device__ __forceinline__ float row_sum(float v, int lanes, float* buf)
-{
-    if constexpr (WARP) {
-        for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        return v;
-    } else {
+// A thread's pieces of the coming rows of one array, in shared memory: STAGES rows of EPT
+// elements, piece s of stage k at [(k * NV + s) * blockDim + thread].  2-byte accesses have
+// no asynchronous form: those pieces are read when the row is due.
+template <typename T, int VEC>
+struct Pieces {
+    static constexpr int NV = EPT / VEC, BYTES = VEC * static_cast<int>(sizeof(T));
+    static constexpr bool ASYNC = BYTES >= 4;
+    static_assert(BYTES == 2 || BYTES == 4 || BYTES == 16, "access width");
+    static constexpr int STAGES = !ASYNC ? 1 : sizeof(T) == 4 ? 3 : 4, AHEAD = STAGES - 1;
+    static constexpr int SMEM = ASYNC ? STAGES * EPT * static_cast<int>(sizeof(T)) : 0;      // per thread
+
+    Raw<T, VEC> next[ASYNC ? 1 : NV];
+    unsigned char* base;
+
+    // pieces beyond the row are zero and stay so
+    __device__ void init(unsigned char* smem, int lane, int lanes, int nvec)
+    {
+        base = smem + threadIdx.x * BYTES;
+        Raw<T, VEC> zero;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
-        __syncthreads();
-        float s = 0.0f;
-        for (int i = 0; i < static_cast<int>(blockDim.x >> 5); ++i) s += buf[i];
-        return s;
+        for (int i = 0; i < VEC; ++i) zero.e[i] = from_f<T>(0.0f);
+#pragma unroll
+        for (int s = 0; s < NV; ++s) {
+            if constexpr (ASYNC) {
+                for (int k = 0; k < STAGES; ++k)
+                    if (s * lanes + lane >= nvec) store_raw<false>(reinterpret_cast<T*>(slot(k, s)), zero);
+            } else {
+                next[s] = zero;
+            }
+        }
     }
-}
+    __device__ unsigned char* slot(int stage, int s) const { return base + (stage * NV + s) * static_cast<int>(blockDim.x) * BYTES; }
+
+    // the pieces of the row at `row` (in: whether there is one) into a stage
+    __device__ void request(const T* row, bool in, int stage, int lane, int lanes, int nvec)
+    {
+        if (!in) return;
+        row += static_cast<int64_t>(lane) * VEC;
+        if constexpr (ASYNC) {
+#pragma unroll 4
+            for (int s = 0; s < NV; ++s) {
+                if (s * lanes + lane >= nvec) break;
+                if constexpr (BYTES == 16) ptx::cp_async_16(slot(stage, s), row, 16);
+                else ptx::cp_async_4(slot(stage, s), row);
+                row += lanes * VEC;
+            }
+        } else {
+#pragma unroll
+            for (int s = 0; s < NV; ++s)
+                if (s * lanes + lane < nvec) load_raw<true>(next[s], row + s * lanes * VEC);
+        }
+    }
+    __device__ void get(Raw<T, VEC>& r, int stage, int s) const
+    {
+        if constexpr (ASYNC) load_raw<false>(r, reinterpret_cast<const T*>(slot(stage, s)));
+        else r = next[s];
+    }
+};
 
 template <typename W, int VEC>
 __device__ __forceinline__ void load_weight(float (&f)[VEC], const W* w, int64_t col, float none)
@@ -55,56 +105,114 @@ __device__ __forceinline__ void load_weight(float (&f)[VEC], const W* w, int64_t
     }
 }
 
+__device__ __forceinline__ float lanes_sum(float v, int lanes)
+{
+    for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
 // `lanes` threads per row (blockDim.x of them when WARP is false).
+// 80 registers: three blocks of 256 threads an SM (element by element the addresses need more).
 template <typename T, typename W, int VEC, bool WARP>
-__global__ void __launch_bounds__(MAX_THREADS)
+__global__ void __maxnreg__(VEC == 1 ? 128 : 80)
 ln_forward_kernel(T* y, int64_t ldy, float* __restrict__ mean_out, float* __restrict__ rstd_out, const T* x,
                   int64_t ldx, const W* __restrict__ w, const W* __restrict__ b, int64_t rows, int cols, float eps,
                   int lanes)
 {
-    constexpr int NV = EPT / VEC;
-    __shared__ float buf[2][MAX_THREADS / 32];
+    using P = Pieces<T, VEC>;
+    constexpr int NV = P::NV, AHEAD = P::AHEAD;
+    extern __shared__ __align__(16) unsigned char smem[];
+    // a warp's sum and sum of squared differences from its own mean; two buffers, so that
+    // one barrier a row is enough: a buffer is written again behind the other one's barrier
+    __shared__ float2 part[2][MAX_WARPS], count[MAX_WARPS];      // count: elements of a warp, and 1 / that
     const int lane = WARP ? (threadIdx.x & (lanes - 1)) : threadIdx.x;
     const int64_t group = WARP ? (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / lanes : blockIdx.x;
     const int64_t groups = WARP ? static_cast<int64_t>(gridDim.x) * blockDim.x / lanes : gridDim.x;
     const int nvec = cols / VEC;
     const float inv_n = 1.0f / static_cast<float>(cols);
+    // elements in this thread's warp (or group)
+    int mine = 0;
+#pragma unroll
+    for (int s = 0; s < NV; ++s) mine += s * lanes + lane < nvec ? VEC : 0;
+    const float warp_n = lanes_sum(static_cast<float>(mine), WARP ? lanes : 32);
+    const float warp_inv = warp_n > 0.0f ? 1.0f / warp_n : 0.0f;
+    if (!WARP && (threadIdx.x & 31) == 0) count[threadIdx.x >> 5] = make_float2(warp_n, warp_inv);   // (read behind a barrier)
+
+    P px;
+    px.init(smem, lane, lanes, nvec);
+    float wf[EPT], bf[EPT];
+#pragma unroll
+    for (int s = 0; s < NV; ++s) {
+        float a[VEC], c[VEC];
+        const int v = s * lanes + lane;
+        if (v < nvec) {
+            load_weight(a, w, static_cast<int64_t>(v) * VEC, 1.0f);
+            load_weight(c, b, static_cast<int64_t>(v) * VEC, 0.0f);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) { wf[s * VEC + i] = a[i]; bf[s * VEC + i] = c[i]; }
+        }
+    }
     // every lane of a warp makes the same number of trips: the shuffles name all of them
     const int64_t first = WARP ? group - (threadIdx.x & 31) / lanes : group;
-    for (int64_t r0 = first; r0 < rows; r0 += groups) {
-        const int64_t r = r0 + (group - first);
-        const bool mine = r < rows;
-        Raw<T, VEC> raw[NV];
-        const T* xr = x + r * ldx;
+    const int64_t off = group - first;
 #pragma unroll
-        for (int s = 0; s < NV; ++s) {
-            const int v = s * lanes + lane;
-            if (mine && v < nvec) load_raw<true>(raw[s], xr + static_cast<int64_t>(v) * VEC);
-        }
+    for (int k = 0; k < AHEAD; ++k) {
+        const int64_t r = first + k * groups + off;
+        px.request(x + r * ldx, r < rows, k, lane, lanes, nvec);
+        if (P::ASYNC) ptx::cp_async_commit();
+    }
+    int stage = 0, flip = 0;
+    for (int64_t r0 = first; r0 < rows; r0 += groups) {
+        const int64_t r = r0 + off;
+        const bool has = r < rows;
+        if constexpr (P::ASYNC) ptx::cp_async_wait<AHEAD - 1>();
+        else px.request(x + r * ldx, has, 0, lane, lanes, nvec);
         float f[EPT], sum = 0.0f;
 #pragma unroll
         for (int s = 0; s < NV; ++s) {
-            const bool in = mine && s * lanes + lane < nvec;
+            Raw<T, VEC> raw;
+            px.get(raw, stage, s);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-                f[s * VEC + i] = in ? to_f(raw[s].e[i]) : 0.0f;
+                f[s * VEC + i] = to_f(raw.e[i]);
                 sum += f[s * VEC + i];
             }
         }
-        const float mean = row_sum<WARP>(sum, lanes, buf[0]) * inv_n;
+        if constexpr (P::ASYNC) {
+            const int64_t rn = r + AHEAD * groups;
+            px.request(x + rn * ldx, rn < rows, (stage + AHEAD) % P::STAGES, lane, lanes, nvec);
+            ptx::cp_async_commit();
+            stage = stage + 1 == P::STAGES ? 0 : stage + 1;
+        }
+        sum = lanes_sum(sum, WARP ? lanes : 32);
+        const float near = sum * warp_inv;               // the mean over this warp's elements
         float sq = 0.0f;
 #pragma unroll
         for (int s = 0; s < NV; ++s) {
             const bool in = s * lanes + lane < nvec;
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-                f[s * VEC + i] -= mean;
-                if (in) sq = fmaf(f[s * VEC + i], f[s * VEC + i], sq);
+                const float d = f[s * VEC + i] - near;
+                if (in) sq = fmaf(d, d, sq);
             }
         }
-        const float var = row_sum<WARP>(sq, lanes, buf[1]) * inv_n;
-        const float rstd = 1.0f / sqrtf(var + eps);
-        if (mine && lane == 0) {
+        sq = lanes_sum(sq, WARP ? lanes : 32);
+        float mean = near;
+        if (!WARP) {
+            // the squares from the common mean: those from the warp's own, and its distance
+            float2* p = part[flip];
+            flip ^= 1;
+            if ((threadIdx.x & 31) == 0) p[threadIdx.x >> 5] = make_float2(sum, sq);
+            __syncthreads();
+            const int i = threadIdx.x & (MAX_WARPS - 1);
+            const bool in = i < static_cast<int>(blockDim.x >> 5);
+            const float2 q = in ? p[i] : make_float2(0.0f, 0.0f), n = in ? count[i] : make_float2(0.0f, 0.0f);
+            mean = lanes_sum(q.x, MAX_WARPS) * inv_n;
+            const float d = fmaf(q.x, n.y, -mean);
+            sq = lanes_sum(fmaf(n.x * d, d, q.y), MAX_WARPS);
+        }
+        const float rstd = rsqrtf(sq * inv_n + eps);
+        if (has && lane == 0) {
             if (mean_out) mean_out[r] = mean;
             if (rstd_out) rstd_out[r] = rstd;
         }
@@ -112,112 +220,175 @@ ln_forward_kernel(T* y, int64_t ldy, float* __restrict__ mean_out, float* __rest
 #pragma unroll
         for (int s = 0; s < NV; ++s) {
             const int v = s * lanes + lane;
-            if (!mine || v >= nvec) continue;
-            float wf[VEC], bf[VEC], o[VEC];
-            load_weight(wf, w, static_cast<int64_t>(v) * VEC, 1.0f);
-            load_weight(bf, b, static_cast<int64_t>(v) * VEC, 0.0f);
+            if (!has || v >= nvec) continue;
+            float o[VEC];
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) o[i] = fmaf(f[s * VEC + i] * rstd, wf[i], bf[i]);
+            for (int i = 0; i < VEC; ++i) o[i] = fmaf((f[s * VEC + i] - mean) * rstd, wf[s * VEC + i], bf[s * VEC + i]);
             store_f<true>(yr + static_cast<int64_t>(v) * VEC, o);
         }
     }
 }
 
+// Sum over a block (rows too long for registers); `buf` is one of two used in turn.
+__device__ __forceinline__ float2 block_sum(float2 v, float2* buf)
+{
+    v.x = lanes_sum(v.x, 32);
+    v.y = lanes_sum(v.y, 32);
+    if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
+    __syncthreads();
+    float2 s = make_float2(0.0f, 0.0f);
+    for (int i = 0; i < static_cast<int>(blockDim.x >> 5); ++i) { s.x += buf[i].x; s.y += buf[i].y; }
+    return s;
+}
+
 // Rows too long for registers: three passes over the row, which the caches hold.
-template <typename T, typename W>
+template <typename T, typename W, int VEC>
 __global__ void __launch_bounds__(MAX_THREADS)
 ln_forward_long_kernel(T* y, int64_t ldy, float* __restrict__ mean_out, float* __restrict__ rstd_out, const T* x,
                        int64_t ldx, const W* __restrict__ w, const W* __restrict__ b, int64_t rows, int64_t cols,
                        float eps)
 {
-    __shared__ float buf[2][MAX_THREADS / 32];
+    __shared__ float2 buf[2][MAX_WARPS];
+    const int64_t nvec = cols / VEC;
     for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
         const T* xr = x + r * ldx;
         float sum = 0.0f;
-        for (int64_t j = threadIdx.x; j < cols; j += blockDim.x) sum += to_f(xr[j]);
-        const float mean = row_sum<false>(sum, 0, buf[0]) / static_cast<float>(cols);
-        float sq = 0.0f;
-        for (int64_t j = threadIdx.x; j < cols; j += blockDim.x) {
-            const float d = to_f(xr[j]) - mean;
-            sq = fmaf(d, d, sq);
+#pragma unroll 4
+        for (int64_t v = threadIdx.x; v < nvec; v += blockDim.x) {
+            float f[VEC];
+            load_f<false>(f, xr + v * VEC);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) sum += f[i];
         }
-        const float rstd = 1.0f / sqrtf(row_sum<false>(sq, 0, buf[1]) / static_cast<float>(cols) + eps);
+        const float mean = block_sum(make_float2(sum, 0.0f), buf[0]).x / static_cast<float>(cols);
+        float sq = 0.0f;
+#pragma unroll 4
+        for (int64_t v = threadIdx.x; v < nvec; v += blockDim.x) {
+            float f[VEC];
+            load_f<false>(f, xr + v * VEC);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) sq = fmaf(f[i] - mean, f[i] - mean, sq);
+        }
+        const float rstd = rsqrtf(block_sum(make_float2(sq, 0.0f), buf[1]).x / static_cast<float>(cols) + eps);
         if (threadIdx.x == 0) {
             if (mean_out) mean_out[r] = mean;
             if (rstd_out) rstd_out[r] = rstd;
         }
         T* yr = y + r * ldy;
-        for (int64_t j = threadIdx.x; j < cols; j += blockDim.x)
-            yr[j] = from_f<T>(fmaf((to_f(xr[j]) - mean) * rstd, w ? to_f(w[j]) : 1.0f, b ? to_f(b[j]) : 0.0f));
+#pragma unroll 2
+        for (int64_t v = threadIdx.x; v < nvec; v += blockDim.x) {
+            float f[VEC], wf[VEC], bf[VEC];
+            load_f<true>(f, xr + v * VEC);
+            load_weight(wf, w, v * VEC, 1.0f);
+            load_weight(bf, b, v * VEC, 0.0f);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) f[i] = fmaf((f[i] - mean) * rstd, wf[i], bf[i]);
+            store_f<true>(yr + v * VEC, f);
+        }
     }
 }
 
 // ---------------------------------------------------------------- backward pass
 
 // partial: [2][gridDim.x][cols] column sums of this block's rows (dweight, then dbias), or null.
-// Dynamic shared memory (WARP, partial != null): 2 * cols floats.
+// Dynamic shared memory: the pieces of x and dy, and later (WARP, partial != null) 2 * cols floats.
 template <typename T, typename W, int VEC, bool WARP>
 __global__ void __launch_bounds__(MAX_THREADS)
 ln_backward_kernel(T* dx, int64_t lddx, float* __restrict__ partial, const T* dy, int64_t lddy, const T* x,
                    int64_t ldx, const W* __restrict__ w, const float* __restrict__ mean_in,
                    const float* __restrict__ rstd_in, int64_t rows, int cols, int accumulate, int lanes)
 {
-    constexpr int NV = EPT / VEC;
-    __shared__ float buf[4][MAX_THREADS / 32];
-    extern __shared__ float cols_sum[];
+    using P = Pieces<T, VEC>;
+    constexpr int NV = P::NV, AHEAD = P::AHEAD;
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ float2 part[2][MAX_WARPS];                // two buffers, one barrier a row
     const int lane = WARP ? (threadIdx.x & (lanes - 1)) : threadIdx.x;
     const int64_t group = WARP ? (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / lanes : blockIdx.x;
     const int64_t groups = WARP ? static_cast<int64_t>(gridDim.x) * blockDim.x / lanes : gridDim.x;
     const int nvec = cols / VEC;
     const float inv_n = 1.0f / static_cast<float>(cols);
-    float dw[EPT], db[EPT];
+    P px, py;
+    px.init(smem, lane, lanes, nvec);
+    py.init(smem + blockDim.x * P::SMEM, lane, lanes, nvec);
+    float dw[EPT], db[EPT], wf[EPT];
 #pragma unroll
-    for (int i = 0; i < EPT; ++i) dw[i] = db[i] = 0.0f;
-    const int64_t first = WARP ? group - (threadIdx.x & 31) / lanes : group;
-    int flip = 0;
-    for (int64_t r0 = first; r0 < rows; r0 += groups, flip ^= 2) {
-        const int64_t r = r0 + (group - first);
-        const bool mine = r < rows;
-        Raw<T, VEC> rx[NV], ry[NV];
-        const T* xr = x + r * ldx;
-        const T* yr = dy + r * lddy;
+    for (int i = 0; i < EPT; ++i) dw[i] = db[i] = wf[i] = 0.0f;
 #pragma unroll
-        for (int s = 0; s < NV; ++s) {
-            const int v = s * lanes + lane;
-            if (mine && v < nvec) {
-                load_raw<true>(rx[s], xr + static_cast<int64_t>(v) * VEC);
-                load_raw<true>(ry[s], yr + static_cast<int64_t>(v) * VEC);
-            }
+    for (int s = 0; s < NV; ++s) {
+        const int v = s * lanes + lane;
+        if (v < nvec) {
+            float a[VEC];
+            load_weight(a, w, static_cast<int64_t>(v) * VEC, 1.0f);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) wf[s * VEC + i] = a[i];
         }
-        const float mean = mine ? mean_in[r] : 0.0f, rstd = mine ? rstd_in[r] : 0.0f;
-        float h[EPT], g[EPT], s1 = 0.0f, s2 = 0.0f;
+    }
+    const int64_t first = WARP ? group - (threadIdx.x & 31) / lanes : group;
+    const int64_t off = group - first;
+    auto request = [&](int64_t r, int stage) {
+        px.request(x + r * ldx, r < rows, stage, lane, lanes, nvec);
+        py.request(dy + r * lddy, r < rows, stage, lane, lanes, nvec);
+        if (P::ASYNC) ptx::cp_async_commit();
+    };
 #pragma unroll
-        for (int s = 0; s < NV; ++s) {
-            const int v = s * lanes + lane;
-            if (mine && v < nvec) {
-                float wf[VEC];
-                load_weight(wf, w, static_cast<int64_t>(v) * VEC, 1.0f);
+    for (int k = 0; k < AHEAD; ++k) request(first + k * groups + off, k);
+    float mean_next = first + off < rows ? mean_in[first + off] : 0.0f;
+    float rstd_next = first + off < rows ? rstd_in[first + off] : 0.0f;
+    int stage = 0, flip = 0;
+    for (int64_t r0 = first; r0 < rows; r0 += groups) {
+        const int64_t r = r0 + off;
+        const bool has = r < rows;
+        const float mean = mean_next, rstd = rstd_next;
+        if constexpr (P::ASYNC) ptx::cp_async_wait<AHEAD - 1>();
+        else request(r, 0);
+        float h[EPT], d[EPT], s1 = 0.0f, s2 = 0.0f;
+        if (!WARP || has) {
+            // (beyond the row dy is zero, and so is all that is added up)
+#pragma unroll
+            for (int s = 0; s < NV; ++s) {
+                Raw<T, VEC> rx, ry;
+                px.get(rx, stage, s);
+                py.get(ry, stage, s);
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
                     const int k = s * VEC + i;
-                    const float d = to_f(ry[s].e[i]);
-                    h[k] = (to_f(rx[s].e[i]) - mean) * rstd;
-                    dw[k] = fmaf(d, h[k], dw[k]);
-                    db[k] += d;
-                    g[k] = d * wf[i];
-                    s1 += g[k];
-                    s2 = fmaf(g[k], h[k], s2);
+                    h[k] = (to_f(rx.e[i]) - mean) * rstd;
+                    d[k] = to_f(ry.e[i]);
+                    dw[k] = fmaf(d[k], h[k], dw[k]);
+                    db[k] += d[k];
+                    const float g = d[k] * wf[k];
+                    s1 += g;
+                    s2 = fmaf(g, h[k], s2);
                 }
             }
         }
-        const float m1 = row_sum<WARP>(s1, lanes, buf[flip]) * inv_n;
-        const float m2 = row_sum<WARP>(s2, lanes, buf[flip + 1]) * inv_n;
+        if (r + groups < rows) {
+            mean_next = mean_in[r + groups];
+            rstd_next = rstd_in[r + groups];
+        }
+        if constexpr (P::ASYNC) {
+            request(r + AHEAD * groups, (stage + AHEAD) % P::STAGES);
+            stage = stage + 1 == P::STAGES ? 0 : stage + 1;
+        }
+        s1 = lanes_sum(s1, WARP ? lanes : 32);
+        s2 = lanes_sum(s2, WARP ? lanes : 32);
+        if (!WARP) {
+            float2* p = part[flip];
+            flip ^= 1;
+            if ((threadIdx.x & 31) == 0) p[threadIdx.x >> 5] = make_float2(s1, s2);
+            __syncthreads();
+            const int i = threadIdx.x & (MAX_WARPS - 1);
+            const float2 q = i < static_cast<int>(blockDim.x >> 5) ? p[i] : make_float2(0.0f, 0.0f);
+            s1 = lanes_sum(q.x, MAX_WARPS);
+            s2 = lanes_sum(q.y, MAX_WARPS);
+        }
         if (dx) {
+            const float m1 = s1 * inv_n, m2 = s2 * inv_n;
             T* dr = dx + r * lddx;
 #pragma unroll
             for (int s = 0; s < NV; ++s) {
                 const int v = s * lanes + lane;
-                if (!mine || v >= nvec) continue;
+                if (!has || v >= nvec) continue;
                 float o[VEC];
                 if (accumulate) {
                     load_f<true>(o, dr + static_cast<int64_t>(v) * VEC);
@@ -228,7 +399,7 @@ ln_backward_kernel(T* dx, int64_t lddx, float* __restrict__ partial, const T* dy
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
                     const int k = s * VEC + i;
-                    o[i] += rstd * (g[k] - m1 - h[k] * m2);
+                    o[i] += rstd * (d[k] * wf[k] - m1 - h[k] * m2);
                 }
                 store_f<true>(dr + static_cast<int64_t>(v) * VEC, o);
             }
@@ -250,7 +421,9 @@ ln_backward_kernel(T* dx, int64_t lddx, float* __restrict__ partial, const T* dy
         }
         return;
     }
-    // the groups of the block one after another, in order
+    // the groups of the block one after another, in order; the pieces' place is free
+    float* cols_sum = reinterpret_cast<float*>(smem);
+    __syncthreads();
     for (int j = threadIdx.x; j < 2 * cols; j += blockDim.x) cols_sum[j] = 0.0f;
     const int my_group = threadIdx.x / lanes;
     for (int gi = 0; gi < static_cast<int>(blockDim.x) / lanes; ++gi) {
@@ -275,32 +448,51 @@ ln_backward_kernel(T* dx, int64_t lddx, float* __restrict__ partial, const T* dy
 }
 
 // Rows too long for registers: dx with two passes over the row, column sums separately.
-template <typename T, typename W>
+template <typename T, typename W, int VEC>
 __global__ void __launch_bounds__(MAX_THREADS)
 ln_backward_long_kernel(T* dx, int64_t lddx, const T* dy, int64_t lddy, const T* x, int64_t ldx,
                         const W* __restrict__ w, const float* __restrict__ mean_in,
                         const float* __restrict__ rstd_in, int64_t rows, int64_t cols, int accumulate)
 {
-    __shared__ float buf[4][MAX_THREADS / 32];
+    __shared__ float2 buf[2][MAX_WARPS];
+    const int64_t nvec = cols / VEC;
     int flip = 0;
-    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x, flip ^= 2) {
+    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x, flip ^= 1) {
         const T* xr = x + r * ldx;
         const T* yr = dy + r * lddy;
         const float mean = mean_in[r], rstd = rstd_in[r];
-        float s1 = 0.0f, s2 = 0.0f;
-        for (int64_t j = threadIdx.x; j < cols; j += blockDim.x) {
-            const float g = to_f(yr[j]) * (w ? to_f(w[j]) : 1.0f);
-            s1 += g;
-            s2 = fmaf(g, (to_f(xr[j]) - mean) * rstd, s2);
+        float2 s = make_float2(0.0f, 0.0f);
+#pragma unroll 2
+        for (int64_t v = threadIdx.x; v < nvec; v += blockDim.x) {
+            float f[VEC], g[VEC], wf[VEC];
+            load_f<false>(f, xr + v * VEC);
+            load_f<false>(g, yr + v * VEC);
+            load_weight(wf, w, v * VEC, 1.0f);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                g[i] *= wf[i];
+                s.x += g[i];
+                s.y = fmaf(g[i], (f[i] - mean) * rstd, s.y);
+            }
         }
-        const float m1 = row_sum<false>(s1, 0, buf[flip]) / static_cast<float>(cols);
-        const float m2 = row_sum<false>(s2, 0, buf[flip + 1]) / static_cast<float>(cols);
+        s = block_sum(s, buf[flip]);
+        const float m1 = s.x / static_cast<float>(cols), m2 = s.y / static_cast<float>(cols);
         T* dr = dx + r * lddx;
-        for (int64_t j = threadIdx.x; j < cols; j += blockDim.x) {
-            const float g = to_f(yr[j]) * (w ? to_f(w[j]) : 1.0f);
-            const float h = (to_f(xr[j]) - mean) * rstd;
-            const float o = rstd * (g - m1 - h * m2);
-            dr[j] = from_f<T>(accumulate ? to_f(dr[j]) + o : o);
+#pragma unroll 2
+        for (int64_t v = threadIdx.x; v < nvec; v += blockDim.x) {
+            float f[VEC], g[VEC], wf[VEC], o[VEC];
+            load_f<false>(f, xr + v * VEC);
+            load_f<false>(g, yr + v * VEC);
+            load_weight(wf, w, v * VEC, 1.0f);
+            if (accumulate) {
+                load_f<false>(o, dr + v * VEC);
+            } else {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) o[i] = 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) o[i] += rstd * (g[i] * wf[i] - m1 - (f[i] - mean) * rstd * m2);
+            store_f<true>(dr + v * VEC, o);
         }
     }
 }
@@ -317,6 +509,7 @@ ln_backward_long_cols_kernel(float* __restrict__ partial, const T* __restrict__ 
     const int64_t per = (rows + gridDim.y - 1) / gridDim.y;
     const int64_t r0 = blockIdx.y * per, r1 = r0 + per < rows ? r0 + per : rows;
     float dw = 0.0f, db = 0.0f;
+#pragma unroll 8
     for (int64_t r = r0; r < r1; ++r) {
         const float d = to_f(dy[r * lddy + j]);
         dw = fmaf(d, (to_f(x[r * ldx + j]) - mean_in[r]) * rstd_in[r], dw);
@@ -357,14 +550,6 @@ ln_reduce_kernel(W* __restrict__ dweight, W* __restrict__ dbias, const float* __
 
 // ------------------------------------------------------------------------- host
 
-struct Shape {
-    int64_t rows, cols;
-    bool vec;           // 16-byte accesses are allowed
-    bool is_long;
-    int lanes, block;   // threads per row, threads per block
-    int64_t grid;       // blocks: enough to fill the device, no more than there is work
-};
-
 int power_of_two_at_least(int64_t n)
 {
     int p = 1;
@@ -372,29 +557,75 @@ int power_of_two_at_least(int64_t n)
     return p;
 }
 
-Shape shape_of(int sm_count, int64_t rows, int64_t cols, int vec_elems, bool vec)
+struct Shape {
+    int lanes, block;   // threads per row, threads per block
+    int64_t blocks;     // that the rows give work to
+};
+
+Shape shape_of(int64_t rows, int64_t cols, int vec)
 {
     Shape s{};
-    s.rows = rows;
-    s.cols = cols;
-    s.vec = vec;
-    s.is_long = cols > REGISTER_COLS;
-    const int64_t nvec = vec ? cols / vec_elems : cols;
-    const int64_t slots = vec ? EPT / vec_elems : EPT;
-    const int64_t threads = (nvec + slots - 1) / slots;
-    if (s.is_long) {
-        s.lanes = s.block = MAX_THREADS;
-    } else if (threads <= 32) {
+    const int64_t threads = cols > REGISTER_COLS ? MAX_THREADS : (cols / vec + EPT / vec - 1) / (EPT / vec);
+    if (threads <= 32) {
         s.lanes = power_of_two_at_least(threads);
         s.block = GROUP_BLOCK;
     } else {
         s.lanes = s.block = static_cast<int>((threads + 31) / 32 * 32);
     }
     const int64_t per_block = s.block / s.lanes;
-    const int64_t want = (rows + per_block - 1) / per_block;
-    const int64_t fill = static_cast<int64_t>(sm_count) * (1024 / s.block);
-    s.grid = want < fill ? want : fill;
+    s.blocks = (rows + per_block - 1) / per_block;
     return s;
+}
+
+// A kernel as a type: what is remembered about it is remembered per kernel, not per signature.
+template <auto K>
+struct Kernel {
+    static constexpr auto run = K;
+};
+
+// How many blocks of this size the device holds at once (asked once per kernel, size and device).
+template <auto K>
+int64_t resident_blocks(const sb200_ctx* ctx, Kernel<K>, int block, int smem)
+{
+    constexpr int DEVICES = 16;
+    static int per_sm[DEVICES][MAX_WARPS + 1] = {};
+    int ask = 0;
+    int& n = ctx->device < DEVICES ? per_sm[ctx->device][block / 32] : ask;
+    if (n == 0) {
+        int got = 0;
+        if (smem > 40 * 1024 && cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return 0;
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&got, K, block, smem) != cudaSuccess) return 0;
+        n = got;
+    }
+    return static_cast<int64_t>(n) * ctx->sm_count;
+}
+
+// The widest access (elements) that fits all rows and the weights: 16, 4 or the element's own bytes.
+template <typename T, typename W>
+int access_width(int64_t cols, const void* w, const void* b, std::initializer_list<std::pair<const void*, int64_t>> arrays)
+{
+    for (int bytes : {16, 4}) {
+        const int vec = bytes / static_cast<int>(sizeof(T));
+        const size_t weights = vec * sizeof(W) < 16 ? vec * sizeof(W) : 16;
+        bool ok = cols % vec == 0 && aligned_to(w, weights) && aligned_to(b, weights);
+        for (const auto& a : arrays) ok = ok && a.second % vec == 0 && aligned_to(a.first, bytes);
+        if (ok) return vec;
+    }
+    return 1;
+}
+
+template <int N>
+using Int = std::integral_constant<int, N>;
+
+// f(Int<vec>{}) for an access width of access_width()
+template <typename T, typename F>
+int with_width(int vec, F f)
+{
+    if (vec == 16 / static_cast<int>(sizeof(T))) return f(Int<16 / static_cast<int>(sizeof(T))>{});
+    if constexpr (sizeof(T) == 2) {
+        if (vec == 2) return f(Int<2>{});
+    }
+    return f(Int<1>{});
 }
 
 int check_types(int type, int weight_type)
@@ -444,31 +675,27 @@ extern "C" int sb200_layer_norm(sb200_ctx* ctx, void* y, int64_t ldy, float* mea
     DeviceGuard dev(ctx->device);
     if (!dev.ok) return SB200_ERR_CUDA;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-    return with_types(type, weight_type, [&](auto t, auto wt) {
+    return with_types(type, weight_type, [&](auto t, auto wt) -> int {
         using T = decltype(t);
         using W = decltype(wt);
-        constexpr int VEC = 16 / sizeof(T);
-        const bool vec = cols % VEC == 0 && ldx % VEC == 0 && ldy % VEC == 0 && aligned_to(x, 16) && aligned_to(y, 16) &&
-                         aligned_to(weight, 16) && aligned_to(bias, 16);
-        const Shape s = shape_of(ctx->sm_count, rows, cols, VEC, vec);
-        const unsigned grid = static_cast<unsigned>(s.grid);
-        T* yp = static_cast<T*>(y);
-        const T* xp = static_cast<const T*>(x);
-        const W* wp = static_cast<const W*>(weight);
-        const W* bp = static_cast<const W*>(bias);
-        const int n = static_cast<int>(s.is_long ? 0 : cols);
-        if (s.is_long)
-            ln_forward_long_kernel<T, W><<<grid, s.block, 0, stream>>>(yp, ldy, mean, rstd, xp, ldx, wp, bp, rows, cols, eps);
-        else if (s.lanes <= 32 && vec)
-            ln_forward_kernel<T, W, VEC, true><<<grid, s.block, 0, stream>>>(yp, ldy, mean, rstd, xp, ldx, wp, bp, rows, n, eps, s.lanes);
-        else if (s.lanes <= 32)
-            ln_forward_kernel<T, W, 1, true><<<grid, s.block, 0, stream>>>(yp, ldy, mean, rstd, xp, ldx, wp, bp, rows, n, eps, s.lanes);
-        else if (vec)
-            ln_forward_kernel<T, W, VEC, false><<<grid, s.block, 0, stream>>>(yp, ldy, mean, rstd, xp, ldx, wp, bp, rows, n, eps, s.lanes);
-        else
-            ln_forward_kernel<T, W, 1, false><<<grid, s.block, 0, stream>>>(yp, ldy, mean, rstd, xp, ldx, wp, bp, rows, n, eps, s.lanes);
-        ctx->launches += 1;
-        return cudaGetLastError() == cudaSuccess ? SB200_OK : SB200_ERR_CUDA;
+        const int width = access_width<T, W>(cols, weight, bias, {{x, ldx}, {y, ldy}});
+        return with_width<T>(width, [&](auto v) -> int {
+            constexpr int VEC = decltype(v)::value;
+            const Shape s = shape_of(rows, cols, VEC);
+            auto launch = [&](auto kern, int smem, auto... last) -> int {
+                const int64_t most = resident_blocks(ctx, kern, s.block, smem);
+                if (most < 1) return SB200_ERR_CUDA;
+                kern.run<<<static_cast<unsigned>(s.blocks < most ? s.blocks : most), s.block, smem, stream>>>(
+                    static_cast<T*>(y), ldy, mean, rstd, static_cast<const T*>(x), ldx, static_cast<const W*>(weight),
+                    static_cast<const W*>(bias), rows, last...);
+                ctx->launches += 1;
+                return static_cast<int>(cudaGetLastError() == cudaSuccess ? SB200_OK : SB200_ERR_CUDA);
+            };
+            const int smem = s.block * Pieces<T, VEC>::SMEM, n = static_cast<int>(cols > REGISTER_COLS ? 0 : cols);
+            if (cols > REGISTER_COLS) return launch(Kernel<ln_forward_long_kernel<T, W, VEC>>{}, 0, cols, eps);
+            if (s.lanes <= 32) return launch(Kernel<ln_forward_kernel<T, W, VEC, true>>{}, smem, n, eps, s.lanes);
+            return launch(Kernel<ln_forward_kernel<T, W, VEC, false>>{}, smem, n, eps, s.lanes);
+        });
     });
 }
 
@@ -497,56 +724,62 @@ extern "C" int sb200_layer_norm_backward(sb200_ctx* ctx, void* dx, int64_t lddx,
     if (!dev.ok) return SB200_ERR_CUDA;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     float* partial = sums ? static_cast<float*>(workspace) : nullptr;
-    return with_types(type, weight_type, [&](auto t, auto wt) {
+    return with_types(type, weight_type, [&](auto t, auto wt) -> int {
         using T = decltype(t);
         using W = decltype(wt);
-        constexpr int VEC = 16 / sizeof(T);
         T* dxp = static_cast<T*>(dx);
         const T* yp = static_cast<const T*>(dy);
         const T* xp = static_cast<const T*>(x);
         const W* wp = static_cast<const W*>(weight);
         int parts = 0;
         if (rows > 0) {
-            const bool vec = cols % VEC == 0 && ldx % VEC == 0 && lddy % VEC == 0 && aligned_to(x, 16) &&
-                             aligned_to(dy, 16) && aligned_to(weight, 16) &&
-                             (!dx || (lddx % VEC == 0 && aligned_to(dx, 16)));
-            const Shape s = shape_of(ctx->sm_count, rows, cols, VEC, vec);
-            const int64_t most = backward_parts(ctx->sm_count, rows, cols);
-            if (s.is_long) {
-                // the column sums first: dx may overwrite dy
-                if (sums) {
-                    parts = static_cast<int>(most);
-                    const dim3 grid(static_cast<unsigned>((cols + 255) / 256), static_cast<unsigned>(parts));
-                    ln_backward_long_cols_kernel<T><<<grid, 256, 0, stream>>>(partial, yp, lddy, xp, ldx, mean, rstd, rows, cols);
-                    ctx->launches += 1;
+            const int width = dx ? access_width<T, W>(cols, weight, nullptr, {{x, ldx}, {dy, lddy}, {dx, lddx}})
+                                 : access_width<T, W>(cols, weight, nullptr, {{x, ldx}, {dy, lddy}});
+            const int64_t bound = backward_parts(ctx->sm_count, rows, cols);
+            const int rc = with_width<T>(width, [&](auto v) -> int {
+                constexpr int VEC = decltype(v)::value;
+                const Shape s = shape_of(rows, cols, VEC);
+                if (cols > REGISTER_COLS) {
+                    // the column sums first: dx may overwrite dy
+                    if (sums) {
+                        parts = static_cast<int>(bound);
+                        const dim3 grid(static_cast<unsigned>((cols + 255) / 256), static_cast<unsigned>(parts));
+                        ln_backward_long_cols_kernel<T><<<grid, 256, 0, stream>>>(partial, yp, lddy, xp, ldx, mean, rstd, rows, cols);
+                        ctx->launches += 1;
+                    }
+                    if (dx) {
+                        Kernel<ln_backward_long_kernel<T, W, VEC>> kern;
+                        const int64_t most = resident_blocks(ctx, kern, s.block, 0);
+                        if (most < 1) return SB200_ERR_CUDA;
+                        kern.run<<<static_cast<unsigned>(s.blocks < most ? s.blocks : most), s.block, 0, stream>>>(
+                            dxp, lddx, yp, lddy, xp, ldx, wp, mean, rstd, rows, cols, accumulate_dx);
+                        ctx->launches += 1;
+                    }
+                    return SB200_OK;
                 }
-                if (dx) {
-                    ln_backward_long_kernel<T, W><<<static_cast<unsigned>(s.grid), s.block, 0, stream>>>(
-                        dxp, lddx, yp, lddy, xp, ldx, wp, mean, rstd, rows, cols, accumulate_dx);
-                    ctx->launches += 1;
-                }
-            } else {
-                const int64_t want = s.grid < most ? s.grid : most;
-                parts = static_cast<int>(want);
-                const unsigned grid = static_cast<unsigned>(want);
                 const int n = static_cast<int>(cols);
-                const size_t smem = s.lanes <= 32 && sums ? static_cast<size_t>(2 * cols) * sizeof(float) : 0;
-                if (s.lanes <= 32 && vec)
-                    ln_backward_kernel<T, W, VEC, true><<<grid, s.block, smem, stream>>>(dxp, lddx, partial, yp, lddy, xp, ldx, wp, mean, rstd, rows, n, accumulate_dx, s.lanes);
-                else if (s.lanes <= 32)
-                    ln_backward_kernel<T, W, 1, true><<<grid, s.block, smem, stream>>>(dxp, lddx, partial, yp, lddy, xp, ldx, wp, mean, rstd, rows, n, accumulate_dx, s.lanes);
-                else if (vec)
-                    ln_backward_kernel<T, W, VEC, false><<<grid, s.block, 0, stream>>>(dxp, lddx, partial, yp, lddy, xp, ldx, wp, mean, rstd, rows, n, accumulate_dx, s.lanes);
-                else
-                    ln_backward_kernel<T, W, 1, false><<<grid, s.block, 0, stream>>>(dxp, lddx, partial, yp, lddy, xp, ldx, wp, mean, rstd, rows, n, accumulate_dx, s.lanes);
-                ctx->launches += 1;
-            }
+                auto launch = [&](auto kern) -> int {
+                    int smem = 2 * s.block * Pieces<T, VEC>::SMEM;
+                    if (s.lanes <= 32 && smem < 2 * 32 * EPT * 4) smem = 2 * 32 * EPT * 4;      // column sums of such rows
+                    const int64_t most = resident_blocks(ctx, kern, s.block, smem);
+                    if (most < 1) return SB200_ERR_CUDA;
+                    int64_t grid = s.blocks < most ? s.blocks : most;
+                    if (grid > bound) grid = bound;
+                    parts = static_cast<int>(grid);
+                    kern.run<<<static_cast<unsigned>(grid), s.block, smem, stream>>>(dxp, lddx, partial, yp, lddy, xp, ldx, wp, mean, rstd, rows, n,
+                                                                                 accumulate_dx, s.lanes);
+                    ctx->launches += 1;
+                    return SB200_OK;
+                };
+                return s.lanes <= 32 ? launch(Kernel<ln_backward_kernel<T, W, VEC, true>>{}) : launch(Kernel<ln_backward_kernel<T, W, VEC, false>>{});
+            });
+            if (rc) return rc;
         }
         if (sums) {
             const dim3 grid(static_cast<unsigned>((cols + 31) / 32), 2);
             ln_reduce_kernel<W><<<grid, 1024, 0, stream>>>(static_cast<W*>(dweight), static_cast<W*>(dbias), partial, parts, cols, accumulate_weight);
             ctx->launches += 1;
         }
-        return cudaGetLastError() == cudaSuccess ? SB200_OK : SB200_ERR_CUDA;
+        return static_cast<int>(cudaGetLastError() == cudaSuccess ? SB200_OK : SB200_ERR_CUDA);
     });
 }

@@ -125,6 +125,24 @@ __device__ __forceinline__ void cp_async_16(void* smem_dst, const void* src, int
                  : "memory");
 }
 
+// 4 bytes, through the L1.
+__device__ __forceinline__ void cp_async_4(void* smem_dst, const void* src)
+{
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(smem_dst)), "l"(src) : "memory");
+}
+
+__device__ __forceinline__ void cp_async_commit()
+{
+    asm volatile("cp.async.commit_group;" ::: "memory");
+}
+
+// Until at most N of this thread's newest groups of copies are pending.
+template <int N>
+__device__ __forceinline__ void cp_async_wait()
+{
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 // Until all of this thread's copies have landed.
 __device__ __forceinline__ void cp_async_wait_all()
 {
