@@ -893,29 +893,46 @@ int product(sb200_ctx* ctx, bool split, const OrthMaps& m, OrthParams p, cudaStr
     return split ? launch_product<WHAT, false, true>(ctx, m, p, stream) : launch_product<WHAT, false, false>(ctx, m, p, stream);
 }
 
-// Largest |f| of an odd or even polynomial over [0, s], by its samples: the polynomials
-// are smooth, 1024 samples are within a thousandth of the maximum.
+// Largest |f(u)| over [0, top]: at its ends or where the derivative d0 + d1 u + d2 u^2 is zero.
 template <typename F>
-double largest(F f, double s)
+double largest(F f, double top, double d0, double d1, double d2)
 {
     double m = 0.0;
-    for (int i = 0; i <= 1024; ++i) {
-        const double v = std::fabs(f(s * i / 1024.0));
-        if (!(v <= m)) m = v;
+    auto look = [&](double u) {
+        const double v = std::fabs(f(u));
+        if (!(v <= m)) m = v;                    // (not a number counts as larger)
+    };
+    look(0.0);
+    look(top);
+    double root[2] = {-1.0, -1.0};
+    if (d2 != 0.0) {
+        const double disc = d1 * d1 - 4.0 * d2 * d0;
+        if (disc >= 0.0) {
+            const double h = -0.5 * (d1 + std::copysign(std::sqrt(disc), d1));
+            root[0] = h / d2;
+            if (h != 0.0) root[1] = d0 / h;
+        }
+    } else if (d1 != 0.0) {
+        root[0] = -d0 / d1;
     }
+    for (double u : root)
+        if (u > 0.0 && u < top) look(u);
     return m;
 }
 
-// Whether every matrix of the iteration stays inside the range of the scaled fp16 parts.
+// Whether every matrix of the iteration stays inside the range of the scaled fp16 parts:
+// s bounds the singular values of X, b s^2 + c s^4 is B's norm, with a in front the norm of
+// what stands in its place for bf16.  One per cent is for rounding.
 bool bounded(double a, double b, double c, int steps)
 {
+    if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) return false;
     double s = 1.01;
-    // b s^2 + c s^4 is B's norm, with a in front what stands in its place for bf16
     for (int k = 0; k < steps; ++k) {
-        const double m = largest([&](double t) { return b * t * t + c * t * t * t * t; }, s);
-        const double d = largest([&](double t) { return a + b * t * t + c * t * t * t * t; }, s);
-        if (!(s * s < LARGEST) || !(m < LARGEST) || !(d < LARGEST)) return false;
-        s = 1.01 * largest([&](double t) { return t * (a + b * t * t + c * t * t * t * t); }, s);
+        const double top = s * s;                // in u = s^2
+        const double m = largest([&](double u) { return b * u + c * u * u; }, top, b, 2.0 * c, 0.0);
+        const double d = largest([&](double u) { return a + b * u + c * u * u; }, top, b, 2.0 * c, 0.0);
+        if (!(top < LARGEST) || !(m < LARGEST) || !(d < LARGEST)) return false;
+        s = 1.01 * largest([&](double u) { return std::sqrt(u) * (a + b * u + c * u * u); }, top, a, 3.0 * b, 5.0 * c);
     }
     return true;
 }

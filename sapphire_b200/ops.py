@@ -25,6 +25,7 @@ class Context:
         if not torch.cuda.is_available():
             raise RuntimeError("sapphire_b200 needs a CUDA device (sm_100a); there is no CPU path")
         self.device = int(device)
+        self.torch_device = torch.device("cuda", self.device)
         h = C.c_void_p()
         L.check("sb200_ctx_create", L.lib().sb200_ctx_create(self.device, C.byref(h)))
         self._h = h
@@ -394,9 +395,19 @@ def scale(ctx, x, factor, out=None):
 
 
 # ---------------------------------------------------- operators of token models
+# These are called on small tensors too, where what bounds them is this side: a
+# contiguous tensor takes the short way through the checks, and what is allocated here
+# is not checked again.
 
 _TYPE = {torch.float32: L.F32, torch.bfloat16: L.BF16, torch.float16: L.F16}
 _INDEX_BITS = {torch.int32: 32, torch.int64: 64}
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or _stream_ptr
+
+
+def _call(name: str, ctx: Context, *args) -> None:
+    rc = getattr(L.lib(), name)(ctx._h, *args, _raw_stream(ctx.device))
+    if rc:
+        raise L.Sb200Error(name, rc)
 
 
 def _type_code(t: torch.Tensor, what: str) -> int:
@@ -407,53 +418,65 @@ def _type_code(t: torch.Tensor, what: str) -> int:
 
 
 def _on_device(ctx: Context, t: torch.Tensor, what: str) -> None:
-    if not t.is_cuda or t.device.index != ctx.device:
+    if t.get_device() != ctx.device:
         raise ValueError(f"{what} must be on cuda:{ctx.device}, got {t.device}")
 
 
 def _rows(ctx: Context, t: torch.Tensor, what: str):
     """(rows, cols, row pitch) of a tensor seen as rows of its contiguous last dimension;
     the leading dimensions must be equally spaced rows."""
-    _on_device(ctx, t, what)
-    if t.dim() < 1:
+    if t.get_device() != ctx.device:
+        _on_device(ctx, t, what)
+    shape = t.shape
+    if not shape:
         raise ValueError(f"{what} needs a last dimension")
-    cols = t.shape[-1]
-    if t.dim() == 2:
-        rows, pitch, inner = t.shape[0], t.stride(0), t.stride(1)
-    elif t.is_contiguous():
-        rows, pitch, inner = (t.numel() // cols if cols else 0), cols, 1
-    else:
-        inner, rows, pitch = t.stride(-1), 1, None
-        for size, step in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
-            if size == 1:
-                continue
-            if pitch is None:
-                pitch = step
-            elif step != pitch * rows:
-                raise ValueError(f"{what}: the rows must be equally spaced")
-            rows *= size
-    if cols > 1 and inner != 1:
+    cols = shape[-1]
+    if t.is_contiguous():
+        return (t.numel() // cols if cols else 0), cols, cols
+    stride = t.stride()
+    if cols > 1 and stride[-1] != 1:
         raise ValueError(f"{what}: the last dimension must be contiguous")
-    if rows <= 1 or pitch is None:
-        pitch = cols if pitch is None or pitch < cols else pitch
-    elif pitch < cols:
+    rows, pitch = 1, None
+    for size, step in zip(reversed(shape[:-1]), reversed(stride[:-1])):
+        if size == 1:
+            continue
+        if pitch is None:
+            pitch = step
+        elif step != pitch * rows:
+            raise ValueError(f"{what}: the rows must be equally spaced")
+        rows *= size
+    if pitch is None:
+        pitch = cols
+    elif pitch < cols and rows > 1:
         raise ValueError(f"{what}: rows overlap")
-    return rows, cols, pitch
+    return rows, cols, max(pitch, cols)
+
+
+def _like(t: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor of t's shape and dtype."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 def _vector(ctx: Context, t: torch.Tensor, n: int, what: str) -> int:
-    _on_device(ctx, t, what)
+    if t.get_device() != ctx.device:
+        _on_device(ctx, t, what)
     if t.numel() != n or not t.is_contiguous():
         raise ValueError(f"{what} must be a contiguous vector of {n} elements")
     return t.data_ptr()
 
 
-def _scratch(name: str, nbytes: int, ctx: Context):
+def _statistic(ctx: Context, t: torch.Tensor, n: int, what: str) -> int:
+    if t.dtype != torch.float32:
+        raise TypeError(f"{what} is float32")
+    return _vector(ctx, t, n, what)
+
+
+def _scratch(name: str, nbytes: int, ctx: Context) -> torch.Tensor:
     """A workspace from torch's allocator: it belongs to the current stream, and inside a
     graph capture to the graph."""
     if nbytes < 0:
         raise L.Sb200Error(name, L.ERR_TOO_LARGE)
-    return torch.empty(max(nbytes, 1), dtype=torch.uint8, device=torch.device("cuda", ctx.device))
+    return torch.empty(nbytes or 1, dtype=torch.uint8, device=ctx.torch_device)
 
 
 def _ids(ctx: Context, ids: torch.Tensor):
@@ -475,14 +498,15 @@ def embedding(ctx: Context, table: torch.Tensor, ids: torch.Tensor, *, scale: fl
     vocab, cols, ldt = _rows(ctx, table, "table")
     ids, bits = _ids(ctx, ids)
     if out is None:
-        out = torch.empty(*ids.shape, cols, dtype=out_dtype or table.dtype, device=table.device)
-    elif out_dtype is not None and out.dtype != out_dtype:
-        raise TypeError("out has another dtype than out_dtype")
-    elif out.shape != (*ids.shape, cols):
-        raise ValueError("out must be [*ids.shape, cols]")
-    _, _, ldo = _rows(ctx, out, "out")
-    _ew("sb200_embedding", ctx, out.data_ptr(), ldo, table.data_ptr(), ldt, ids.data_ptr(), bits, ids.numel(), vocab,
-        cols, scale, _type_code(table, "table"), _type_code(out, "out"))
+        out, ldo = torch.empty((*ids.shape, cols), dtype=out_dtype or table.dtype, device=ctx.torch_device), cols
+    else:
+        if out_dtype is not None and out.dtype != out_dtype:
+            raise TypeError("out has another dtype than out_dtype")
+        if out.shape != (*ids.shape, cols):
+            raise ValueError("out must be [*ids.shape, cols]")
+        ldo = _rows(ctx, out, "out")[2]
+    _call("sb200_embedding", ctx, out.data_ptr(), ldo, table.data_ptr(), ldt, ids.data_ptr(), bits, ids.numel(), vocab,
+          cols, scale, _type_code(table, "table"), _type_code(out, "out"))
     return out
 
 
@@ -497,13 +521,24 @@ def embedding_backward(ctx: Context, dtable: torch.Tensor, dout: torch.Tensor, i
     ids, bits = _ids(ctx, ids)
     if dout.shape != (*ids.shape, cols):
         raise ValueError("dout must be [*ids.shape, cols]")
-    _, _, ldo = _rows(ctx, dout, "dout")
-    n = ids.numel()
-    ws = _scratch("sb200_embedding_backward",
-                  L.lib().sb200_embedding_backward_workspace(ctx.handle, n, vocab, cols), ctx)
-    _ew("sb200_embedding_backward", ctx, dtable.data_ptr(), ldt, dout.data_ptr(), ldo, ids.data_ptr(), bits, n, vocab,
-        cols, scale, _type_code(dtable, "dtable"), _type_code(dout, "dout"), int(accumulate), ws.data_ptr(), ws.numel())
+    ldo, n = _rows(ctx, dout, "dout")[2], ids.numel()
+    nbytes = L.lib().sb200_embedding_backward_workspace(ctx._h, n, vocab, cols)
+    ws = _scratch("sb200_embedding_backward", nbytes, ctx)
+    _call("sb200_embedding_backward", ctx, dtable.data_ptr(), ldt, dout.data_ptr(), ldo, ids.data_ptr(), bits, n, vocab,
+          cols, scale, _type_code(dtable, "dtable"), _type_code(dout, "dout"), int(accumulate), ws.data_ptr(), nbytes)
     return dtable
+
+
+def _norm_weights(ctx, cols, code, weight, bias, names):
+    """(type code, pointer, pointer) of two vectors of one dtype, either of which may be None."""
+    wcode, wptr, bptr = code, None, None
+    if weight is not None:
+        wcode, wptr = _type_code(weight, names[0]), _vector(ctx, weight, cols, names[0])
+        if bias is not None and bias.dtype != weight.dtype:
+            raise TypeError(f"{names[0]} and {names[1]} must have one dtype")
+    if bias is not None:
+        wcode, bptr = _type_code(bias, names[1]), _vector(ctx, bias, cols, names[1])
+    return wcode, wptr, bptr
 
 
 def layer_norm(ctx: Context, x: torch.Tensor, weight: Optional[torch.Tensor] = None,
@@ -513,34 +548,21 @@ def layer_norm(ctx: Context, x: torch.Tensor, weight: Optional[torch.Tensor] = N
     the leading shape, as the backward pass wants them.  ``out`` may be ``x``.  weight and
     bias are of x's dtype or float32."""
     rows, cols, ldx = _rows(ctx, x, "x")
-    if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    elif out.shape != x.shape or out.dtype != x.dtype:
-        raise ValueError("out must have x's shape and dtype")
-    if mean is None:
-        mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    if rstd is None:
-        rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    if mean.dtype != torch.float32 or rstd.dtype != torch.float32:
-        raise TypeError("mean and rstd are float32")
     code = _type_code(x, "x")
-    wcode, wptr, bptr = _norm_weights(ctx, cols, code, weight, bias)
-    _, _, ldo = _rows(ctx, out, "out")
-    _ew("sb200_layer_norm", ctx, out.data_ptr(), ldo, _vector(ctx, mean, rows, "mean"), _vector(ctx, rstd, rows, "rstd"),
-        x.data_ptr(), ldx, wptr, bptr, rows, cols, eps, code, wcode)
+    if out is None:
+        out, ldo = _like(x), cols
+    else:
+        if out.shape != x.shape or out.dtype != x.dtype:
+            raise ValueError("out must have x's shape and dtype")
+        ldo = _rows(ctx, out, "out")[2]
+    if mean is None:
+        mean = torch.empty(rows if x.dim() == 2 else x.shape[:-1], dtype=torch.float32, device=ctx.torch_device)
+    if rstd is None:
+        rstd = torch.empty_like(mean)
+    wcode, wptr, bptr = _norm_weights(ctx, cols, code, weight, bias, ("weight", "bias"))
+    _call("sb200_layer_norm", ctx, out.data_ptr(), ldo, _statistic(ctx, mean, rows, "mean"),
+          _statistic(ctx, rstd, rows, "rstd"), x.data_ptr(), ldx, wptr, bptr, rows, cols, eps, code, wcode)
     return out, mean, rstd
-
-
-def _norm_weights(ctx, cols, code, weight, bias, names=("weight", "bias")):
-    """(type code, pointer, pointer) of two vectors of one dtype, either of which may be None."""
-    wcode = code
-    for t, what in zip((weight, bias), names):
-        if t is not None:
-            wcode = _type_code(t, what)
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise TypeError(f"{names[0]} and {names[1]} must have one dtype")
-    return (wcode, None if weight is None else _vector(ctx, weight, cols, names[0]),
-            None if bias is None else _vector(ctx, bias, cols, names[1]))
 
 
 def layer_norm_backward(ctx: Context, dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
@@ -552,33 +574,32 @@ def layer_norm_backward(ctx: Context, dy: torch.Tensor, x: torch.Tensor, mean: t
     residual branch's gradient), ``accumulate_weight`` to dweight and dbias (further
     micro-batches): the buffers concerned must then be given.  ``dx`` may be ``dy``."""
     rows, cols, ldx = _rows(ctx, x, "x")
+    code = _type_code(x, "x")
     if dy.shape != x.shape or dy.dtype != x.dtype:
         raise ValueError("dy must have x's shape and dtype")
-    _, _, ldy = _rows(ctx, dy, "dy")
+    ldy = _rows(ctx, dy, "dy")[2]
     if (accumulate_dx and dx is None) or (accumulate_weight and (dweight is None or dbias is None)):
         raise ValueError("accumulating needs the buffers that are added to")
-    if mean.dtype != torch.float32 or rstd.dtype != torch.float32:
-        raise TypeError("mean and rstd are float32")
     if dx is None:
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    elif dx.shape != x.shape or dx.dtype != x.dtype:
-        raise ValueError("dx must have x's shape and dtype")
-    code = _type_code(x, "x")
+        dx, lddx = _like(x), cols
+    else:
+        if dx.shape != x.shape or dx.dtype != x.dtype:
+            raise ValueError("dx must have x's shape and dtype")
+        lddx = _rows(ctx, dx, "dx")[2]
     wdtype = weight.dtype if weight is not None else dweight.dtype if dweight is not None else x.dtype
     if dweight is None:
-        dweight = torch.empty(cols, dtype=wdtype, device=x.device)
+        dweight = torch.empty(cols, dtype=wdtype, device=ctx.torch_device)
     if dbias is None:
-        dbias = torch.empty(cols, dtype=wdtype, device=x.device)
-    if dweight.dtype != wdtype or dbias.dtype != wdtype:
-        raise TypeError("dweight and dbias must have the weight's dtype")
+        dbias = torch.empty(cols, dtype=wdtype, device=ctx.torch_device)
     wcode, dwptr, dbptr = _norm_weights(ctx, cols, code, dweight, dbias, ("dweight", "dbias"))
-    _, _, lddx = _rows(ctx, dx, "dx")
-    ws = _scratch("sb200_layer_norm_backward",
-                  L.lib().sb200_layer_norm_backward_workspace(ctx.handle, rows, cols), ctx)
-    _ew("sb200_layer_norm_backward", ctx, dx.data_ptr(), lddx, dwptr, dbptr, dy.data_ptr(), ldy, x.data_ptr(), ldx,
-        None if weight is None else _vector(ctx, weight, cols, "weight"), _vector(ctx, mean, rows, "mean"),
-        _vector(ctx, rstd, rows, "rstd"), rows, cols, code, wcode, int(accumulate_dx), int(accumulate_weight),
-        ws.data_ptr(), ws.numel())
+    if dweight.dtype != wdtype:
+        raise TypeError("dweight and dbias must have the weight's dtype")
+    nbytes = L.lib().sb200_layer_norm_backward_workspace(ctx._h, rows, cols)
+    ws = _scratch("sb200_layer_norm_backward", nbytes, ctx)
+    _call("sb200_layer_norm_backward", ctx, dx.data_ptr(), lddx, dwptr, dbptr, dy.data_ptr(), ldy, x.data_ptr(), ldx,
+          None if weight is None else _vector(ctx, weight, cols, "weight"), _statistic(ctx, mean, rows, "mean"),
+          _statistic(ctx, rstd, rows, "rstd"), rows, cols, code, wcode, int(accumulate_dx), int(accumulate_weight),
+          ws.data_ptr(), nbytes)
     return dx, dweight, dbias
 
 
@@ -590,11 +611,11 @@ def orthogonalize(ctx: Context, g: torch.Tensor, *, steps: int = 5, coefficients
     ``sgd_update``."""
     if g.dim() not in (2, 3):
         raise ValueError("expected [rows, cols] or [batch, rows, cols]")
+    code = _type_code(g, "g")
     if out is None:
-        out = torch.empty(g.shape, dtype=g.dtype, device=g.device)
+        out = _like(g)
     elif out.shape != g.shape or out.dtype != g.dtype:
         raise ValueError("out must have g's shape and dtype")
-    code = _type_code(g, "g")
     batch = g.shape[0] if g.dim() == 3 else 1
     (rows, cols), geometry = g.shape[-2:], []
     for t, what in ((out, "out"), (g, "g")):
@@ -604,6 +625,7 @@ def orthogonalize(ctx: Context, g: torch.Tensor, *, steps: int = 5, coefficients
         ld = t.stride(-2) if rows > 1 else max(cols, t.stride(-2))
         geometry += [t.data_ptr(), ld, t.stride(0) if t.dim() == 3 else 0]
     a, b, c = coefficients
-    ws = _scratch("sb200_orthogonalize", L.lib().sb200_orthogonalize_workspace(rows, cols, batch, code), ctx)
-    _ew("sb200_orthogonalize", ctx, *geometry, rows, cols, batch, int(steps), a, b, c, eps, code, ws.data_ptr(), ws.numel())
+    nbytes = L.lib().sb200_orthogonalize_workspace(rows, cols, batch, code)
+    ws = _scratch("sb200_orthogonalize", nbytes, ctx)
+    _call("sb200_orthogonalize", ctx, *geometry, rows, cols, batch, int(steps), a, b, c, eps, code, ws.data_ptr(), nbytes)
     return out
