@@ -9,20 +9,26 @@
 //
 // The gradient needs the tokens of one vocabulary row together and in a fixed order, so
 // that the sum is the same run to run.  The token positions are sorted by vocabulary row
-// with a stable radix sort (9 bits a pass: two passes up to 262143 rows); the sorted list
-// is cut into pieces of equal length, whatever rows they hold, so that a frequent token
-// does not make one block slow; a block adds up the runs of its piece, stores the runs
-// that lie inside it and leaves the sums of a run that crosses into a neighbour to a
-// second kernel that adds them in order.
+// with a stable radix sort (9 bits a pass: two passes up to 262143 rows): up to 16384
+// tokens by one block in shared memory, while the other SMs fill the table with zeros;
+// more by up to 64 blocks, two launches a pass, which also mark the rows that occur, so
+// that only the others are filled.  The sorted list is cut into pieces of equal length,
+// whatever rows they hold, so that a frequent token does not make one block slow; a block
+// adds up the runs that start in its piece, up to a piece's length beyond its end.  Runs
+// longer than a piece leave a partial sum in every piece they touch, and a second kernel
+// adds those in order; it works through a list of these runs (one block a piece, most of
+// them with nothing to join, took 99 us where the sums took 129).
 #include <type_traits>
 
+#include "ptx.cuh"
 #include "typed.cuh"
 
 namespace sb200 {
 namespace {
 
 constexpr int LOOKUP_THREADS = 256;
-constexpr int LOOKUP_ROWS = 4;           // tokens a thread has in flight
+template <int VEC>
+constexpr int LOOKUP_ROWS = VEC >= 4 ? 4 : 8;          // tokens a thread has in flight
 
 __device__ __forceinline__ void report_range(unsigned* status) { atomicCAS(status, 0u, static_cast<unsigned>(FAULT_TOKEN_RANGE)); }
 
@@ -33,12 +39,13 @@ lookup_kernel(TA* __restrict__ out, int64_t ldo, const TT* __restrict__ table, i
               const I* __restrict__ ids, int64_t n, int64_t vocab, int nvec, float scale, int lanes,
               unsigned* status)
 {
+    constexpr int ROWS = LOOKUP_ROWS<VEC>;
     const int lane = threadIdx.x & (lanes - 1);
     const int per_block = LOOKUP_THREADS / lanes;
-    const int64_t t0 = (static_cast<int64_t>(blockIdx.x) * per_block) * LOOKUP_ROWS + threadIdx.x / lanes;
-    int64_t id[LOOKUP_ROWS];
+    const int64_t t0 = (static_cast<int64_t>(blockIdx.x) * per_block) * ROWS + threadIdx.x / lanes;
+    int64_t id[ROWS];
 #pragma unroll
-    for (int k = 0; k < LOOKUP_ROWS; ++k) {
+    for (int k = 0; k < ROWS; ++k) {
         const int64_t t = t0 + static_cast<int64_t>(k) * per_block;
         id[k] = t < n ? static_cast<int64_t>(ids[t]) : -1;
         if (id[k] >= vocab) {
@@ -47,12 +54,12 @@ lookup_kernel(TA* __restrict__ out, int64_t ldo, const TT* __restrict__ table, i
         }
     }
     for (int v = lane; v < nvec; v += lanes) {
-        Raw<TT, VEC> r[LOOKUP_ROWS];
+        Raw<TT, VEC> r[ROWS];
 #pragma unroll
-        for (int k = 0; k < LOOKUP_ROWS; ++k)
+        for (int k = 0; k < ROWS; ++k)
             if (id[k] >= 0) load_raw<false>(r[k], table + id[k] * ldt + static_cast<int64_t>(v) * VEC);
 #pragma unroll
-        for (int k = 0; k < LOOKUP_ROWS; ++k) {
+        for (int k = 0; k < ROWS; ++k) {
             const int64_t t = t0 + static_cast<int64_t>(k) * per_block;
             if (t >= n) continue;
             float f[VEC];
@@ -198,28 +205,132 @@ sort_scatter_kernel(uint32_t* __restrict__ keys_out, uint32_t* __restrict__ pos_
     }
 }
 
+// ------------------------------------------------------------- sort by one block
+
+constexpr int SMALL_ROUNDS = 16;                             // items a thread at most
+constexpr int SMALL_TOKENS = SORT_THREADS * SMALL_ROUNDS;
+constexpr int SMALL_SMEM = SMALL_TOKENS * 6 + SORT_WARPS * DIGITS * 2 + DIGITS * 4 + SORT_WARPS * 4;
+
+// Fills rows [v0, v1) with zeros, those marked in `touched` (if any) left out; `lanes` (power
+// of two) threads a row.
+template <typename TT, int VEC>
+__device__ __forceinline__ void zero_rows(TT* dtable, int64_t ldt, int64_t nvec, int64_t v0, int64_t v1,
+                                          const uint32_t* touched)
+{
+    Raw<TT, VEC> zero;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) zero.e[i] = from_f<TT>(0.0f);
+    int lanes = 1;
+    while (lanes < nvec && lanes < static_cast<int>(blockDim.x)) lanes <<= 1;
+    const int lane = threadIdx.x & (lanes - 1), rows = blockDim.x / lanes;
+    for (int64_t v = v0 + threadIdx.x / lanes; v < v1; v += rows) {
+        if (touched && ((touched[v >> 5] >> (v & 31)) & 1u)) continue;
+        TT* row = dtable + v * ldt;
+#pragma unroll 4
+        for (int64_t k = lane; k < nvec; k += lanes) store_raw<true>(row + k * VEC, zero);
+    }
+}
+
+// Block 0 sorts n <= SMALL_TOKENS tokens; the others fill dtable (null: none of them) with zeros.
+// A whole pass in shared memory: an item's place is (items of smaller digits) + (items of its
+// digit in the warps before) + (its rank in its warp).
+template <typename I, typename TT, int VEC>
+__global__ void __launch_bounds__(SORT_THREADS)
+sort_small_kernel(uint32_t* __restrict__ keys_out, uint32_t* __restrict__ pos_out, uint32_t* __restrict__ long_runs,
+                  const I* __restrict__ ids, int n, int64_t vocab, int passes, TT* __restrict__ dtable, int64_t ldt,
+                  int64_t nvec, unsigned* status)
+{
+    ptx::griddep_launch_dependents();
+    if (blockIdx.x > 0) {
+        // neighbouring rows to a block, so that its stores are neighbours
+        const int64_t per = (vocab + gridDim.x - 2) / (gridDim.x - 1), v0 = (blockIdx.x - 1) * per;
+        zero_rows<TT, VEC>(dtable, ldt, nvec, v0, min(vocab, v0 + per), nullptr);
+        return;
+    }
+    extern __shared__ __align__(16) unsigned char smem[];
+    uint32_t* skey = reinterpret_cast<uint32_t*>(smem);
+    uint32_t* offset = skey + SMALL_TOKENS;
+    uint32_t* scan = offset + DIGITS;
+    unsigned short* ahead = reinterpret_cast<unsigned short*>(scan + SORT_WARPS);      // [SORT_WARPS][DIGITS]
+    unsigned short* spos = ahead + SORT_WARPS * DIGITS;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rounds = (n + SORT_THREADS - 1) / SORT_THREADS;
+    const int i0 = warp * rounds * 32 + lane;
+    if (threadIdx.x == 0) *long_runs = 0;
+    for (int pass = 0; pass < passes; ++pass) {
+        const int shift = pass * DIGIT_BITS;
+        for (int d = threadIdx.x; d < SORT_WARPS * DIGITS / 2; d += SORT_THREADS) reinterpret_cast<uint32_t*>(ahead)[d] = 0;
+        __syncthreads();
+        uint32_t key[SMALL_ROUNDS], where[SMALL_ROUNDS];     // where: rank in the warp << 16 | position in ids
+#pragma unroll
+        for (int k = 0; k < SMALL_ROUNDS; ++k) {
+            const int i = i0 + k * 32;
+            key[k] = where[k] = 0;
+            if (k < rounds && i < n) {
+                key[k] = pass == 0 ? key_of(ids[i], vocab, status) : skey[i];
+                where[k] = pass == 0 ? i : spos[i];
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < SMALL_ROUNDS; ++k) {
+            if (k >= rounds) break;
+            const bool in = i0 + k * 32 < n;
+            const uint32_t digit = in ? (key[k] >> shift) & (DIGITS - 1) : static_cast<uint32_t>(DIGITS);
+            const unsigned same = __match_any_sync(0xffffffffu, digit);
+            const unsigned lower = same & ((1u << lane) - 1u);
+            unsigned short* mine = ahead + warp * DIGITS + digit;
+            if (in) where[k] |= static_cast<uint32_t>(__popc(lower) + *mine) << 16;
+            __syncwarp();
+            if (in && lower == 0) *mine += static_cast<unsigned short>(__popc(same));
+            __syncwarp();
+        }
+        __syncthreads();
+        uint32_t total = 0;
+        if (threadIdx.x < DIGITS) {
+#pragma unroll 8
+            for (int w = 0; w < SORT_WARPS; ++w) {
+                const uint32_t c = ahead[w * DIGITS + threadIdx.x];
+                ahead[w * DIGITS + threadIdx.x] = static_cast<unsigned short>(total);
+                total += c;
+            }
+        }
+        uint32_t incl = total;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t up = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += up;
+        }
+        if (lane == 31) scan[warp] = incl;
+        __syncthreads();
+        if (threadIdx.x < DIGITS) {
+            uint32_t base = 0;
+            for (int w = 0; w < warp; ++w) base += scan[w];
+            offset[threadIdx.x] = base + incl - total;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < SMALL_ROUNDS; ++k) {
+            if (k < rounds && i0 + k * 32 < n) {
+                const uint32_t digit = (key[k] >> shift) & (DIGITS - 1);
+                const uint32_t to = offset[digit] + ahead[warp * DIGITS + digit] + (where[k] >> 16);
+                skey[to] = key[k];
+                spos[to] = static_cast<unsigned short>(where[k]);
+            }
+        }
+        __syncthreads();
+    }
+    for (int i = threadIdx.x; i < n; i += SORT_THREADS) {
+        keys_out[i] = skey[i];
+        pos_out[i] = spos[i];
+    }
+}
+
 // --------------------------------------------------------------------- gradient
 
 constexpr int GRAD_THREADS = 256;
 constexpr int GRAD_UNROLL = 8;           // token rows a thread has in flight
-constexpr int MAX_PIECE = 1024;          // sorted tokens per block at most
-
-// Zeroes the rows no token names; one warp a row.
-template <typename TT, int VEC>
-__global__ void __launch_bounds__(256)
-zero_rows_kernel(TT* __restrict__ dtable, int64_t ldt, const uint32_t* __restrict__ touched, int64_t vocab,
-                 int64_t nvec)
-{
-    const int64_t warps = static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5);
-    Raw<TT, VEC> zero;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) zero.e[i] = from_f<TT>(0.0f);
-    for (int64_t v = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5); v < vocab; v += warps) {
-        if ((touched[v >> 5] >> (v & 31)) & 1u) continue;
-        TT* row = dtable + v * ldt;
-        for (int64_t k = threadIdx.x & 31; k < nvec; k += 32) store_raw<true>(row + k * VEC, zero);
-    }
-}
+constexpr int MAX_PIECE = 1024;          // sorted tokens per piece at most
+constexpr int64_t ZERO_UNIT = 64 * 1024; // bytes of the table a block fills, about
 
 template <typename TT, int VEC>
 __device__ __forceinline__ void write_row(TT* p, const float (&sum)[VEC], float scale, int accumulate)
@@ -236,104 +347,151 @@ __device__ __forceinline__ void write_row(TT* p, const float (&sum)[VEC], float 
     store_f<true>(p, o);
 }
 
-// Block (piece, column tile).  edge: [pieces][2][nvec * VEC] sums of the runs that cross a
-// piece's ends: [0] of the run that came in from the piece before (whether or not it also
-// goes on), [1] of a run that starts here and goes on.
+struct GradArgs {
+    const uint32_t *keys, *pos;
+    float* edge;                 // [pieces][2][cols]: see the kernel
+    uint32_t* long_runs;         // count, then the pieces in which a long run starts
+    const uint32_t* touched;     // rows that occur (null: nothing is filled with zeros)
+    int64_t n, vocab, nvec, ldt, ldo;
+    int64_t units, zero_units, zero_rows;        // pieces x column tiles; blocks that fill zero_rows rows each
+    int piece, tiles, accumulate;
+    float scale;
+};
+
+// Blocks that add up a piece's share of one column tile, and blocks that fill rows with
+// zeros, in proportion.  edge: sums of long runs (more tokens than a piece): [0] of a run
+// that came in from the piece before, whether or not it goes on; [1] of one that starts here.
 template <typename TT, typename TA, int VEC>
 __global__ void __launch_bounds__(GRAD_THREADS)
-grad_pieces_kernel(TT* __restrict__ dtable, int64_t ldt, float* __restrict__ edge, const TA* __restrict__ dout,
-                   int64_t ldo, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos, int64_t n,
-                   int piece, int64_t vocab, int64_t nvec, float scale, int accumulate)
+grad_pieces_kernel(TT* __restrict__ dtable, const TA* __restrict__ dout, const GradArgs a)
 {
-    __shared__ uint32_t skey[MAX_PIECE + 2], spos[MAX_PIECE];
-    const int64_t i0 = static_cast<int64_t>(blockIdx.x) * piece;
-    const int count = static_cast<int>(min(static_cast<int64_t>(piece), n - i0));
-    // skey[0] and skey[count + 1]: the neighbours' keys, or a key that no row has
-    for (int i = threadIdx.x; i < count + 2; i += blockDim.x) {
-        const int64_t at = i0 + i - 1;
-        skey[i] = at >= 0 && at < n ? keys[at] : 0xffffffffu;
+    ptx::griddep_launch_dependents();
+    ptx::griddep_wait();
+    int64_t unit = blockIdx.x;
+    if (a.zero_units > 0) {
+        const int64_t all = a.units + a.zero_units;
+        const int64_t z = unit * a.zero_units / all, after = (unit + 1) * a.zero_units / all;
+        if (after > z) {
+            zero_rows<TT, VEC>(dtable, a.ldt, a.nvec, z * a.zero_rows, min(a.vocab, (z + 1) * a.zero_rows), a.touched);
+            return;
+        }
+        unit -= z;
     }
-    for (int i = threadIdx.x; i < count; i += blockDim.x) spos[i] = pos[i0 + i];
+    extern __shared__ uint32_t window[];                     // keys of [i0 - piece - 1, i1 + piece], positions of [i0, i1 + piece)
+    __shared__ int first_from, first_to, last_from, last_to; // the runs at the piece's ends, relative to i0
+    const int piece = a.piece;
+    const int64_t p = unit / a.tiles, i0 = p * piece;
+    const int count = static_cast<int>(min(static_cast<int64_t>(piece), a.n - i0));
+    const uint32_t* key = window + piece + 1;                // key[i]: of sorted token i0 + i
+    uint32_t* spos = window + 3 * piece + 2;
+    for (int i = threadIdx.x; i < 3 * piece + 2; i += blockDim.x) {
+        const int64_t at = i0 + i - piece - 1;
+        window[i] = at >= 0 && at < a.n ? a.keys[at] : 0xffffffffu;      // no row's key
+    }
+    for (int i = threadIdx.x; i < 2 * piece; i += blockDim.x) spos[i] = i0 + i < a.n ? a.pos[i0 + i] : 0;
+    if (threadIdx.x == 0) {
+        first_from = last_from = -piece;
+        first_to = last_to = count + piece;
+    }
     __syncthreads();
-    const int64_t v = static_cast<int64_t>(blockIdx.y) * blockDim.x + threadIdx.x;
-    if (v >= nvec) return;
+    const uint32_t k_first = key[0], k_last = key[count - 1];
+    for (int i = static_cast<int>(threadIdx.x) - piece; i < count + piece; i += blockDim.x) {
+        const uint32_t k = key[i];
+        if (i < 0 && k != k_first) atomicMax(&first_from, i + 1);
+        if (i >= 0 && k != k_first) atomicMin(&first_to, i);
+        if (i < count && k != k_last) atomicMax(&last_from, i + 1);
+        if (i >= count && k != k_last) atomicMin(&last_to, i);
+    }
+    __syncthreads();
+    // a run that came in: a short one is its first piece's, of a long one this piece has a part
+    const bool came_in = key[-1] == k_first;
+    const bool first_long = came_in && first_to - first_from > piece;
+    const int begin = came_in && !first_long ? first_to : 0;
+    // a run that starts here and goes on: a short one to its end, of a long one the part here
+    const bool goes_on = key[count] == k_last && last_from >= 0 && !(came_in && last_from <= 0);
+    const bool last_long = goes_on && last_to - last_from > piece;
+    const int end = goes_on && !last_long ? last_to : count;
+    const int tile = static_cast<int>(unit % a.tiles);
+    if (threadIdx.x == 0 && tile == 0 && last_long && k_last < a.vocab) a.long_runs[1 + atomicAdd(a.long_runs, 1u)] = static_cast<uint32_t>(p);
+    const int64_t v = static_cast<int64_t>(tile) * blockDim.x + threadIdx.x;
+    if (v >= a.nvec) return;
     const TA* src = dout + v * VEC;
     float sum[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) sum[i] = 0.0f;
-    bool came_in = skey[0] == skey[1];
-    for (int b = 0; b < count; b += GRAD_UNROLL) {
+    bool first = first_long;
+    for (int b = begin; b < end; b += GRAD_UNROLL) {
         Raw<TA, VEC> r[GRAD_UNROLL];
 #pragma unroll
         for (int k = 0; k < GRAD_UNROLL; ++k)
-            if (b + k < count && skey[b + k + 1] < vocab) load_raw<true>(r[k], src + static_cast<int64_t>(spos[b + k]) * ldo);
+            if (b + k < end && key[b + k] < a.vocab) load_raw<true>(r[k], src + static_cast<int64_t>(spos[b + k]) * a.ldo);
 #pragma unroll
         for (int k = 0; k < GRAD_UNROLL; ++k) {
-            if (b + k >= count) break;
-            const uint32_t key = skey[b + k + 1];
-            if (key >= vocab) break;                         // padding sorts last
+            const int i = b + k;
+            if (i >= end) break;
+            const uint32_t row = key[i];
+            if (row >= a.vocab) break;                       // padding sorts last
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) sum[i] += to_f(r[k].e[i]);
-            if (skey[b + k + 2] == key && b + k + 1 < count) continue;
-            const bool goes_on = skey[b + k + 2] == key;
-            if (came_in || goes_on) {
-                float* e = edge + ((static_cast<int64_t>(blockIdx.x) * 2 + (came_in ? 0 : 1)) * nvec + v) * VEC;
+            for (int e = 0; e < VEC; ++e) sum[e] += to_f(r[k].e[e]);
+            if (i + 1 < end && key[i + 1] == row) continue;
+            const bool cut = last_long && i + 1 == end;
+            if (first || cut) {
+                float* to = a.edge + ((p * 2 + (first ? 0 : 1)) * a.nvec + v) * VEC;
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) e[i] = sum[i];
+                for (int e = 0; e < VEC; ++e) to[e] = sum[e];
             } else {
-                write_row<TT, VEC>(dtable + static_cast<int64_t>(key) * ldt + v * VEC, sum, scale, accumulate);
+                write_row<TT, VEC>(dtable + static_cast<int64_t>(row) * a.ldt + v * VEC, sum, a.scale, a.accumulate);
             }
-            came_in = false;
+            first = false;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) sum[i] = 0.0f;
+            for (int e = 0; e < VEC; ++e) sum[e] = 0.0f;
         }
     }
 }
 
-// Block (piece, column tile): if a run starts in this piece and goes on, adds its parts.
+// Adds the parts of the long runs: a block takes one run and one column tile at a time.
 // blockDim.x = lanes * slices; a slice adds neighbouring pieces, the slices are added in order.
 template <typename TT, int VEC>
 __global__ void __launch_bounds__(GRAD_THREADS)
-grad_join_kernel(TT* __restrict__ dtable, int64_t ldt, const float* __restrict__ edge,
-                 const uint32_t* __restrict__ keys, int64_t n, int piece, int64_t vocab, int64_t nvec, float scale,
-                 int accumulate, int lanes)
+grad_join_kernel(TT* __restrict__ dtable, const GradArgs a, int lanes, int col_tiles)
 {
+    ptx::griddep_wait();
     __shared__ float part[GRAD_THREADS * VEC];
-    const int64_t p = blockIdx.x, i0 = p * piece, i1 = i0 + piece;
-    if (i1 >= n) return;                                     // the last piece hands nothing on
-    const uint32_t key = keys[i1 - 1];
-    if (key >= vocab || keys[i1] != key) return;
-    if (i0 > 0 && keys[i0] == key && keys[i0 - 1] == key) return;      // it started further ahead
-    // last piece whose first key is this one
-    int64_t lo = p + 1, hi = (n - 1) / piece;
-    while (lo < hi) {
-        const int64_t mid = (lo + hi + 1) / 2;
-        if (keys[mid * piece] == key) lo = mid; else hi = mid - 1;
-    }
-    const int64_t parts = lo - p + 1;                        // this piece's [1], then [0] of p + 1 .. lo
+    const int64_t runs = *a.long_runs;
     const int lane = threadIdx.x % lanes, slice = threadIdx.x / lanes, slices = blockDim.x / lanes;
-    const int64_t v = static_cast<int64_t>(blockIdx.y) * lanes + lane;
-    const int64_t per = (parts + slices - 1) / slices;
-    const int64_t q0 = slice * per, q1 = min(parts, q0 + per);
-    float sum[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) sum[i] = 0.0f;
-    if (v < nvec) {
-#pragma unroll 4
-        for (int64_t q = q0; q < q1; ++q) {
-            const float* e = edge + (((p + q) * 2 + (q == 0 ? 1 : 0)) * nvec + v) * VEC;
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) sum[i] += e[i];
+    for (int64_t job = blockIdx.x; job < runs * col_tiles; job += gridDim.x) {
+        const int64_t p = a.long_runs[1 + job / col_tiles];
+        const int64_t v = job % col_tiles * lanes + lane;
+        const uint32_t key = a.keys[(p + 1) * a.piece - 1];
+        int64_t lo = p + 1, hi = (a.n - 1) / a.piece;        // last piece whose first key is this one
+        while (lo < hi) {
+            const int64_t mid = (lo + hi + 1) / 2;
+            if (a.keys[mid * a.piece] == key) lo = mid; else hi = mid - 1;
         }
+        const int64_t parts = lo - p + 1;                    // this piece's [1], then [0] of p + 1 .. lo
+        const int64_t per = (parts + slices - 1) / slices;
+        const int64_t q0 = slice * per, q1 = min(parts, q0 + per);
+        float sum[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) sum[i] = 0.0f;
+        if (v < a.nvec) {
+#pragma unroll 4
+            for (int64_t q = q0; q < q1; ++q) {
+                const float* e = a.edge + (((p + q) * 2 + (q == 0 ? 1 : 0)) * a.nvec + v) * VEC;
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) sum[i] += e[i];
+            }
+        }
+        __syncthreads();                                     // the job before has read its parts
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) part[threadIdx.x * VEC + i] = sum[i];
+        __syncthreads();
+        if (slice != 0 || v >= a.nvec) continue;
+        for (int s = 1; s < slices; ++s)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) sum[i] += part[(s * lanes + lane) * VEC + i];
+        write_row<TT, VEC>(dtable + static_cast<int64_t>(key) * a.ldt + v * VEC, sum, a.scale, a.accumulate);
     }
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) part[threadIdx.x * VEC + i] = sum[i];
-    __syncthreads();
-    if (slice != 0 || v >= nvec) return;
-    for (int s = 1; s < slices; ++s)
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) sum[i] += part[(s * lanes + lane) * VEC + i];
-    write_row<TT, VEC>(dtable + static_cast<int64_t>(key) * ldt + v * VEC, sum, scale, accumulate);
 }
 
 // ------------------------------------------------------------------------- host
@@ -359,16 +517,25 @@ int with_types(int table_type, int type, F f)
     return type == SB200_F32 ? f(f16{}, float{}) : f(f16{}, f16{});
 }
 
-// 16 bytes of the narrower of the two types
-template <typename TT, typename TA>
-constexpr int wide() { return 16 / (sizeof(TT) < sizeof(TA) ? sizeof(TT) : sizeof(TA)); }
+template <int N>
+using Int = std::integral_constant<int, N>;
 
-template <typename TT, typename TA>
-bool can_vector(const void* table, int64_t ldt, const void* act, int64_t lda, int64_t cols)
+// f(Int<elements per access>{}): 16 bytes of the narrower type where all rows allow it, two
+// elements where one side has 16 bits, else one element.
+template <typename TT, typename TA, typename F>
+int with_width(const void* table, int64_t ldt, const void* act, int64_t lda, int64_t cols, F f)
 {
-    constexpr int VEC = wide<TT, TA>();
-    return cols % VEC == 0 && (ldt * static_cast<int64_t>(sizeof(TT))) % 16 == 0 &&
-           (lda * static_cast<int64_t>(sizeof(TA))) % 16 == 0 && aligned_to(table, 16) && aligned_to(act, 16);
+    constexpr int NARROW = sizeof(TT) < sizeof(TA) ? sizeof(TT) : sizeof(TA);
+    auto fits = [&](int vec) {
+        const size_t bt = vec * sizeof(TT) < 16 ? vec * sizeof(TT) : 16, ba = vec * sizeof(TA) < 16 ? vec * sizeof(TA) : 16;
+        return cols % vec == 0 && (ldt * static_cast<int64_t>(sizeof(TT))) % bt == 0 &&
+               (lda * static_cast<int64_t>(sizeof(TA))) % ba == 0 && aligned_to(table, bt) && aligned_to(act, ba);
+    };
+    if (fits(16 / NARROW)) return f(Int<16 / NARROW>{});
+    if constexpr (NARROW == 2) {
+        if (fits(2)) return f(Int<2>{});
+    }
+    return f(Int<1>{});
 }
 
 int power_of_two(int64_t n, int most)
@@ -379,17 +546,19 @@ int power_of_two(int64_t n, int most)
 }
 
 struct GradPlan {
-    int64_t blocks, per_block;           // of the sort
+    bool small;                          // sorted by one block
+    int64_t blocks, per_block;           // of the sort otherwise
     int passes;
     int piece;
     int64_t pieces;
     // byte offsets into the workspace
-    int64_t counts, touched, keys[2], pos[2], edge, total;
+    int64_t counts, long_runs, touched, keys[2], pos[2], edge, total;
 };
 
 GradPlan plan_grad(int sm_count, int64_t n, int64_t vocab, int64_t cols)
 {
     GradPlan g{};
+    g.small = n <= SMALL_TOKENS;
     const int64_t tiles = n > 0 ? (n + SORT_TILE - 1) / SORT_TILE : 1;
     const int64_t tiles_per_block = (tiles + SORT_BLOCKS - 1) / SORT_BLOCKS;
     g.per_block = tiles_per_block * SORT_TILE;
@@ -403,31 +572,51 @@ GradPlan plan_grad(int sm_count, int64_t n, int64_t vocab, int64_t cols)
     int64_t piece = n * tiles_n / (16ll * sm_count);
     if (piece < GRAD_UNROLL) piece = GRAD_UNROLL;
     if (piece > 32) piece = 32;
-    if (n / piece > 8192) piece = n / 8192;                  // long lists: bounds the edge sums
+    if (n / piece > 8192) piece = n / 8192;                  // long lists: bounds the partial sums
     if (piece > MAX_PIECE) piece = MAX_PIECE;
     g.piece = static_cast<int>(piece);
     g.pieces = (n + piece - 1) / piece;
     int64_t at = 0;
     auto take = [&](int64_t bytes) { const int64_t o = at; at += (bytes + 255) / 256 * 256; return o; };
-    g.counts = take(g.blocks * DIGITS * 4);
+    g.long_runs = take((g.pieces + 1) * 4);                  // cleared together with the next
     g.touched = take((vocab + 31) / 32 * 4);
+    g.counts = take(g.blocks * DIGITS * 4);
     for (int i = 0; i < 2; ++i) { g.keys[i] = take(n * 4); g.pos[i] = take(n * 4); }
     g.edge = take(g.pieces * 2 * cols * 4);
     g.total = at;
     return g;
 }
 
+// Launches that may overlap the tail of the kernel before (which every one of them waits for).
+template <typename... A, typename... B>
+int launch_after(sb200_ctx* ctx, void (*kern)(A...), int64_t grid, int block, size_t smem, cudaStream_t stream, B... args)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(grid));
+    cfg.blockDim = dim3(static_cast<unsigned>(block));
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    ctx->launches += 1;
+    return cudaLaunchKernelEx(&cfg, kern, static_cast<A>(args)...) == cudaSuccess ? SB200_OK : SB200_ERR_CUDA;
+}
+
+// More than SMALL_TOKENS: two launches a pass.  Returns the buffer (0 or 1) of the result.
 template <typename I>
-void sort_tokens(sb200_ctx* ctx, const GradPlan& g, unsigned char* ws, const I* ids, int64_t n, int64_t vocab,
-                 uint32_t* touched, const uint32_t** keys, const uint32_t** pos, cudaStream_t stream)
+int sort_large(sb200_ctx* ctx, const GradPlan& g, unsigned char* ws, const I* ids, int64_t n, int64_t vocab,
+               uint32_t* touched, cudaStream_t stream)
 {
     auto u32 = [&](int64_t at) { return reinterpret_cast<uint32_t*>(ws + at); };
     uint32_t* counts = u32(g.counts);
     const unsigned grid = static_cast<unsigned>(g.blocks);
-    const uint32_t *kin = nullptr, *pin = nullptr;
     for (int pass = 0; pass < g.passes; ++pass) {
-        const int shift = pass * DIGIT_BITS;
-        uint32_t *kout = u32(g.keys[pass & 1]), *pout = u32(g.pos[pass & 1]);
+        const int shift = pass * DIGIT_BITS, to = pass & 1;
+        uint32_t *kout = u32(g.keys[to]), *pout = u32(g.pos[to]);
+        const uint32_t *kin = u32(g.keys[to ^ 1]), *pin = u32(g.pos[to ^ 1]);
         if (pass == 0) {
             sort_count_kernel<I, true><<<grid, SORT_THREADS, 0, stream>>>(counts, touched, ids, nullptr, n, g.per_block, vocab, shift, ctx->d_status);
             sort_scatter_kernel<I, true><<<grid, SORT_THREADS, 0, stream>>>(kout, pout, counts, ids, nullptr, nullptr, n, g.per_block, vocab, shift, ctx->d_status);
@@ -436,34 +625,63 @@ void sort_tokens(sb200_ctx* ctx, const GradPlan& g, unsigned char* ws, const I* 
             sort_scatter_kernel<I, false><<<grid, SORT_THREADS, 0, stream>>>(kout, pout, counts, nullptr, kin, pin, n, g.per_block, vocab, shift, ctx->d_status);
         }
         ctx->launches += 2;
-        kin = kout;
-        pin = pout;
     }
-    *keys = kin;
-    *pos = pin;
+    return (g.passes - 1) & 1;
 }
 
-template <typename TT, typename TA, int VEC>
-void launch_grad(sb200_ctx* ctx, const GradPlan& g, TT* dtable, int64_t ldt, float* edge, const TA* dout, int64_t ldo,
-                 const uint32_t* keys, const uint32_t* pos, const uint32_t* touched, int64_t n, int64_t vocab,
-                 int64_t cols, float scale, int accumulate, cudaStream_t stream)
+template <typename I, typename TT, typename TA, int VEC>
+int launch_grad(sb200_ctx* ctx, const GradPlan& g, unsigned char* ws, TT* dtable, int64_t ldt, const TA* dout, int64_t ldo,
+                const I* ids, int64_t n, int64_t vocab, int64_t cols, float scale, int accumulate, cudaStream_t stream)
 {
+    auto u32 = [&](int64_t at) { return reinterpret_cast<uint32_t*>(ws + at); };
     const int64_t nvec = cols / VEC;
-    if (!accumulate) {
-        int64_t grid = (vocab + 7) / 8;
-        if (grid > 16ll * ctx->sm_count) grid = 16ll * ctx->sm_count;
-        zero_rows_kernel<TT, VEC><<<static_cast<unsigned>(grid), 256, 0, stream>>>(dtable, ldt, touched, vocab, nvec);
+    uint32_t* touched = nullptr;
+    int buffer = 0;
+    if (g.small) {
+        auto kern = sort_small_kernel<I, TT, VEC>;
+        static bool attr_done[16] = {};
+        if (ctx->device >= 16 || !attr_done[ctx->device]) {
+            if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMALL_SMEM) != cudaSuccess) return SB200_ERR_CUDA;
+            if (ctx->device < 16) attr_done[ctx->device] = true;
+        }
+        int64_t fill = accumulate ? 0 : vocab < ctx->sm_count ? vocab : ctx->sm_count - 1;
+        kern<<<static_cast<unsigned>(1 + fill), SORT_THREADS, SMALL_SMEM, stream>>>(
+            u32(g.keys[0]), u32(g.pos[0]), u32(g.long_runs), ids, static_cast<int>(n), vocab, g.passes, dtable, ldt, nvec, ctx->d_status);
         ctx->launches += 1;
+        if (cudaGetLastError() != cudaSuccess) return SB200_ERR_CUDA;
+        if (n == 0) return SB200_OK;
+    } else {
+        const int64_t clear = accumulate ? 4 : g.touched + (vocab + 31) / 32 * 4 - g.long_runs;
+        if (cudaMemsetAsync(ws + g.long_runs, 0, static_cast<size_t>(clear), stream) != cudaSuccess) return SB200_ERR_CUDA;
+        if (!accumulate) touched = u32(g.touched);
+        buffer = sort_large(ctx, g, ws, ids, n, vocab, touched, stream);
+        if (cudaGetLastError() != cudaSuccess) return SB200_ERR_CUDA;
     }
-    if (n == 0) return;
+    GradArgs a{};
+    a.keys = u32(g.keys[buffer]);
+    a.pos = u32(g.pos[buffer]);
+    a.edge = reinterpret_cast<float*>(ws + g.edge);
+    a.long_runs = u32(g.long_runs);
+    a.touched = touched;
+    a.n = n; a.vocab = vocab; a.nvec = nvec; a.ldt = ldt; a.ldo = ldo;
     const int threads = power_of_two(nvec, GRAD_THREADS) < 32 ? 32 : power_of_two(nvec, GRAD_THREADS);
-    const dim3 grid(static_cast<unsigned>(g.pieces), static_cast<unsigned>((nvec + threads - 1) / threads));
-    grad_pieces_kernel<TT, TA, VEC><<<grid, threads, 0, stream>>>(dtable, ldt, edge, dout, ldo, keys, pos, n, g.piece, vocab, nvec, scale, accumulate);
+    a.tiles = static_cast<int>((nvec + threads - 1) / threads);
+    a.units = g.pieces * a.tiles;
+    if (touched) {
+        const int64_t row = cols * static_cast<int64_t>(sizeof(TT));
+        a.zero_rows = row < ZERO_UNIT ? ZERO_UNIT / row : 1;
+        a.zero_units = (vocab + a.zero_rows - 1) / a.zero_rows;
+    }
+    a.piece = g.piece;
+    a.accumulate = accumulate;
+    a.scale = scale;
+    if (a.units + a.zero_units > INT32_MAX) return SB200_ERR_TOO_LARGE;
+    if (const int rc = launch_after(ctx, grad_pieces_kernel<TT, TA, VEC>, a.units + a.zero_units, threads,
+                                    static_cast<size_t>(5 * g.piece + 2) * 4, stream, dtable, dout, a)) return rc;
     // few columns a block and many slices: a run of many pieces is added by slices at the same time
-    const int lanes = threads < 32 ? threads : 32;
-    const dim3 join(static_cast<unsigned>(g.pieces), static_cast<unsigned>((nvec + lanes - 1) / lanes));
-    grad_join_kernel<TT, VEC><<<join, GRAD_THREADS, 0, stream>>>(dtable, ldt, edge, keys, n, g.piece, vocab, nvec, scale, accumulate, lanes);
-    ctx->launches += 2;
+    const int lanes = 32, col_tiles = static_cast<int>((nvec + lanes - 1) / lanes);
+    const int64_t jobs = g.pieces * col_tiles, most = 4ll * ctx->sm_count;
+    return launch_after(ctx, grad_join_kernel<TT, VEC>, jobs < most ? jobs : most, GRAD_THREADS, 0, stream, dtable, a, lanes, col_tiles);
 }
 
 }  // namespace
@@ -484,27 +702,26 @@ extern "C" int sb200_embedding(sb200_ctx* ctx, void* out, int64_t ldo, const voi
     DeviceGuard dev(ctx->device);
     if (!dev.ok) return SB200_ERR_CUDA;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-    return with_types(table_type, type, [&](auto tt, auto ta) {
+    return with_types(table_type, type, [&](auto tt, auto ta) -> int {
         using TT = decltype(tt);
         using TA = decltype(ta);
-        constexpr int WIDE = wide<TT, TA>();
-        const bool vec = can_vector<TT, TA>(table, ldt, out, ldo, cols);
-        const int64_t nvec = vec ? cols / WIDE : cols;
-        const int lanes = power_of_two(nvec, LOOKUP_THREADS);
-        const int64_t per_block = static_cast<int64_t>(LOOKUP_THREADS / lanes) * LOOKUP_ROWS;
-        const unsigned grid = static_cast<unsigned>((n + per_block - 1) / per_block);
-        auto go = [&](auto id, auto v) {
-            using I = decltype(id);
-            lookup_kernel<TT, TA, I, decltype(v)::value><<<grid, LOOKUP_THREADS, 0, stream>>>(
-                static_cast<TA*>(out), ldo, static_cast<const TT*>(table), ldt, static_cast<const I*>(ids), n, vocab,
-                static_cast<int>(nvec), scale, lanes, ctx->d_status);
-        };
-        using One = std::integral_constant<int, 1>;
-        using Wide = std::integral_constant<int, WIDE>;
-        if (index_bits == 64) { if (vec) go(int64_t{}, Wide{}); else go(int64_t{}, One{}); }
-        else { if (vec) go(int32_t{}, Wide{}); else go(int32_t{}, One{}); }
-        ctx->launches += 1;
-        return cudaGetLastError() == cudaSuccess ? SB200_OK : SB200_ERR_CUDA;
+        return with_width<TT, TA>(table, ldt, out, ldo, cols, [&](auto v) -> int {
+            constexpr int VEC = decltype(v)::value;
+            const int64_t nvec = cols / VEC;
+            const int lanes = power_of_two(nvec, LOOKUP_THREADS);
+            const int64_t per_block = static_cast<int64_t>(LOOKUP_THREADS / lanes) * LOOKUP_ROWS<VEC>;
+            const unsigned grid = static_cast<unsigned>((n + per_block - 1) / per_block);
+            auto go = [&](auto id) {
+                using I = decltype(id);
+                lookup_kernel<TT, TA, I, VEC><<<grid, LOOKUP_THREADS, 0, stream>>>(
+                    static_cast<TA*>(out), ldo, static_cast<const TT*>(table), ldt, static_cast<const I*>(ids), n, vocab,
+                    static_cast<int>(nvec), scale, lanes, ctx->d_status);
+            };
+            if (index_bits == 64) go(int64_t{});
+            else go(int32_t{});
+            ctx->launches += 1;
+            return cudaGetLastError() == cudaSuccess ? SB200_OK : SB200_ERR_CUDA;
+        });
     });
 }
 
@@ -531,28 +748,16 @@ extern "C" int sb200_embedding_backward(sb200_ctx* ctx, void* dtable, int64_t ld
     if (!dev.ok) return SB200_ERR_CUDA;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     unsigned char* ws = static_cast<unsigned char*>(workspace);
-    uint32_t* touched = nullptr;
-    if (!accumulate) {
-        touched = reinterpret_cast<uint32_t*>(ws + g.touched);
-        if (cudaMemsetAsync(touched, 0, static_cast<size_t>((vocab + 31) / 32 * 4), stream) != cudaSuccess) return SB200_ERR_CUDA;
-    }
-    const uint32_t *keys = nullptr, *pos = nullptr;
-    if (n > 0) {
-        if (index_bits == 64)
-            sort_tokens(ctx, g, ws, static_cast<const int64_t*>(ids), n, vocab, touched, &keys, &pos, stream);
-        else
-            sort_tokens(ctx, g, ws, static_cast<const int32_t*>(ids), n, vocab, touched, &keys, &pos, stream);
-    }
-    float* edge = reinterpret_cast<float*>(ws + g.edge);
-    return with_types(table_type, type, [&](auto tt, auto ta) {
+    return with_types(table_type, type, [&](auto tt, auto ta) -> int {
         using TT = decltype(tt);
         using TA = decltype(ta);
         TT* dt = static_cast<TT*>(dtable);
         const TA* dy = static_cast<const TA*>(dout);
-        if (can_vector<TT, TA>(dtable, ldt, dout, ldo, cols))
-            launch_grad<TT, TA, wide<TT, TA>()>(ctx, g, dt, ldt, edge, dy, ldo, keys, pos, touched, n, vocab, cols, scale, accumulate, stream);
-        else
-            launch_grad<TT, TA, 1>(ctx, g, dt, ldt, edge, dy, ldo, keys, pos, touched, n, vocab, cols, scale, accumulate, stream);
-        return cudaGetLastError() == cudaSuccess ? SB200_OK : SB200_ERR_CUDA;
+        return with_width<TT, TA>(dtable, ldt, dout, ldo, cols, [&](auto v) -> int {
+            constexpr int VEC = decltype(v)::value;
+            if (index_bits == 64)
+                return launch_grad<int64_t, TT, TA, VEC>(ctx, g, ws, dt, ldt, dy, ldo, static_cast<const int64_t*>(ids), n, vocab, cols, scale, accumulate, stream);
+            return launch_grad<int32_t, TT, TA, VEC>(ctx, g, ws, dt, ldt, dy, ldo, static_cast<const int32_t*>(ids), n, vocab, cols, scale, accumulate, stream);
+        });
     });
 }
