@@ -350,7 +350,7 @@ __device__ __forceinline__ void write_row(TT* p, const float (&sum)[VEC], float 
 struct GradArgs {
     const uint32_t *keys, *pos;
     float* edge;                 // [pieces][2][cols]: see the kernel
-    uint32_t* long_runs;         // count, then the pieces in which a long run starts
+    uint32_t* long_runs;         // count, then from word 2 the pieces in which long runs start, and their rows
     const uint32_t* touched;     // rows that occur (null: nothing is filled with zeros)
     int64_t n, vocab, nvec, ldt, ldo;
     int64_t units, zero_units, zero_rows;        // pieces x column tiles; blocks that fill zero_rows rows each
@@ -412,7 +412,8 @@ grad_pieces_kernel(TT* __restrict__ dtable, const TA* __restrict__ dout, const G
     const bool last_long = goes_on && last_to - last_from > piece;
     const int end = goes_on && !last_long ? last_to : count;
     const int tile = static_cast<int>(unit % a.tiles);
-    if (threadIdx.x == 0 && tile == 0 && last_long && k_last < a.vocab) a.long_runs[1 + atomicAdd(a.long_runs, 1u)] = static_cast<uint32_t>(p);
+    if (threadIdx.x == 0 && tile == 0 && last_long && k_last < a.vocab)
+        reinterpret_cast<uint2*>(a.long_runs)[1 + atomicAdd(a.long_runs, 1u)] = make_uint2(static_cast<uint32_t>(p), k_last);
     const int64_t v = static_cast<int64_t>(tile) * blockDim.x + threadIdx.x;
     if (v >= a.nvec) return;
     const TA* src = dout + v * VEC;
@@ -457,18 +458,20 @@ grad_join_kernel(TT* __restrict__ dtable, const GradArgs a, int lanes, int col_t
 {
     ptx::griddep_wait();
     __shared__ float part[GRAD_THREADS * VEC];
-    const int64_t runs = *a.long_runs;
+    const int64_t runs = *a.long_runs, pieces = (a.n + a.piece - 1) / a.piece;
     const int lane = threadIdx.x % lanes, slice = threadIdx.x / lanes, slices = blockDim.x / lanes;
     for (int64_t job = blockIdx.x; job < runs * col_tiles; job += gridDim.x) {
-        const int64_t p = a.long_runs[1 + job / col_tiles];
-        const int64_t v = job % col_tiles * lanes + lane;
-        const uint32_t key = a.keys[(p + 1) * a.piece - 1];
-        int64_t lo = p + 1, hi = (a.n - 1) / a.piece;        // last piece whose first key is this one
-        while (lo < hi) {
-            const int64_t mid = (lo + hi + 1) / 2;
-            if (a.keys[mid * a.piece] == key) lo = mid; else hi = mid - 1;
+        const uint2 run = reinterpret_cast<const uint2*>(a.long_runs)[1 + job / col_tiles];
+        const int64_t p = run.x, v = job % col_tiles * lanes + lane;
+        const uint32_t key = run.y;
+        // pieces behind p that begin with this row, a block's width at a time
+        int64_t parts = 1;                                   // this piece's [1], then [0] of the next ones
+        for (;;) {
+            const int64_t q = p + parts + threadIdx.x;
+            const int same = __syncthreads_count(q < pieces && a.keys[q * a.piece] == key);
+            parts += same;
+            if (same < static_cast<int>(blockDim.x)) break;
         }
-        const int64_t parts = lo - p + 1;                    // this piece's [1], then [0] of p + 1 .. lo
         const int64_t per = (parts + slices - 1) / slices;
         const int64_t q0 = slice * per, q1 = min(parts, q0 + per);
         float sum[VEC];
@@ -482,7 +485,6 @@ grad_join_kernel(TT* __restrict__ dtable, const GradArgs a, int lanes, int col_t
                 for (int i = 0; i < VEC; ++i) sum[i] += e[i];
             }
         }
-        __syncthreads();                                     // the job before has read its parts
 #pragma unroll
         for (int i = 0; i < VEC; ++i) part[threadIdx.x * VEC + i] = sum[i];
         __syncthreads();
@@ -578,7 +580,7 @@ GradPlan plan_grad(int sm_count, int64_t n, int64_t vocab, int64_t cols)
     g.pieces = (n + piece - 1) / piece;
     int64_t at = 0;
     auto take = [&](int64_t bytes) { const int64_t o = at; at += (bytes + 255) / 256 * 256; return o; };
-    g.long_runs = take((g.pieces + 1) * 4);                  // cleared together with the next
+    g.long_runs = take((g.pieces + 1) * 8);                  // cleared together with the next
     g.touched = take((vocab + 31) / 32 * 4);
     g.counts = take(g.blocks * DIGITS * 4);
     for (int i = 0; i < 2; ++i) { g.keys[i] = take(n * 4); g.pos[i] = take(n * 4); }
@@ -680,7 +682,7 @@ int launch_grad(sb200_ctx* ctx, const GradPlan& g, unsigned char* ws, TT* dtable
                                     static_cast<size_t>(5 * g.piece + 2) * 4, stream, dtable, dout, a)) return rc;
     // few columns a block and many slices: a run of many pieces is added by slices at the same time
     const int lanes = 32, col_tiles = static_cast<int>((nvec + lanes - 1) / lanes);
-    const int64_t jobs = g.pieces * col_tiles, most = 4ll * ctx->sm_count;
+    const int64_t jobs = g.pieces * col_tiles, most = 8ll * ctx->sm_count;
     return launch_after(ctx, grad_join_kernel<TT, VEC>, jobs < most ? jobs : most, GRAD_THREADS, 0, stream, dtable, a, lanes, col_tiles);
 }
 
