@@ -27,19 +27,20 @@ namespace sb200 {
 namespace {
 
 constexpr int LOOKUP_THREADS = 256;
-template <int VEC>
-constexpr int LOOKUP_ROWS = VEC >= 4 ? 4 : 8;          // tokens a thread has in flight
+constexpr int LOOKUP_LANES = 64;         // threads a token at most
 
 __device__ __forceinline__ void report_range(unsigned* status) { atomicCAS(status, 0u, static_cast<unsigned>(FAULT_TOKEN_RANGE)); }
 
-// `lanes` (power of two) threads per token, VEC elements an access.
-template <typename TT, typename TA, typename I, int VEC>
+// `lanes` (power of two) threads per token, VEC elements an access.  What counts is how many
+// accesses a thread has under way: eight of one row where rows are long enough (65536 x
+// 4096 bf16: 125 us; two of each of four rows, 145), else one of each of ROWS rows.  The
+// result is stored as usual, not as a stream: it is read next (and 7 us faster).
+template <typename TT, typename TA, typename I, int VEC, int ROWS>
 __global__ void __launch_bounds__(LOOKUP_THREADS)
 lookup_kernel(TA* __restrict__ out, int64_t ldo, const TT* __restrict__ table, int64_t ldt,
               const I* __restrict__ ids, int64_t n, int64_t vocab, int nvec, float scale, int lanes,
               unsigned* status)
 {
-    constexpr int ROWS = LOOKUP_ROWS<VEC>;
     const int lane = threadIdx.x & (lanes - 1);
     const int per_block = LOOKUP_THREADS / lanes;
     const int64_t t0 = (static_cast<int64_t>(blockIdx.x) * per_block) * ROWS + threadIdx.x / lanes;
@@ -53,6 +54,7 @@ lookup_kernel(TA* __restrict__ out, int64_t ldo, const TT* __restrict__ table, i
             id[k] = -1;
         }
     }
+#pragma unroll (ROWS == 1 ? 8 : 1)
     for (int v = lane; v < nvec; v += lanes) {
         Raw<TT, VEC> r[ROWS];
 #pragma unroll
@@ -65,7 +67,7 @@ lookup_kernel(TA* __restrict__ out, int64_t ldo, const TT* __restrict__ table, i
             float f[VEC];
 #pragma unroll
             for (int i = 0; i < VEC; ++i) f[i] = id[k] >= 0 ? to_f(r[k].e[i]) * scale : 0.0f;
-            store_f<true>(out + t * ldo + static_cast<int64_t>(v) * VEC, f);
+            store_f<false>(out + t * ldo + static_cast<int64_t>(v) * VEC, f);
         }
     }
 }
@@ -76,7 +78,7 @@ constexpr int DIGIT_BITS = 9;
 constexpr int DIGITS = 1 << DIGIT_BITS;
 constexpr int SORT_THREADS = 1024;
 constexpr int SORT_WARPS = SORT_THREADS / 32;
-constexpr int SORT_ROUNDS = 2;                               // items a thread per tile
+constexpr int SORT_ROUNDS = 1;                               // items a thread per tile
 constexpr int SORT_TILE = SORT_THREADS * SORT_ROUNDS;
 constexpr int SORT_BLOCKS = 64;                              // at most: every block reads all counts
 
@@ -97,6 +99,8 @@ sort_count_kernel(uint32_t* __restrict__ counts, uint32_t* __restrict__ touched,
                   unsigned* status)
 {
     __shared__ uint32_t hist[DIGITS];
+    ptx::griddep_launch_dependents();
+    ptx::griddep_wait();
     for (int d = threadIdx.x; d < DIGITS; d += SORT_THREADS) hist[d] = 0;
     __syncthreads();
     const int64_t i0 = blockIdx.x * per_block, i1 = min(n, i0 + per_block);
@@ -127,10 +131,13 @@ sort_scatter_kernel(uint32_t* __restrict__ keys_out, uint32_t* __restrict__ pos_
     __shared__ uint32_t scan[SORT_WARPS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int blocks = gridDim.x;
+    ptx::griddep_launch_dependents();
+    ptx::griddep_wait();
 
     // first place of a digit: all items of smaller digits, then the blocks before this one
     uint32_t total = 0, before = 0;
     if (threadIdx.x < DIGITS) {
+#pragma unroll 16
         for (int b = 0; b < blocks; ++b) {
             const uint32_t c = counts[b * DIGITS + threadIdx.x];
             total += c;
@@ -607,28 +614,26 @@ int launch_after(sb200_ctx* ctx, void (*kern)(A...), int64_t grid, int block, si
     return cudaLaunchKernelEx(&cfg, kern, static_cast<A>(args)...) == cudaSuccess ? SB200_OK : SB200_ERR_CUDA;
 }
 
-// More than SMALL_TOKENS: two launches a pass.  Returns the buffer (0 or 1) of the result.
+// More than SMALL_TOKENS: two launches a pass.  *buffer: which (0 or 1) holds the result.
 template <typename I>
 int sort_large(sb200_ctx* ctx, const GradPlan& g, unsigned char* ws, const I* ids, int64_t n, int64_t vocab,
-               uint32_t* touched, cudaStream_t stream)
+               uint32_t* touched, int* buffer, cudaStream_t stream)
 {
     auto u32 = [&](int64_t at) { return reinterpret_cast<uint32_t*>(ws + at); };
     uint32_t* counts = u32(g.counts);
-    const unsigned grid = static_cast<unsigned>(g.blocks);
     for (int pass = 0; pass < g.passes; ++pass) {
         const int shift = pass * DIGIT_BITS, to = pass & 1;
         uint32_t *kout = u32(g.keys[to]), *pout = u32(g.pos[to]);
         const uint32_t *kin = u32(g.keys[to ^ 1]), *pin = u32(g.pos[to ^ 1]);
-        if (pass == 0) {
-            sort_count_kernel<I, true><<<grid, SORT_THREADS, 0, stream>>>(counts, touched, ids, nullptr, n, g.per_block, vocab, shift, ctx->d_status);
-            sort_scatter_kernel<I, true><<<grid, SORT_THREADS, 0, stream>>>(kout, pout, counts, ids, nullptr, nullptr, n, g.per_block, vocab, shift, ctx->d_status);
-        } else {
-            sort_count_kernel<I, false><<<grid, SORT_THREADS, 0, stream>>>(counts, nullptr, nullptr, kin, n, g.per_block, vocab, shift, ctx->d_status);
-            sort_scatter_kernel<I, false><<<grid, SORT_THREADS, 0, stream>>>(kout, pout, counts, nullptr, kin, pin, n, g.per_block, vocab, shift, ctx->d_status);
-        }
-        ctx->launches += 2;
+        int rc = launch_after(ctx, pass == 0 ? sort_count_kernel<I, true> : sort_count_kernel<I, false>, g.blocks, SORT_THREADS, 0, stream,
+                              counts, touched, ids, kin, n, g.per_block, vocab, shift, ctx->d_status);
+        if (!rc)
+            rc = launch_after(ctx, pass == 0 ? sort_scatter_kernel<I, true> : sort_scatter_kernel<I, false>, g.blocks, SORT_THREADS, 0,
+                              stream, kout, pout, counts, ids, kin, pin, n, g.per_block, vocab, shift, ctx->d_status);
+        if (rc) return rc;
     }
-    return (g.passes - 1) & 1;
+    *buffer = (g.passes - 1) & 1;
+    return SB200_OK;
 }
 
 template <typename I, typename TT, typename TA, int VEC>
@@ -656,8 +661,7 @@ int launch_grad(sb200_ctx* ctx, const GradPlan& g, unsigned char* ws, TT* dtable
         const int64_t clear = accumulate ? 4 : g.touched + (vocab + 31) / 32 * 4 - g.long_runs;
         if (cudaMemsetAsync(ws + g.long_runs, 0, static_cast<size_t>(clear), stream) != cudaSuccess) return SB200_ERR_CUDA;
         if (!accumulate) touched = u32(g.touched);
-        buffer = sort_large(ctx, g, ws, ids, n, vocab, touched, stream);
-        if (cudaGetLastError() != cudaSuccess) return SB200_ERR_CUDA;
+        if (const int rc = sort_large(ctx, g, ws, ids, n, vocab, touched, &buffer, stream)) return rc;
     }
     GradArgs a{};
     a.keys = u32(g.keys[buffer]);
@@ -710,17 +714,22 @@ extern "C" int sb200_embedding(sb200_ctx* ctx, void* out, int64_t ldo, const voi
         return with_width<TT, TA>(table, ldt, out, ldo, cols, [&](auto v) -> int {
             constexpr int VEC = decltype(v)::value;
             const int64_t nvec = cols / VEC;
-            const int lanes = power_of_two(nvec, LOOKUP_THREADS);
-            const int64_t per_block = static_cast<int64_t>(LOOKUP_THREADS / lanes) * LOOKUP_ROWS<VEC>;
-            const unsigned grid = static_cast<unsigned>((n + per_block - 1) / per_block);
-            auto go = [&](auto id) {
+            const int lanes = power_of_two(nvec, LOOKUP_LANES);
+            auto go = [&](auto id, auto r) {
                 using I = decltype(id);
-                lookup_kernel<TT, TA, I, VEC><<<grid, LOOKUP_THREADS, 0, stream>>>(
+                constexpr int ROWS = decltype(r)::value;
+                const int64_t per_block = static_cast<int64_t>(LOOKUP_THREADS / lanes) * ROWS;
+                const unsigned grid = static_cast<unsigned>((n + per_block - 1) / per_block);
+                lookup_kernel<TT, TA, I, VEC, ROWS><<<grid, LOOKUP_THREADS, 0, stream>>>(
                     static_cast<TA*>(out), ldo, static_cast<const TT*>(table), ldt, static_cast<const I*>(ids), n, vocab,
                     static_cast<int>(nvec), scale, lanes, ctx->d_status);
             };
-            if (index_bits == 64) go(int64_t{});
-            else go(int32_t{});
+            auto rows = [&](auto id) {
+                if (nvec > LOOKUP_LANES) go(id, Int<1>{});
+                else go(id, Int<4>{});
+            };
+            if (index_bits == 64) rows(int64_t{});
+            else rows(int32_t{});
             ctx->launches += 1;
             return cudaGetLastError() == cudaSuccess ? SB200_OK : SB200_ERR_CUDA;
         });
