@@ -580,7 +580,7 @@ GradPlan plan_grad(int sm_count, int64_t n, int64_t vocab, int64_t cols)
     const int64_t tiles_n = (cols + 4 * GRAD_THREADS - 1) / (4 * GRAD_THREADS);
     int64_t piece = n * tiles_n / (16ll * sm_count);
     if (piece < GRAD_UNROLL) piece = GRAD_UNROLL;
-    if (piece > 32) piece = 32;
+    if (piece > 64) piece = 64;
     if (n / piece > 8192) piece = n / 8192;                  // long lists: bounds the partial sums
     if (piece > MAX_PIECE) piece = MAX_PIECE;
     g.piece = static_cast<int>(piece);
@@ -596,24 +596,6 @@ GradPlan plan_grad(int sm_count, int64_t n, int64_t vocab, int64_t cols)
     return g;
 }
 
-// Launches that may overlap the tail of the kernel before (which every one of them waits for).
-template <typename... A, typename... B>
-int launch_after(sb200_ctx* ctx, void (*kern)(A...), int64_t grid, int block, size_t smem, cudaStream_t stream, B... args)
-{
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(grid));
-    cfg.blockDim = dim3(static_cast<unsigned>(block));
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    ctx->launches += 1;
-    return cudaLaunchKernelEx(&cfg, kern, static_cast<A>(args)...) == cudaSuccess ? SB200_OK : SB200_ERR_CUDA;
-}
-
 // More than SMALL_TOKENS: two launches a pass.  *buffer: which (0 or 1) holds the result.
 template <typename I>
 int sort_large(sb200_ctx* ctx, const GradPlan& g, unsigned char* ws, const I* ids, int64_t n, int64_t vocab,
@@ -625,10 +607,10 @@ int sort_large(sb200_ctx* ctx, const GradPlan& g, unsigned char* ws, const I* id
         const int shift = pass * DIGIT_BITS, to = pass & 1;
         uint32_t *kout = u32(g.keys[to]), *pout = u32(g.pos[to]);
         const uint32_t *kin = u32(g.keys[to ^ 1]), *pin = u32(g.pos[to ^ 1]);
-        int rc = launch_after(ctx, pass == 0 ? sort_count_kernel<I, true> : sort_count_kernel<I, false>, g.blocks, SORT_THREADS, 0, stream,
+        int rc = launch_after(ctx, pass == 0 ? sort_count_kernel<I, true> : sort_count_kernel<I, false>, static_cast<unsigned>(g.blocks), SORT_THREADS, 0, stream,
                               counts, touched, ids, kin, n, g.per_block, vocab, shift, ctx->d_status);
         if (!rc)
-            rc = launch_after(ctx, pass == 0 ? sort_scatter_kernel<I, true> : sort_scatter_kernel<I, false>, g.blocks, SORT_THREADS, 0,
+            rc = launch_after(ctx, pass == 0 ? sort_scatter_kernel<I, true> : sort_scatter_kernel<I, false>, static_cast<unsigned>(g.blocks), SORT_THREADS, 0,
                               stream, kout, pout, counts, ids, kin, pin, n, g.per_block, vocab, shift, ctx->d_status);
         if (rc) return rc;
     }
@@ -682,12 +664,12 @@ int launch_grad(sb200_ctx* ctx, const GradPlan& g, unsigned char* ws, TT* dtable
     a.accumulate = accumulate;
     a.scale = scale;
     if (a.units + a.zero_units > INT32_MAX) return SB200_ERR_TOO_LARGE;
-    if (const int rc = launch_after(ctx, grad_pieces_kernel<TT, TA, VEC>, a.units + a.zero_units, threads,
+    if (const int rc = launch_after(ctx, grad_pieces_kernel<TT, TA, VEC>, static_cast<unsigned>(a.units + a.zero_units), threads,
                                     static_cast<size_t>(5 * g.piece + 2) * 4, stream, dtable, dout, a)) return rc;
     // few columns a block and many slices: a run of many pieces is added by slices at the same time
     const int lanes = 32, col_tiles = static_cast<int>((nvec + lanes - 1) / lanes);
     const int64_t jobs = g.pieces * col_tiles, most = 8ll * ctx->sm_count;
-    return launch_after(ctx, grad_join_kernel<TT, VEC>, jobs < most ? jobs : most, GRAD_THREADS, 0, stream, dtable, a, lanes, col_tiles);
+    return launch_after(ctx, grad_join_kernel<TT, VEC>, static_cast<unsigned>(jobs < most ? jobs : most), GRAD_THREADS, 0, stream, dtable, a, lanes, col_tiles);
 }
 
 }  // namespace

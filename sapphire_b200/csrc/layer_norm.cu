@@ -29,22 +29,22 @@
 namespace sb200 {
 namespace {
 
-constexpr int EPT = 16;                 // elements of a row per thread
+constexpr int EPT = 16;                 // elements of a row per thread (backward pass)
 constexpr int MAX_THREADS = 512;        // threads per row at most
 constexpr int MAX_WARPS = MAX_THREADS / 32;
 constexpr int REGISTER_COLS = EPT * MAX_THREADS;
 constexpr int GROUP_BLOCK = 256;        // block size when a row belongs to a warp or less
 
-// A thread's pieces of the coming rows of one array, in shared memory: STAGES rows of EPT
+// A thread's pieces of the coming rows of one array, in shared memory: STAGES rows of E
 // elements, piece s of stage k at [(k * NV + s) * blockDim + thread].  2-byte accesses have
 // no asynchronous form: those pieces are read when the row is due.
-template <typename T, int VEC>
+template <typename T, int VEC, int E>
 struct Pieces {
-    static constexpr int NV = EPT / VEC, BYTES = VEC * static_cast<int>(sizeof(T));
+    static constexpr int NV = E / VEC, BYTES = VEC * static_cast<int>(sizeof(T));
     static constexpr bool ASYNC = BYTES >= 4;
     static_assert(BYTES == 2 || BYTES == 4 || BYTES == 16, "access width");
     static constexpr int STAGES = !ASYNC ? 1 : sizeof(T) == 4 ? 3 : 4, AHEAD = STAGES - 1;
-    static constexpr int SMEM = ASYNC ? STAGES * EPT * static_cast<int>(sizeof(T)) : 0;      // per thread
+    static constexpr int SMEM = ASYNC ? STAGES * E * static_cast<int>(sizeof(T)) : 0;      // per thread
 
     Raw<T, VEC> next[ASYNC ? 1 : NV];
     unsigned char* base;
@@ -111,15 +111,74 @@ __device__ __forceinline__ float lanes_sum(float v, int lanes)
     return v;
 }
 
-// `lanes` threads per row (blockDim.x of them when WARP is false).
-// 80 registers: three blocks of 256 threads an SM (element by element the addresses need more).
-template <typename T, typename W, int VEC, bool WARP>
-__global__ void __maxnreg__(VEC == 1 ? 128 : 80)
+// E elements of this thread's pieces as pairs: pair j holds elements 2 j and 2 j + 1, of
+// two pieces when a piece is one element.
+template <int VEC, int E, typename P, typename T>
+__device__ __forceinline__ void get_pairs(float2 (&f)[E / 2], const P& pieces, int stage)
+{
+#pragma unroll
+    for (int s = 0; s < P::NV; s += VEC == 1 ? 2 : 1) {
+        Raw<T, VEC> a;
+        pieces.get(a, stage, s);
+        if constexpr (VEC == 1) {
+            Raw<T, VEC> b;
+            pieces.get(b, stage, s + 1);
+            f[s / 2] = make_float2(to_f(a.e[0]), to_f(b.e[0]));
+        } else {
+#pragma unroll
+            for (int i = 0; i < VEC; i += 2) f[(s * VEC + i) / 2] = pair_f(a.e + i);
+        }
+    }
+}
+
+// This thread's weights, in the same order; `none` where there are none.
+template <int VEC, int E, typename W>
+__device__ __forceinline__ void get_weights(float2 (&f)[E / 2], const W* w, float none, int lane, int lanes, int nvec)
+{
+    float* one = reinterpret_cast<float*>(f);
+#pragma unroll
+    for (int s = 0; s < E / VEC; ++s) {
+        float a[VEC];
+        const int v = s * lanes + lane;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) a[i] = none;
+        if (w && v < nvec) load_f<false>(a, w + static_cast<int64_t>(v) * VEC);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) one[s * VEC + i] = a[i];
+    }
+}
+
+// The pairs back into pieces of a row.
+template <int VEC, int E, typename T>
+__device__ __forceinline__ void put_pairs(T* row, const float2 (&f)[E / 2], int lane, int lanes, int nvec)
+{
+    row += static_cast<int64_t>(lane) * VEC;
+#pragma unroll
+    for (int s = 0; s < E / VEC; ++s) {
+        if (s * lanes + lane < nvec) {
+            Raw<T, VEC> r;
+            if constexpr (VEC == 1) {
+                r.e[0] = from_f<T>(s & 1 ? f[s / 2].y : f[s / 2].x);
+            } else {
+#pragma unroll
+                for (int i = 0; i < VEC; i += 2) set_pair(r.e + i, f[(s * VEC + i) / 2]);
+            }
+            store_raw<true>(row + s * lanes * VEC, r);
+        }
+    }
+}
+
+// `lanes` threads per row (blockDim.x of them when WARP is false), E elements each: what a
+// row costs a thread beside its elements (two sums over the warp, one over the block) is as
+// much as 16 elements, so rows of more than a warp get 32; pairs of elements share an
+// instruction.  What bounds it is the instructions, not the memory, when rows are of 16 bits.
+template <typename T, typename W, int VEC, int E, bool WARP>
+__global__ void __maxnreg__(E == 32 || VEC == 1 ? 128 : 80)
 ln_forward_kernel(T* y, int64_t ldy, float* __restrict__ mean_out, float* __restrict__ rstd_out, const T* x,
                   int64_t ldx, const W* __restrict__ w, const W* __restrict__ b, int64_t rows, int cols, float eps,
                   int lanes)
 {
-    using P = Pieces<T, VEC>;
+    using P = Pieces<T, VEC, E>;
     constexpr int NV = P::NV, AHEAD = P::AHEAD;
     extern __shared__ __align__(16) unsigned char smem[];
     // a warp's sum and sum of squared differences from its own mean; two buffers, so that
@@ -138,20 +197,10 @@ ln_forward_kernel(T* y, int64_t ldy, float* __restrict__ mean_out, float* __rest
     const float warp_inv = warp_n > 0.0f ? 1.0f / warp_n : 0.0f;
     if (!WARP && (threadIdx.x & 31) == 0) count[threadIdx.x >> 5] = make_float2(warp_n, warp_inv);   // (read behind a barrier)
 
+    ptx::griddep_launch_dependents();
+    ptx::griddep_wait();
     P px;
     px.init(smem, lane, lanes, nvec);
-    float wf[EPT], bf[EPT];
-#pragma unroll
-    for (int s = 0; s < NV; ++s) {
-        float a[VEC], c[VEC];
-        const int v = s * lanes + lane;
-        if (v < nvec) {
-            load_weight(a, w, static_cast<int64_t>(v) * VEC, 1.0f);
-            load_weight(c, b, static_cast<int64_t>(v) * VEC, 0.0f);
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) { wf[s * VEC + i] = a[i]; bf[s * VEC + i] = c[i]; }
-        }
-    }
     // every lane of a warp makes the same number of trips: the shuffles name all of them
     const int64_t first = WARP ? group - (threadIdx.x & 31) / lanes : group;
     const int64_t off = group - first;
@@ -161,42 +210,47 @@ ln_forward_kernel(T* y, int64_t ldy, float* __restrict__ mean_out, float* __rest
         px.request(x + r * ldx, r < rows, k, lane, lanes, nvec);
         if (P::ASYNC) ptx::cp_async_commit();
     }
+    float2 wf[E / 2], bf[E / 2];
+    get_weights<VEC, E>(wf, w, 1.0f, lane, lanes, nvec);
+    get_weights<VEC, E>(bf, b, 0.0f, lane, lanes, nvec);
     int stage = 0, flip = 0;
     for (int64_t r0 = first; r0 < rows; r0 += groups) {
         const int64_t r = r0 + off;
         const bool has = r < rows;
         if constexpr (P::ASYNC) ptx::cp_async_wait<AHEAD - 1>();
         else px.request(x + r * ldx, has, 0, lane, lanes, nvec);
-        float f[EPT], sum = 0.0f;
-#pragma unroll
-        for (int s = 0; s < NV; ++s) {
-            Raw<T, VEC> raw;
-            px.get(raw, stage, s);
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                f[s * VEC + i] = to_f(raw.e[i]);
-                sum += f[s * VEC + i];
-            }
-        }
+        float2 f[E / 2];
+        get_pairs<VEC, E, P, T>(f, px, stage);
         if constexpr (P::ASYNC) {
             const int64_t rn = r + AHEAD * groups;
             px.request(x + rn * ldx, rn < rows, (stage + AHEAD) % P::STAGES, lane, lanes, nvec);
             ptx::cp_async_commit();
             stage = stage + 1 == P::STAGES ? 0 : stage + 1;
         }
-        sum = lanes_sum(sum, WARP ? lanes : 32);
+        float2 s2 = f[0];
+#pragma unroll
+        for (int j = 1; j < E / 2; ++j) s2 = add2(s2, f[j]);
+        const float sum = lanes_sum(s2.x + s2.y, WARP ? lanes : 32);
         const float near = sum * warp_inv;               // the mean over this warp's elements
-        float sq = 0.0f;
+        float2 q2 = both(0.0f);
 #pragma unroll
-        for (int s = 0; s < NV; ++s) {
+        for (int s = 0; s < NV; s += VEC == 1 ? 2 : 1) {
             const bool in = s * lanes + lane < nvec;
+            if constexpr (VEC == 1) {
+                float2 g = f[s / 2];                     // beyond the row: no difference
+                if (!in) g.x = near;
+                if ((s + 1) * lanes + lane >= nvec) g.y = near;
+                const float2 d = add2(g, both(-near));
+                q2 = fma2(d, d, q2);
+            } else if (in) {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const float d = f[s * VEC + i] - near;
-                if (in) sq = fmaf(d, d, sq);
+                for (int i = 0; i < VEC; i += 2) {
+                    const float2 d = add2(f[(s * VEC + i) / 2], both(-near));
+                    q2 = fma2(d, d, q2);
+                }
             }
         }
-        sq = lanes_sum(sq, WARP ? lanes : 32);
+        float sq = lanes_sum(q2.x + q2.y, WARP ? lanes : 32);
         float mean = near;
         if (!WARP) {
             // the squares from the common mean: those from the warp's own, and its distance
@@ -211,21 +265,15 @@ ln_forward_kernel(T* y, int64_t ldy, float* __restrict__ mean_out, float* __rest
             const float d = fmaf(q.x, n.y, -mean);
             sq = lanes_sum(fmaf(n.x * d, d, q.y), MAX_WARPS);
         }
-        const float rstd = rsqrtf(sq * inv_n + eps);
-        if (has && lane == 0) {
+        const float rstd = rsqrtf(fmaf(sq, inv_n, eps));
+        if (!has) continue;
+        if (lane == 0) {
             if (mean_out) mean_out[r] = mean;
             if (rstd_out) rstd_out[r] = rstd;
         }
-        T* yr = y + r * ldy;
 #pragma unroll
-        for (int s = 0; s < NV; ++s) {
-            const int v = s * lanes + lane;
-            if (!has || v >= nvec) continue;
-            float o[VEC];
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) o[i] = fmaf((f[s * VEC + i] - mean) * rstd, wf[s * VEC + i], bf[s * VEC + i]);
-            store_f<true>(yr + static_cast<int64_t>(v) * VEC, o);
-        }
+        for (int j = 0; j < E / 2; ++j) f[j] = fma2(mul2(add2(f[j], both(-mean)), both(rstd)), wf[j], bf[j]);
+        put_pairs<VEC, E>(y + r * ldy, f, lane, lanes, nvec);
     }
 }
 
@@ -250,6 +298,8 @@ ln_forward_long_kernel(T* y, int64_t ldy, float* __restrict__ mean_out, float* _
 {
     __shared__ float2 buf[2][MAX_WARPS];
     const int64_t nvec = cols / VEC;
+    ptx::griddep_launch_dependents();
+    ptx::griddep_wait();
     for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
         const T* xr = x + r * ldx;
         float sum = 0.0f;
@@ -298,7 +348,7 @@ ln_backward_kernel(T* dx, int64_t lddx, float* __restrict__ partial, const T* dy
                    int64_t ldx, const W* __restrict__ w, const float* __restrict__ mean_in,
                    const float* __restrict__ rstd_in, int64_t rows, int cols, int accumulate, int lanes)
 {
-    using P = Pieces<T, VEC>;
+    using P = Pieces<T, VEC, EPT>;
     constexpr int NV = P::NV, AHEAD = P::AHEAD;
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ float2 part[2][MAX_WARPS];                // two buffers, one barrier a row
@@ -310,19 +360,8 @@ ln_backward_kernel(T* dx, int64_t lddx, float* __restrict__ partial, const T* dy
     P px, py;
     px.init(smem, lane, lanes, nvec);
     py.init(smem + blockDim.x * P::SMEM, lane, lanes, nvec);
-    float dw[EPT], db[EPT], wf[EPT];
-#pragma unroll
-    for (int i = 0; i < EPT; ++i) dw[i] = db[i] = wf[i] = 0.0f;
-#pragma unroll
-    for (int s = 0; s < NV; ++s) {
-        const int v = s * lanes + lane;
-        if (v < nvec) {
-            float a[VEC];
-            load_weight(a, w, static_cast<int64_t>(v) * VEC, 1.0f);
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) wf[s * VEC + i] = a[i];
-        }
-    }
+    ptx::griddep_launch_dependents();
+    ptx::griddep_wait();
     const int64_t first = WARP ? group - (threadIdx.x & 31) / lanes : group;
     const int64_t off = group - first;
     auto request = [&](int64_t r, int stage) {
@@ -332,6 +371,10 @@ ln_backward_kernel(T* dx, int64_t lddx, float* __restrict__ partial, const T* dy
     };
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) request(first + k * groups + off, k);
+    float2 dw2[EPT / 2], db2[EPT / 2], wf[EPT / 2];
+#pragma unroll
+    for (int j = 0; j < EPT / 2; ++j) dw2[j] = db2[j] = both(0.0f);
+    get_weights<VEC, EPT>(wf, w, 1.0f, lane, lanes, nvec);
     float mean_next = first + off < rows ? mean_in[first + off] : 0.0f;
     float rstd_next = first + off < rows ? rstd_in[first + off] : 0.0f;
     int stage = 0, flip = 0;
@@ -341,25 +384,19 @@ ln_backward_kernel(T* dx, int64_t lddx, float* __restrict__ partial, const T* dy
         const float mean = mean_next, rstd = rstd_next;
         if constexpr (P::ASYNC) ptx::cp_async_wait<AHEAD - 1>();
         else request(r, 0);
-        float h[EPT], d[EPT], s1 = 0.0f, s2 = 0.0f;
+        float2 h[EPT / 2], d[EPT / 2], a1 = both(0.0f), a2 = both(0.0f);
         if (!WARP || has) {
             // (beyond the row dy is zero, and so is all that is added up)
+            get_pairs<VEC, EPT, P, T>(h, px, stage);
+            get_pairs<VEC, EPT, P, T>(d, py, stage);
 #pragma unroll
-            for (int s = 0; s < NV; ++s) {
-                Raw<T, VEC> rx, ry;
-                px.get(rx, stage, s);
-                py.get(ry, stage, s);
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    const int k = s * VEC + i;
-                    h[k] = (to_f(rx.e[i]) - mean) * rstd;
-                    d[k] = to_f(ry.e[i]);
-                    dw[k] = fmaf(d[k], h[k], dw[k]);
-                    db[k] += d[k];
-                    const float g = d[k] * wf[k];
-                    s1 += g;
-                    s2 = fmaf(g, h[k], s2);
-                }
+            for (int j = 0; j < EPT / 2; ++j) {
+                h[j] = mul2(add2(h[j], both(-mean)), both(rstd));
+                dw2[j] = fma2(d[j], h[j], dw2[j]);
+                db2[j] = add2(db2[j], d[j]);
+                d[j] = mul2(d[j], wf[j]);                // from here on dy * weight
+                a1 = add2(a1, d[j]);
+                a2 = fma2(d[j], h[j], a2);
             }
         }
         if (r + groups < rows) {
@@ -370,8 +407,8 @@ ln_backward_kernel(T* dx, int64_t lddx, float* __restrict__ partial, const T* dy
             request(r + AHEAD * groups, (stage + AHEAD) % P::STAGES);
             stage = stage + 1 == P::STAGES ? 0 : stage + 1;
         }
-        s1 = lanes_sum(s1, WARP ? lanes : 32);
-        s2 = lanes_sum(s2, WARP ? lanes : 32);
+        float s1 = lanes_sum(a1.x + a1.y, WARP ? lanes : 32);
+        float s2 = lanes_sum(a2.x + a2.y, WARP ? lanes : 32);
         if (!WARP) {
             float2* p = part[flip];
             flip ^= 1;
@@ -382,30 +419,30 @@ ln_backward_kernel(T* dx, int64_t lddx, float* __restrict__ partial, const T* dy
             s1 = lanes_sum(q.x, MAX_WARPS);
             s2 = lanes_sum(q.y, MAX_WARPS);
         }
-        if (dx) {
+        if (dx && has) {
             const float m1 = s1 * inv_n, m2 = s2 * inv_n;
             T* dr = dx + r * lddx;
 #pragma unroll
-            for (int s = 0; s < NV; ++s) {
-                const int v = s * lanes + lane;
-                if (!has || v >= nvec) continue;
-                float o[VEC];
-                if (accumulate) {
-                    load_f<true>(o, dr + static_cast<int64_t>(v) * VEC);
-                } else {
+            for (int j = 0; j < EPT / 2; ++j) d[j] = mul2(fma2(h[j], both(-m2), add2(d[j], both(-m1))), both(rstd));
+            if (accumulate) {
 #pragma unroll
-                    for (int i = 0; i < VEC; ++i) o[i] = 0.0f;
-                }
+                for (int s = 0; s < NV; ++s) {
+                    if (s * lanes + lane >= nvec) continue;
+                    float o[VEC];
+                    load_f<true>(o, dr + static_cast<int64_t>(s * lanes + lane) * VEC);
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    const int k = s * VEC + i;
-                    o[i] += rstd * (d[k] * wf[k] - m1 - h[k] * m2);
+                    for (int i = 0; i < VEC; ++i) {
+                        float2& t = d[(s * VEC + i) / 2];
+                        if ((s * VEC + i) & 1) t.y += o[i]; else t.x += o[i];
+                    }
                 }
-                store_f<true>(dr + static_cast<int64_t>(v) * VEC, o);
             }
+            put_pairs<VEC, EPT>(dr, d, lane, lanes, nvec);
         }
     }
     if (!partial) return;
+    const float* dw = reinterpret_cast<const float*>(dw2);
+    const float* db = reinterpret_cast<const float*>(db2);
     float* pw = partial + static_cast<int64_t>(blockIdx.x) * cols;
     float* pb = pw + static_cast<int64_t>(gridDim.x) * cols;
     if (!WARP) {
@@ -526,6 +563,8 @@ ln_reduce_kernel(W* __restrict__ dweight, W* __restrict__ dbias, const float* __
                  int64_t cols, int accumulate)
 {
     __shared__ float sh[32][33];
+    ptx::griddep_launch_dependents();
+    ptx::griddep_wait();
     W* out = blockIdx.y ? dbias : dweight;
     if (!out) return;
     const float* src = partial + static_cast<int64_t>(blockIdx.y) * parts * cols;
@@ -562,15 +601,15 @@ struct Shape {
     int64_t blocks;     // that the rows give work to
 };
 
-Shape shape_of(int64_t rows, int64_t cols, int vec)
+Shape shape_of(int64_t rows, int64_t cols, int vec, int ept)
 {
     Shape s{};
-    const int64_t threads = cols > REGISTER_COLS ? MAX_THREADS : (cols / vec + EPT / vec - 1) / (EPT / vec);
+    const int64_t threads = (cols / vec + ept / vec - 1) / (ept / vec);
     if (threads <= 32) {
         s.lanes = power_of_two_at_least(threads);
         s.block = GROUP_BLOCK;
     } else {
-        s.lanes = s.block = static_cast<int>((threads + 31) / 32 * 32);
+        s.lanes = s.block = threads > MAX_THREADS ? MAX_THREADS : static_cast<int>((threads + 31) / 32 * 32);
     }
     const int64_t per_block = s.block / s.lanes;
     s.blocks = (rows + per_block - 1) / per_block;
@@ -681,20 +720,30 @@ extern "C" int sb200_layer_norm(sb200_ctx* ctx, void* y, int64_t ldy, float* mea
         const int width = access_width<T, W>(cols, weight, bias, {{x, ldx}, {y, ldy}});
         return with_width<T>(width, [&](auto v) -> int {
             constexpr int VEC = decltype(v)::value;
-            const Shape s = shape_of(rows, cols, VEC);
+            // 32 elements a thread for rows of more than 512 columns, so that a warp holds 1024;
+            // 16 where 2-byte accesses hold every element in a register of its own
+            constexpr bool WIDE = VEC * sizeof(T) >= 4;
+            constexpr int MANY = WIDE ? 32 : 16;
+            const bool many = WIDE && cols > 16 * 32;
+            const Shape s = shape_of(rows, cols, VEC, many ? MANY : 16);
             auto launch = [&](auto kern, int smem, auto... last) -> int {
                 const int64_t most = resident_blocks(ctx, kern, s.block, smem);
                 if (most < 1) return SB200_ERR_CUDA;
-                kern.run<<<static_cast<unsigned>(s.blocks < most ? s.blocks : most), s.block, smem, stream>>>(
-                    static_cast<T*>(y), ldy, mean, rstd, static_cast<const T*>(x), ldx, static_cast<const W*>(weight),
-                    static_cast<const W*>(bias), rows, last...);
-                ctx->launches += 1;
-                return static_cast<int>(cudaGetLastError() == cudaSuccess ? SB200_OK : SB200_ERR_CUDA);
+                return launch_after(ctx, kern.run, static_cast<unsigned>(s.blocks < most ? s.blocks : most), s.block, smem, stream, static_cast<T*>(y), ldy, mean,
+                                    rstd, static_cast<const T*>(x), ldx, static_cast<const W*>(weight), static_cast<const W*>(bias), rows,
+                                    last...);
             };
-            const int smem = s.block * Pieces<T, VEC>::SMEM, n = static_cast<int>(cols > REGISTER_COLS ? 0 : cols);
-            if (cols > REGISTER_COLS) return launch(Kernel<ln_forward_long_kernel<T, W, VEC>>{}, 0, cols, eps);
-            if (s.lanes <= 32) return launch(Kernel<ln_forward_kernel<T, W, VEC, true>>{}, smem, n, eps, s.lanes);
-            return launch(Kernel<ln_forward_kernel<T, W, VEC, false>>{}, smem, n, eps, s.lanes);
+            if (cols > MANY * MAX_THREADS) return launch(Kernel<ln_forward_long_kernel<T, W, VEC>>{}, 0, cols, eps);
+            const int n = static_cast<int>(cols);
+            if (many) {
+                const int smem = s.block * Pieces<T, VEC, MANY>::SMEM;
+                if (s.lanes <= 32) return launch(Kernel<ln_forward_kernel<T, W, VEC, MANY, true>>{}, smem, n, eps, s.lanes);
+                return launch(Kernel<ln_forward_kernel<T, W, VEC, MANY, false>>{}, smem, n, eps, s.lanes);
+            }
+            const int smem = s.block * Pieces<T, VEC, 16>::SMEM;
+            if (s.lanes <= 32) return launch(Kernel<ln_forward_kernel<T, W, VEC, 16, true>>{}, smem, n, eps, s.lanes);
+            if constexpr (WIDE) return SB200_ERR_INVALID_ARG;    // (not reached: such rows have 32 elements a thread)
+            else return launch(Kernel<ln_forward_kernel<T, W, VEC, 16, false>>{}, smem, n, eps, s.lanes);
         });
     });
 }
@@ -738,7 +787,7 @@ extern "C" int sb200_layer_norm_backward(sb200_ctx* ctx, void* dx, int64_t lddx,
             const int64_t bound = backward_parts(ctx->sm_count, rows, cols);
             const int rc = with_width<T>(width, [&](auto v) -> int {
                 constexpr int VEC = decltype(v)::value;
-                const Shape s = shape_of(rows, cols, VEC);
+                const Shape s = shape_of(rows, cols, VEC, EPT);
                 if (cols > REGISTER_COLS) {
                     // the column sums first: dx may overwrite dy
                     if (sums) {
@@ -759,17 +808,15 @@ extern "C" int sb200_layer_norm_backward(sb200_ctx* ctx, void* dx, int64_t lddx,
                 }
                 const int n = static_cast<int>(cols);
                 auto launch = [&](auto kern) -> int {
-                    int smem = 2 * s.block * Pieces<T, VEC>::SMEM;
+                    int smem = 2 * s.block * Pieces<T, VEC, EPT>::SMEM;
                     if (s.lanes <= 32 && smem < 2 * 32 * EPT * 4) smem = 2 * 32 * EPT * 4;      // column sums of such rows
                     const int64_t most = resident_blocks(ctx, kern, s.block, smem);
                     if (most < 1) return SB200_ERR_CUDA;
                     int64_t grid = s.blocks < most ? s.blocks : most;
                     if (grid > bound) grid = bound;
                     parts = static_cast<int>(grid);
-                    kern.run<<<static_cast<unsigned>(grid), s.block, smem, stream>>>(dxp, lddx, partial, yp, lddy, xp, ldx, wp, mean, rstd, rows, n,
-                                                                                 accumulate_dx, s.lanes);
-                    ctx->launches += 1;
-                    return SB200_OK;
+                    return launch_after(ctx, kern.run, static_cast<unsigned>(grid), s.block, smem, stream, dxp, lddx, partial, yp, lddy, xp, ldx, wp, mean, rstd,
+                                        rows, n, accumulate_dx, s.lanes);
                 };
                 return s.lanes <= 32 ? launch(Kernel<ln_backward_kernel<T, W, VEC, true>>{}) : launch(Kernel<ln_backward_kernel<T, W, VEC, false>>{});
             });
@@ -777,8 +824,8 @@ extern "C" int sb200_layer_norm_backward(sb200_ctx* ctx, void* dx, int64_t lddx,
         }
         if (sums) {
             const dim3 grid(static_cast<unsigned>((cols + 31) / 32), 2);
-            ln_reduce_kernel<W><<<grid, 1024, 0, stream>>>(static_cast<W*>(dweight), static_cast<W*>(dbias), partial, parts, cols, accumulate_weight);
-            ctx->launches += 1;
+            if (const int rc = launch_after(ctx, ln_reduce_kernel<W>, grid, 1024, 0, stream, static_cast<W*>(dweight), static_cast<W*>(dbias),
+                                            partial, parts, cols, accumulate_weight)) return rc;
         }
         return static_cast<int>(cudaGetLastError() == cudaSuccess ? SB200_OK : SB200_ERR_CUDA);
     });

@@ -33,6 +33,25 @@ struct DeviceGuard {
 
 inline bool aligned_to(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
+// A launch that may overlap the tail of the kernel before; the kernel itself waits for that
+// one (ptx::griddep_wait) before it touches global memory.
+template <typename... A, typename... B>
+inline int launch_after(sb200_ctx* ctx, void (*kern)(A...), dim3 grid, int block, size_t smem, cudaStream_t stream, B... args)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(static_cast<unsigned>(block));
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    ctx->launches += 1;
+    return cudaLaunchKernelEx(&cfg, kern, static_cast<A>(args)...) == cudaSuccess ? SB200_OK : SB200_ERR_CUDA;
+}
+
 __device__ __forceinline__ float to_f(float x) { return x; }
 __device__ __forceinline__ float to_f(bf16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float to_f(f16 x) { return __half2float(x); }
@@ -40,6 +59,42 @@ template <typename T> __device__ __forceinline__ T from_f(float x);
 template <> __device__ __forceinline__ float from_f<float>(float x) { return x; }
 template <> __device__ __forceinline__ bf16 from_f<bf16>(float x) { return __float2bfloat16_rn(x); }
 template <> __device__ __forceinline__ f16 from_f<f16>(float x) { return __float2half_rn(x); }
+
+// Two fp32 operations an instruction (each element rounded as by the scalar one).
+__device__ __forceinline__ float2 add2(float2 a, float2 b)
+{
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b)
+{
+    float2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)));
+    return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
+{
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)),
+          "l"(reinterpret_cast<const unsigned long long&>(c)));
+    return d;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
+// Two neighbouring elements of an array, as fp32.
+__device__ __forceinline__ float2 pair_f(const float* p) { return make_float2(p[0], p[1]); }
+__device__ __forceinline__ float2 pair_f(const bf16* p) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(p)); }
+__device__ __forceinline__ float2 pair_f(const f16* p) { return __half22float2(*reinterpret_cast<const __half2*>(p)); }
+__device__ __forceinline__ void set_pair(float* p, float2 v) { p[0] = v.x; p[1] = v.y; }
+__device__ __forceinline__ void set_pair(bf16* p, float2 v) { *reinterpret_cast<__nv_bfloat162*>(p) = __float22bfloat162_rn(v); }
+__device__ __forceinline__ void set_pair(f16* p, float2 v) { *reinterpret_cast<__half2*>(p) = __float22half2_rn(v); }
 
 // VEC consecutive elements as raw words; the pointer is aligned to min(16, VEC * sizeof(T)).
 template <typename T, int VEC>
