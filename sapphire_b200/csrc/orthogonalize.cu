@@ -29,7 +29,7 @@
 #include <type_traits>
 
 #include "gemm_common.cuh"
-#include "typed.cuh"
+#include "orthogonalize.cuh"
 
 namespace sb200 {
 
@@ -41,9 +41,8 @@ constexpr int KB = 64;                           // fp16 elements of k per block
 constexpr int MMA_K = 16;
 constexpr int TILE_BYTES = 128 * KB * 2;         // 128 rows (or columns) x 64 k
 constexpr int MN_CHUNK_BYTES = 64 * KB * 2;      // MN-major: 64 k rows x 64 columns
-constexpr int CHUNK_KB = 2;                      // k-blocks per accumulation chain with two parts
-constexpr float SCALE = 8192.0f;                 // 2^13
-constexpr float INV_SCALE = 1.0f / 8192.0f;
+constexpr int CHUNK_KB = 2;                      // k-blocks per accumulation chain with two parts (1 in the sliced kernel)
+constexpr float SCALE = ORTH_SCALE, INV_SCALE = ORTH_INV_SCALE;
 constexpr double LARGEST = 7.5;                  // of a singular value: 7.5 * 2^13 < 65504
 constexpr int EPI_WARPS = 16;
 constexpr int THREADS = 64 + EPI_WARPS * 32;
@@ -123,29 +122,6 @@ __device__ __forceinline__ void orth_tile(int t, const OrthParams& p, bool symme
     }
     tm = row;
     tn = row + t;
-}
-
-template <int N>
-__device__ __forceinline__ void split_f16(const float* v, Raw<f16, N>& hi, Raw<f16, N>& lo)
-{
-#pragma unroll
-    for (int e = 0; e < N; e += 2) {
-        const __half2 h = __floats2half2_rn(v[e], v[e + 1]);
-        const float2 f = __half22float2(h);
-        *reinterpret_cast<__half2*>(&hi.e[e]) = h;
-        *reinterpret_cast<__half2*>(&lo.e[e]) = __floats2half2_rn(v[e] - f.x, v[e + 1] - f.y);
-    }
-}
-
-// hi + lo of eight elements
-__device__ __forceinline__ void join_f16(float (&v)[8], const Raw<f16, 8>& hi)
-{
-#pragma unroll
-    for (int e = 0; e < 8; e += 2) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi.e[e]));
-        v[e] += f.x;
-        v[e + 1] += f.y;
-    }
 }
 
 __device__ __forceinline__ void store_transposed(const Raw<f16, 8>& hi, const Raw<f16, 8>& lo, f16* out, const Split& m,
@@ -564,12 +540,12 @@ orth_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         // order.  A warp takes whole rows, so that what crosses between the SMs and what goes
         // to memory are runs of 512 and 256 bytes (a thread a row took 8 us for 64 KB).
         __syncthreads();
+        const int share = 128 / p.slices;
         ptx::cluster_sync();
         if (warp >= 2 && *abort_flag == 0) {
             const int b = unit / p.tiles;
             int tm, tn;
             orth_tile(unit % p.tiles, p, SYMMETRIC, tm, tn);
-            const int share = 128 / p.slices;
             const int first = static_cast<int>(rank) * share;    // of this CTA's rows
             const int col = tn * BN + lane * 4;
             const bool mirror = SYMMETRIC && tn > tm;
@@ -730,7 +706,7 @@ orth_split_kernel(Split x, const double* __restrict__ partial, int parts, const 
                   int64_t stride, int64_t rows, int64_t cols, float eps)
 {
     __shared__ float tile[TALL ? 64 : 1][65];
-    __shared__ float inv_sh;
+    __shared__ double squares;
     const T* m = g + blockIdx.z * stride;
     const int64_t r0 = static_cast<int64_t>(blockIdx.y) * 64, c0 = static_cast<int64_t>(blockIdx.x) * 64;
     const int tx = (threadIdx.x & 7) * 8, ty = threadIdx.x >> 3;
@@ -751,10 +727,10 @@ orth_split_kernel(Split x, const double* __restrict__ partial, int parts, const 
         for (int i = threadIdx.x; i < parts; i += 32) s += partial[blockIdx.z * parts + i];
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (threadIdx.x == 0) inv_sh = static_cast<float>(static_cast<double>(SCALE) / (sqrt(s) + static_cast<double>(eps)));
+        if (threadIdx.x == 0) squares = s;
     }
     __syncthreads();
-    const float inv = inv_sh;
+    const OrthInverse inv(squares, eps);
     f16* out = x.p + blockIdx.z * x.batch_stride;
     const int64_t xr0 = TALL ? c0 : r0, xc0 = TALL ? r0 : c0, xrows = TALL ? cols : rows;
     if (TALL) {
@@ -770,7 +746,7 @@ orth_split_kernel(Split x, const double* __restrict__ partial, int parts, const 
         if (r >= xrows) continue;
         float v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = (TALL ? tile[tx + e][ty + k * 32] : to_f(in[k].e[e])) * inv;
+        for (int e = 0; e < 8; ++e) v[e] = inv(TALL ? tile[tx + e][ty + k * 32] : to_f(in[k].e[e]));
         Raw<f16, 8> hi, lo;
         split_f16(v, hi, lo);
         f16* o = out + r * x.ld + xc0 + tx;      // the pitch is a multiple of 64: the columns fit
@@ -888,6 +864,7 @@ template <int WHAT>
 int product(sb200_ctx* ctx, bool split, const OrthMaps& m, OrthParams p, cudaStream_t stream)
 {
     p.slices = slices_for(ctx, p.rows, p.cols, p.batch, p.num_kb, WHAT != APPLY, split);
+    p.chunk_kb = !split ? p.num_kb : p.slices == 0 ? CHUNK_KB : 1;
     if (p.slices == 0)
         return split ? launch_product<WHAT, true, true>(ctx, m, p, stream) : launch_product<WHAT, true, false>(ctx, m, p, stream);
     return split ? launch_product<WHAT, false, true>(ctx, m, p, stream) : launch_product<WHAT, false, false>(ctx, m, p, stream);
@@ -969,6 +946,8 @@ extern "C" int sb200_orthogonalize(sb200_ctx* ctx, void* out, int64_t ldo, int64
     DeviceGuard dev(ctx->device);
     if (!dev.ok) return SB200_ERR_CUDA;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    const OrthCall call{out, ldo, batch > 1 ? stride_out : 0, g, ldg, batch > 1 ? stride_g : 0, rows, cols, batch, steps, a, b, c, eps, type};
+    if (orthogonalize_small_fits(ctx, call)) return launch_orthogonalize_small(ctx, call, stream);
     unsigned char* ws = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~uintptr_t(255));
     const int tall = rows > cols;
 
@@ -1029,7 +1008,6 @@ extern "C" int sb200_orthogonalize(sb200_ctx* ctx, void* out, int64_t ldo, int64
         // A = X X^T
         p.rows = p.cols = p.R;
         p.num_kb = kb_c;
-        p.chunk_kb = q.split ? CHUNK_KB : kb_c;
         p.prev = p.out = A;
         p.out_parts = q.split ? 2 : 1;
         p.alpha = INV_SCALE;
@@ -1037,7 +1015,6 @@ extern "C" int sb200_orthogonalize(sb200_ctx* ctx, void* out, int64_t ldo, int64
         if (const int rc = product<GRAM>(ctx, q.split, {x_rows[from], x_rows[from]}, p, stream)) return rc;
         // B = b A + c A A (+ a on the diagonal)
         p.num_kb = kb_r;
-        p.chunk_kb = q.split ? CHUNK_KB : kb_r;
         p.out = B;
         p.coef = b;
         p.alpha = c * INV_SCALE;

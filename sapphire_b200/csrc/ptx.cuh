@@ -345,6 +345,18 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t cluster_addr)
     return v;
 }
 
+__device__ __forceinline__ double ld_cluster_f64(uint32_t cluster_addr)
+{
+    double v;
+    asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(cluster_addr) : "memory");
+    return v;
+}
+
+__device__ __forceinline__ void st_cluster_b64(uint32_t cluster_addr, uint2 v)
+{
+    asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(cluster_addr), "r"(v.x), "r"(v.y) : "memory");
+}
+
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr)
 {
     // default (CTA-scope release) semantics: what the arrival orders are this
