@@ -219,7 +219,7 @@ constexpr int SMALL_TOKENS = SORT_THREADS * SMALL_ROUNDS;
 constexpr int SMALL_SMEM = SMALL_TOKENS * 6 + SORT_WARPS * DIGITS * 2 + DIGITS * 4 + SORT_WARPS * 4;
 
 // Fills rows [v0, v1) with zeros, those marked in `touched` (if any) left out; `lanes` (power
-// of two) threads a row.
+// of two) threads a row.  A word of marks serves 32 rows.
 template <typename TT, int VEC>
 __device__ __forceinline__ void zero_rows(TT* dtable, int64_t ldt, int64_t nvec, int64_t v0, int64_t v1,
                                           const uint32_t* touched)
@@ -230,8 +230,14 @@ __device__ __forceinline__ void zero_rows(TT* dtable, int64_t ldt, int64_t nvec,
     int lanes = 1;
     while (lanes < nvec && lanes < static_cast<int>(blockDim.x)) lanes <<= 1;
     const int lane = threadIdx.x & (lanes - 1), rows = blockDim.x / lanes;
+    uint32_t marks = 0;
+    int64_t marks_of = -1;
     for (int64_t v = v0 + threadIdx.x / lanes; v < v1; v += rows) {
-        if (touched && ((touched[v >> 5] >> (v & 31)) & 1u)) continue;
+        if (touched && (v >> 5) != marks_of) {
+            marks_of = v >> 5;
+            marks = touched[marks_of];
+        }
+        if ((marks >> (v & 31)) & 1u) continue;
         TT* row = dtable + v * ldt;
 #pragma unroll 4
         for (int64_t k = lane; k < nvec; k += lanes) store_raw<true>(row + k * VEC, zero);
@@ -338,6 +344,7 @@ constexpr int GRAD_THREADS = 256;
 constexpr int GRAD_UNROLL = 8;           // token rows a thread has in flight
 constexpr int MAX_PIECE = 1024;          // sorted tokens per piece at most
 constexpr int64_t ZERO_UNIT = 64 * 1024; // bytes of the table a block fills, about
+constexpr int64_t ZERO_ROWS = 256;       // and rows at most
 
 template <typename TT, int VEC>
 __device__ __forceinline__ void write_row(TT* p, const float (&sum)[VEC], float scale, int accumulate)
@@ -360,16 +367,20 @@ struct GradArgs {
     uint32_t* long_runs;         // count, then from word 2 the pieces in which long runs start, and their rows
     const uint32_t* touched;     // rows that occur (null: nothing is filled with zeros)
     int64_t n, vocab, nvec, ldt, ldo;
-    int64_t units, zero_units, zero_rows;        // pieces x column tiles; blocks that fill zero_rows rows each
-    int piece, tiles, accumulate;
+    int64_t units, zero_units, zero_rows;        // pieces (`groups` a block) x column tiles; blocks that fill zero_rows rows each
+    int64_t pieces;
+    int piece, groups, tiles, accumulate;
     float scale;
 };
 
 // Blocks that add up a piece's share of one column tile, and blocks that fill rows with
 // zeros, in proportion.  edge: sums of long runs (more tokens than a piece): [0] of a run
 // that came in from the piece before, whether or not it goes on; [1] of one that starts here.
-template <typename TT, typename TA, int VEC>
-__global__ void __launch_bounds__(GRAD_THREADS)
+// Four blocks of 256 threads an SM (64 registers), six where an access is short: with three
+// it is a tenth slower.
+// ONE: one piece a block (compiled apart: known places of the window are worth a tenth).
+template <typename TT, typename TA, int VEC, bool ONE>
+__global__ void __launch_bounds__(GRAD_THREADS, VEC < 4 ? 6 : VEC == 8 && sizeof(TA) == 4 ? 2 : 4)
 grad_pieces_kernel(TT* __restrict__ dtable, const TA* __restrict__ dout, const GradArgs a)
 {
     ptx::griddep_launch_dependents();
@@ -384,25 +395,32 @@ grad_pieces_kernel(TT* __restrict__ dtable, const TA* __restrict__ dout, const G
         }
         unit -= z;
     }
-    extern __shared__ uint32_t window[];                     // keys of [i0 - piece - 1, i1 + piece], positions of [i0, i1 + piece)
-    __shared__ int first_from, first_to, last_from, last_to; // the runs at the piece's ends, relative to i0
-    const int piece = a.piece;
-    const int64_t p = unit / a.tiles, i0 = p * piece;
-    const int count = static_cast<int>(min(static_cast<int64_t>(piece), a.n - i0));
+    // Narrow tables: several pieces to a block, a group of lanes each.
+    extern __shared__ uint32_t windows[];        // per group: keys of [i0 - piece - 1, i1 + piece], positions of [i0, i1 + piece)
+    __shared__ int ends[GRAD_THREADS / 32][4];   // where the runs at the piece's ends begin and end, relative to i0
+    const int piece = a.piece, groups = ONE ? 1 : a.groups, lanes = ONE ? blockDim.x : blockDim.x / groups;
+    const int group = ONE ? 0 : threadIdx.x / lanes, lane = ONE ? threadIdx.x : threadIdx.x % lanes;
+    const int64_t p = unit / a.tiles * groups + group, i0 = p * piece;
+    const int count = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(piece), a.n - i0)));
+    uint32_t* window = windows + group * (5 * piece + 2);
     const uint32_t* key = window + piece + 1;                // key[i]: of sorted token i0 + i
     uint32_t* spos = window + 3 * piece + 2;
-    for (int i = threadIdx.x; i < 3 * piece + 2; i += blockDim.x) {
+    int& first_from = ends[group][0];
+    int& first_to = ends[group][1];
+    int& last_from = ends[group][2];
+    int& last_to = ends[group][3];
+    for (int i = lane; i < 3 * piece + 2; i += lanes) {
         const int64_t at = i0 + i - piece - 1;
         window[i] = at >= 0 && at < a.n ? a.keys[at] : 0xffffffffu;      // no row's key
     }
-    for (int i = threadIdx.x; i < 2 * piece; i += blockDim.x) spos[i] = i0 + i < a.n ? a.pos[i0 + i] : 0;
-    if (threadIdx.x == 0) {
+    for (int i = lane; i < 2 * piece; i += lanes) spos[i] = i0 + i < a.n ? a.pos[i0 + i] : 0;
+    if (lane == 0) {
         first_from = last_from = -piece;
         first_to = last_to = count + piece;
     }
     __syncthreads();
-    const uint32_t k_first = key[0], k_last = key[count - 1];
-    for (int i = static_cast<int>(threadIdx.x) - piece; i < count + piece; i += blockDim.x) {
+    const uint32_t k_first = key[0], k_last = key[count > 0 ? count - 1 : 0];
+    for (int i = lane - piece; i < count + piece; i += lanes) {
         const uint32_t k = key[i];
         if (i < 0 && k != k_first) atomicMax(&first_from, i + 1);
         if (i >= 0 && k != k_first) atomicMin(&first_to, i);
@@ -410,18 +428,19 @@ grad_pieces_kernel(TT* __restrict__ dtable, const TA* __restrict__ dout, const G
         if (i >= count && k != k_last) atomicMin(&last_to, i);
     }
     __syncthreads();
+    if (count == 0) return;                      // a group behind the last piece
     // a run that came in: a short one is its first piece's, of a long one this piece has a part
     const bool came_in = key[-1] == k_first;
     const bool first_long = came_in && first_to - first_from > piece;
     const int begin = came_in && !first_long ? first_to : 0;
     // a run that starts here and goes on: a short one to its end, of a long one the part here
-    const bool goes_on = key[count] == k_last && last_from >= 0 && !(came_in && last_from <= 0);
+    const bool goes_on = key[count] == k_last && last_from >= 0;
     const bool last_long = goes_on && last_to - last_from > piece;
     const int end = goes_on && !last_long ? last_to : count;
     const int tile = static_cast<int>(unit % a.tiles);
-    if (threadIdx.x == 0 && tile == 0 && last_long && k_last < a.vocab)
+    if (lane == 0 && tile == 0 && last_long && k_last < a.vocab)
         reinterpret_cast<uint2*>(a.long_runs)[1 + atomicAdd(a.long_runs, 1u)] = make_uint2(static_cast<uint32_t>(p), k_last);
-    const int64_t v = static_cast<int64_t>(tile) * blockDim.x + threadIdx.x;
+    const int64_t v = static_cast<int64_t>(tile) * lanes + lane;
     if (v >= a.nvec) return;
     const TA* src = dout + v * VEC;
     float sum[VEC];
@@ -465,7 +484,7 @@ grad_join_kernel(TT* __restrict__ dtable, const GradArgs a, int lanes, int col_t
 {
     ptx::griddep_wait();
     __shared__ float part[GRAD_THREADS * VEC];
-    const int64_t runs = *a.long_runs, pieces = (a.n + a.piece - 1) / a.piece;
+    const int64_t runs = *a.long_runs;
     const int lane = threadIdx.x % lanes, slice = threadIdx.x / lanes, slices = blockDim.x / lanes;
     for (int64_t job = blockIdx.x; job < runs * col_tiles; job += gridDim.x) {
         const uint2 run = reinterpret_cast<const uint2*>(a.long_runs)[1 + job / col_tiles];
@@ -475,7 +494,7 @@ grad_join_kernel(TT* __restrict__ dtable, const GradArgs a, int lanes, int col_t
         int64_t parts = 1;                                   // this piece's [1], then [0] of the next ones
         for (;;) {
             const int64_t q = p + parts + threadIdx.x;
-            const int same = __syncthreads_count(q < pieces && a.keys[q * a.piece] == key);
+            const int same = __syncthreads_count(q < a.pieces && a.keys[q * a.piece] == key);
             parts += same;
             if (same < static_cast<int>(blockDim.x)) break;
         }
@@ -652,20 +671,26 @@ int launch_grad(sb200_ctx* ctx, const GradPlan& g, unsigned char* ws, TT* dtable
     a.long_runs = u32(g.long_runs);
     a.touched = touched;
     a.n = n; a.vocab = vocab; a.nvec = nvec; a.ldt = ldt; a.ldo = ldo;
-    const int threads = power_of_two(nvec, GRAD_THREADS) < 32 ? 32 : power_of_two(nvec, GRAD_THREADS);
-    a.tiles = static_cast<int>((nvec + threads - 1) / threads);
-    a.units = g.pieces * a.tiles;
+    // a block of 64 to 256 threads per piece; for narrow tables a group of 32 lanes (the windows
+    // of a block's groups stay within 40 KB)
+    const int threads = nvec > 32 ? power_of_two(nvec, GRAD_THREADS) : GRAD_THREADS;
+    a.groups = nvec > 32 ? 1 : GRAD_THREADS / 32;
+    while (a.groups > 1 && a.groups * (5 * g.piece + 2) * 4 > 40 * 1024) a.groups /= 2;
+    const int lanes_each = threads / a.groups;
+    a.pieces = g.pieces;
+    a.tiles = static_cast<int>((nvec + lanes_each - 1) / lanes_each);
+    a.units = (g.pieces + a.groups - 1) / a.groups * a.tiles;
     if (touched) {
         const int64_t row = cols * static_cast<int64_t>(sizeof(TT));
-        a.zero_rows = row < ZERO_UNIT ? ZERO_UNIT / row : 1;
+        a.zero_rows = row * ZERO_ROWS < ZERO_UNIT ? ZERO_ROWS : row < ZERO_UNIT ? ZERO_UNIT / row : 1;
         a.zero_units = (vocab + a.zero_rows - 1) / a.zero_rows;
     }
     a.piece = g.piece;
     a.accumulate = accumulate;
     a.scale = scale;
     if (a.units + a.zero_units > INT32_MAX) return SB200_ERR_TOO_LARGE;
-    if (const int rc = launch_after(ctx, grad_pieces_kernel<TT, TA, VEC>, static_cast<unsigned>(a.units + a.zero_units), threads,
-                                    static_cast<size_t>(5 * g.piece + 2) * 4, stream, dtable, dout, a)) return rc;
+    if (const int rc = launch_after(ctx, a.groups == 1 ? grad_pieces_kernel<TT, TA, VEC, true> : grad_pieces_kernel<TT, TA, VEC, false>, static_cast<unsigned>(a.units + a.zero_units), threads,
+                                    static_cast<size_t>(a.groups) * (5 * g.piece + 2) * 4, stream, dtable, dout, a)) return rc;
     // few columns a block and many slices: a run of many pieces is added by slices at the same time
     const int lanes = 32, col_tiles = static_cast<int>((nvec + lanes - 1) / lanes);
     const int64_t jobs = g.pieces * col_tiles, most = 8ll * ctx->sm_count;
