@@ -631,8 +631,12 @@ int64_t resident_blocks(const sb200_ctx* ctx, Kernel<K>, int block, int smem)
     int ask = 0;
     int& n = ctx->device < DEVICES ? per_sm[ctx->device][block / 32] : ask;
     if (n == 0) {
+        // the limit for every block size: one size must not take back what another was granted
         int got = 0;
-        if (smem > 40 * 1024 && cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return 0;
+        cudaFuncAttributes attr;
+        if (cudaFuncGetAttributes(&attr, K) != cudaSuccess) return 0;
+        const int most = 227 * 1024 - static_cast<int>(attr.sharedSizeBytes);
+        if (smem > most || cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess) return 0;
         if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&got, K, block, smem) != cudaSuccess) return 0;
         n = got;
     }

@@ -557,11 +557,17 @@ def layer_norm(ctx: Context, x: torch.Tensor, weight: Optional[torch.Tensor] = N
         ldo = _rows(ctx, out, "out")[2]
     if mean is None:
         mean = torch.empty(rows if x.dim() == 2 else x.shape[:-1], dtype=torch.float32, device=ctx.torch_device)
+        mptr = mean.data_ptr()
+    else:
+        mptr = _statistic(ctx, mean, rows, "mean")
     if rstd is None:
         rstd = torch.empty_like(mean)
+        rptr = rstd.data_ptr()
+    else:
+        rptr = _statistic(ctx, rstd, rows, "rstd")
     wcode, wptr, bptr = _norm_weights(ctx, cols, code, weight, bias, ("weight", "bias"))
-    _call("sb200_layer_norm", ctx, out.data_ptr(), ldo, _statistic(ctx, mean, rows, "mean"),
-          _statistic(ctx, rstd, rows, "rstd"), x.data_ptr(), ldx, wptr, bptr, rows, cols, eps, code, wcode)
+    _call("sb200_layer_norm", ctx, out.data_ptr(), ldo, mptr, rptr, x.data_ptr(), ldx, wptr, bptr, rows, cols, eps, code,
+          wcode)
     return out, mean, rstd
 
 
@@ -587,13 +593,18 @@ def layer_norm_backward(ctx: Context, dy: torch.Tensor, x: torch.Tensor, mean: t
             raise ValueError("dx must have x's shape and dtype")
         lddx = _rows(ctx, dx, "dx")[2]
     wdtype = weight.dtype if weight is not None else dweight.dtype if dweight is not None else x.dtype
-    if dweight is None:
+    if dweight is None and dbias is None:
         dweight = torch.empty(cols, dtype=wdtype, device=ctx.torch_device)
-    if dbias is None:
-        dbias = torch.empty(cols, dtype=wdtype, device=ctx.torch_device)
-    wcode, dwptr, dbptr = _norm_weights(ctx, cols, code, dweight, dbias, ("dweight", "dbias"))
-    if dweight.dtype != wdtype:
-        raise TypeError("dweight and dbias must have the weight's dtype")
+        dbias = torch.empty_like(dweight)
+        wcode, dwptr, dbptr = _type_code(dweight, "weight"), dweight.data_ptr(), dbias.data_ptr()
+    else:
+        if dweight is None:
+            dweight = torch.empty(cols, dtype=wdtype, device=ctx.torch_device)
+        if dbias is None:
+            dbias = torch.empty(cols, dtype=wdtype, device=ctx.torch_device)
+        wcode, dwptr, dbptr = _norm_weights(ctx, cols, code, dweight, dbias, ("dweight", "dbias"))
+        if dweight.dtype != wdtype:
+            raise TypeError("dweight and dbias must have the weight's dtype")
     nbytes = L.lib().sb200_layer_norm_backward_workspace(ctx._h, rows, cols)
     ws = _scratch("sb200_layer_norm_backward", nbytes, ctx)
     _call("sb200_layer_norm_backward", ctx, dx.data_ptr(), lddx, dwptr, dbptr, dy.data_ptr(), ldy, x.data_ptr(), ldx,

@@ -349,6 +349,19 @@ def test_layer_norm_large_offsets(ctx):
     check(y, h, tol * (1 + h.abs()) + 8 * U * h.abs())
 
 
+def test_layer_norm_row_lengths_in_any_order(ctx):
+    """One kernel serves several block sizes with different amounts of shared memory: what a
+    shorter row needs must not be all that a longer one gets afterwards."""
+    g = gen(12)
+    xs = {cols: randn(g, 5, cols) for cols in (16000, 8000, 4000, 2000, 1100)}
+    first = {}
+    for cols in (16000, 8000, 4000, 2000, 1100, 16000, 2000, 8000, 1100, 4000):
+        y, mean, rstd = ops.layer_norm(ctx, xs[cols])
+        dx, dw, db = ops.layer_norm_backward(ctx, y, xs[cols], mean, rstd)
+        got = first.setdefault(cols, (y, dx, dw))
+        assert all(torch.equal(p, q) for p, q in zip(got, (y, dx, dw)))
+
+
 def test_layer_norm_no_rows(ctx):
     dw, db = torch.full((16,), 3.0, device=DEV), torch.full((16,), 3.0, device=DEV)
     empty, stat = torch.empty(0, 16, device=DEV), torch.empty(0, device=DEV)
