@@ -641,7 +641,7 @@ int sb200_layer_norm_backward(sb200_ctx* ctx, void* dx, int64_t lddx, void* dwei
 
 /*
  * The orthogonalised update of `batch` matrices g [rows, cols] (gradients or their
- * momentum), as the Muon optimizer takes it in the place of the gradient itself:
+ * momentum), which an optimizer may take in the place of the gradient itself:
  *     X = g / (|g| + eps)  (Frobenius norm),  then `steps` times
  *     A = X X^T,  X = a X + (b A + c A A) X   (with X^T X on the right for a tall g),
  * out = X.  The usual coefficients 3.4445, -4.7750, 2.0315 and five steps bring the
@@ -649,8 +649,9 @@ int sb200_layer_norm_backward(sb200_ctx* ctx, void* dx, int64_t lddx, void* dwei
  * SB200_F32 and SB200_F16 are computed to about fp32 accuracy (operands in two fp16
  * parts, 22 bits); SB200_BF16 with operands of 11 bits, its own result having 8.
  * Coefficients that let a singular value s, or |b s^2 + c s^4| with or without a in
- * front, pass about 7 on the way are refused (SB200_ERR_UNSUPPORTED).  Limits (SB200_ERR_TOO_LARGE): sides
- * <= 2^20, batch <= 65535, steps <= 64.  The waits inside the kernels are bounded like those of the GEMM.
+ * front, pass about 7 on the way are refused (SB200_ERR_UNSUPPORTED).  Limits
+ * (SB200_ERR_TOO_LARGE): sides <= 2^20, batch <= 65535, steps <= 64.  The waits inside
+ * the kernels are bounded like those of the GEMM.
  */
 int64_t sb200_orthogonalize_workspace(int64_t rows, int64_t cols, int64_t batch, int type);
 int sb200_orthogonalize(sb200_ctx* ctx, void* out, int64_t ldo, int64_t stride_out,

@@ -386,12 +386,15 @@ ln_backward_kernel(T* dx, int64_t lddx, float* __restrict__ partial, const T* dy
         else request(r, 0);
         float2 h[EPT / 2], d[EPT / 2], a1 = both(0.0f), a2 = both(0.0f);
         if (!WARP || has) {
-            // (beyond the row dy is zero, and so is all that is added up)
+            // beyond the row dy is zero, and so is all that is added up: h must be finite there, and
+            // (0 - mean) rstd need not be where the row itself is (a constant one of large numbers)
             get_pairs<VEC, EPT, P, T>(h, px, stage);
             get_pairs<VEC, EPT, P, T>(d, py, stage);
 #pragma unroll
             for (int j = 0; j < EPT / 2; ++j) {
-                h[j] = mul2(add2(h[j], both(-mean)), both(rstd));
+                const int s0 = 2 * j / VEC, s1 = (2 * j + 1) / VEC;
+                const float2 by = make_float2(s0 * lanes + lane < nvec ? rstd : 0.0f, s1 * lanes + lane < nvec ? rstd : 0.0f);
+                h[j] = mul2(add2(h[j], both(-mean)), by);
                 dw2[j] = fma2(d[j], h[j], dw2[j]);
                 db2[j] = add2(db2[j], d[j]);
                 d[j] = mul2(d[j], wf[j]);                // from here on dy * weight

@@ -338,6 +338,24 @@ def test_layer_norm_constant_rows_and_bad_values(ctx):
     assert torch.equal(alone[0], y[1])
 
 
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("cols", [3, 8, 100, 1100, 4004])
+def test_layer_norm_backward_of_constant_rows_of_large_numbers(ctx, t, cols):
+    """h is 0 in such a row, but (0 - mean) * rstd, which lanes beyond the row could take for
+    theirs, is not finite: 2^120 * 316 > 2^128."""
+    g = gen(cols)
+    x = torch.full((5, cols), 2.0 ** 120, dtype=t, device=DEV)
+    dy, w = randn(g, 5, cols, dtype=t), randn(g, cols)
+    mean, rstd = torch.full((5,), 2.0 ** 120, device=DEV), torch.full((5,), 316.0, device=DEV)
+    dx, dw, _ = ops.layer_norm_backward(ctx, dy, x, mean, rstd, w)
+    gw = dy.cpu().double() * w.cpu().double()
+    m1 = gw.mean(-1, keepdim=True)
+    want = 316.0 * (gw - m1)
+    size = 316.0 * (gw.abs() * 6 * U + (depth(cols) + 10) * U * gw.abs().mean(-1, keepdim=True) + 6 * U * m1.abs()) + 2 * U * want.abs()
+    check(dx, want, size + half_step(t) * (want.abs() + size) * 1.001 + tiny(t))
+    assert (dw == 0).all()
+
+
 def test_layer_norm_large_offsets(ctx):
     """Rows far from zero: the variance comes from differences to the mean."""
     g = gen(2)
@@ -546,6 +564,56 @@ def test_other_streams_and_captured_graphs(ctx):
         graphs[k].replay()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(outs[k], want[k]))
+
+
+@pytest.mark.parametrize("rows,cols", [(300, 700), (2304, 2500)])
+def test_captured_products_and_long_sorts(ctx, rows, cols):
+    """The larger ways of the calls in a graph, replayed after their inputs have changed."""
+    g = gen(13)
+    m, ids, dout = gradient(g, rows, cols), token_ids(g, 20000, 3000, torch.int64).to(DEV), randn(g, 20000, 24)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o = ops.orthogonalize(ctx, m)
+        dt = ops.embedding_backward(ctx, torch.empty(3000, 24, device=DEV), dout, ids)
+    for _ in range(2):
+        m.copy_(gradient(g, rows, cols))
+        ids.copy_(ids.flip(0))
+        o.fill_(float("nan"))
+        dt.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(o, ops.orthogonalize(ctx, m))
+        assert torch.equal(dt, ops.embedding_backward(ctx, torch.empty(3000, 24, device=DEV), dout, ids))
+    ctx.check_device_status()
+
+
+def test_offsets_beyond_32_bits(ctx):
+    """Rows so far apart that the last ones start more than 2^32 elements in."""
+    g = gen(14)
+    rows, cols, pitch = 300, 200, 1 << 24
+    def far():
+        return torch.empty(rows * pitch, dtype=BF16, device=DEV).view(rows, pitch)[:, :cols]
+    a, b = far(), far()
+    small = randn(g, rows, cols, dtype=BF16)
+    a.copy_(small)
+    ids = torch.randint(0, rows, (500,), generator=g)
+    ids[:3] = torch.tensor([rows - 1, 0, rows - 1])
+    ids = ids.to(DEV)
+    e = ops.embedding(ctx, a, ids)
+    assert torch.equal(e, small[ids])
+    b.zero_()
+    ops.embedding(ctx, small, torch.arange(rows, device=DEV), out=b)
+    assert torch.equal(b, small)
+    ops.embedding_backward(ctx, b, e, ids)
+    assert torch.equal(b, ops.embedding_backward(ctx, torch.empty_like(small), e, ids))
+    y, mean, rstd = ops.layer_norm(ctx, small)
+    ops.layer_norm(ctx, a, out=b)
+    assert torch.equal(b, y)
+    dx, _, _ = ops.layer_norm_backward(ctx, small, small, mean, rstd)
+    ops.layer_norm_backward(ctx, a, a, mean, rstd, dx=b)
+    assert torch.equal(b, dx)
+    ops.orthogonalize(ctx, a, out=b)
+    assert torch.equal(b, ops.orthogonalize(ctx, small))
 
 
 # ------------------------------------------------------------ a run of them together
