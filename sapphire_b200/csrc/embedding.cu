@@ -711,7 +711,9 @@ extern "C" int sb200_embedding(sb200_ctx* ctx, void* out, int64_t ldo, const voi
     if (const int rc = check_types(table_type, type, index_bits)) return rc;
     if (n > MAX_TOKENS || vocab > MAX_VOCAB || cols > MAX_COLS) return SB200_ERR_TOO_LARGE;
     if (n == 0 || cols == 0) return SB200_OK;
-    if (!out || !ids || (vocab > 0 && !table) || !aligned_to(ids, index_bits / 8)) return SB200_ERR_INVALID_ARG;
+    if (!out || !ids || (vocab > 0 && !table) || !aligned_to(ids, index_bits / 8) || !aligned_to(out, type_bytes(type)) ||
+        !aligned_to(table, type_bytes(table_type)))
+        return SB200_ERR_INVALID_ARG;
     DeviceGuard dev(ctx->device);
     if (!dev.ok) return SB200_ERR_CUDA;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
@@ -759,7 +761,9 @@ extern "C" int sb200_embedding_backward(sb200_ctx* ctx, void* dtable, int64_t ld
     if (const int rc = check_types(table_type, type, index_bits)) return rc;
     if (n > MAX_TOKENS || vocab > MAX_VOCAB || cols > MAX_COLS) return SB200_ERR_TOO_LARGE;
     if (vocab == 0 || cols == 0 || (n == 0 && accumulate)) return SB200_OK;
-    if (!dtable || (n > 0 && (!dout || !ids || !aligned_to(ids, index_bits / 8)))) return SB200_ERR_INVALID_ARG;
+    if (!dtable || !aligned_to(dtable, type_bytes(table_type)) || !aligned_to(dout, type_bytes(type)) ||
+        (n > 0 && (!dout || !ids || !aligned_to(ids, index_bits / 8))))
+        return SB200_ERR_INVALID_ARG;
     const GradPlan g = plan_grad(ctx->sm_count, n, vocab, cols);
     if (!workspace || !aligned_to(workspace, 16) || workspace_bytes < g.total) return SB200_ERR_INVALID_ARG;
     DeviceGuard dev(ctx->device);

@@ -17,8 +17,10 @@
 // bf16 forward: 291 us).  In the backward pass every thread keeps the column sums of its
 // columns in registers over all the rows its block sees, writes one partial sum a block,
 // and a second kernel adds the partials in block order: no atomics, the same bits run to
-// run.  Rows that 16-byte accesses do not fit take 4-byte ones, odd rows of 16-bit
-// elements 2-byte ones.
+// run.  Rows that 16-byte accesses do not fit take 4-byte ones.  Odd rows of 16-bit elements
+// take 16-byte ones all the same where all arrays' rows start at the same distance from a
+// boundary: the grid makes steps of 8 rows, so that the distance is a thread's own and its
+// columns stay (16384 x 4095 bf16: forward 225 -> 128 us, backward 474 -> 169), else 2-byte ones.
 #include <initializer_list>
 #include <type_traits>
 #include <utility>
@@ -48,6 +50,33 @@ struct Pieces {
 
     Raw<T, VEC> next[ASYNC ? 1 : NV];
     unsigned char* base;
+
+    // The pieces of a row that starts `shift` elements behind a 16-byte boundary (SHIFT): piece v
+    // holds elements v VEC - shift and the following ones.  What lies before the row comes
+    // along in the first piece (clean() makes it zero), except where that is not of the array.
+    __device__ void request_shifted(const T* row, bool in, bool at_start, int stage, int lane, int lanes, int nvec, int cols, int shift)
+    {
+        if (!in) return;
+        if constexpr (BYTES == 16) {
+#pragma unroll 4
+            for (int s = 0; s < NV; ++s) {
+                const int v = s * lanes + lane;
+                if (v >= nvec) break;
+                const int at = v * VEC - shift, end = cols - at < VEC ? cols - at : VEC;
+                if (at < 0 && at_start) {
+                    T* to = reinterpret_cast<T*>(slot(stage, s));
+                    for (int i = -at; i < VEC; ++i) to[i] = i < end ? row[at + i] : from_f<T>(0.0f);
+                } else {
+                    ptx::cp_async_16(slot(stage, s), row + at, end * static_cast<int>(sizeof(T)));
+                }
+            }
+        }
+    }
+    __device__ void clean(int stage, int lane, int shift)
+    {
+        if (lane == 0)
+            for (int i = 0; i < shift; ++i) reinterpret_cast<T*>(slot(stage, 0))[i] = from_f<T>(0.0f);
+    }
 
     // pieces beyond the row are zero and stay so
     __device__ void init(unsigned char* smem, int lane, int lanes, int nvec)
@@ -105,6 +134,13 @@ __device__ __forceinline__ void load_weight(float (&f)[VEC], const W* w, int64_t
     }
 }
 
+// Elements from a 16-byte boundary to the start of row r.
+template <typename T>
+__device__ __forceinline__ int row_shift(const T* x, int64_t ldx, int64_t r)
+{
+    return static_cast<int>((reinterpret_cast<uintptr_t>(x) / sizeof(T) + static_cast<uintptr_t>(r * ldx)) % (16 / sizeof(T)));
+}
+
 __device__ __forceinline__ float lanes_sum(float v, int lanes)
 {
     for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -132,8 +168,9 @@ __device__ __forceinline__ void get_pairs(float2 (&f)[E / 2], const P& pieces, i
 }
 
 // This thread's weights, in the same order; `none` where there are none.
-template <int VEC, int E, typename W>
-__device__ __forceinline__ void get_weights(float2 (&f)[E / 2], const W* w, float none, int lane, int lanes, int nvec)
+template <int VEC, int E, bool SHIFT, typename W>
+__device__ __forceinline__ void get_weights(float2 (&f)[E / 2], const W* w, float none, int lane, int lanes, int nvec, int cols,
+                                            int shift)
 {
     float* one = reinterpret_cast<float*>(f);
 #pragma unroll
@@ -142,20 +179,65 @@ __device__ __forceinline__ void get_weights(float2 (&f)[E / 2], const W* w, floa
         const int v = s * lanes + lane;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) a[i] = none;
-        if (w && v < nvec) load_f<false>(a, w + static_cast<int64_t>(v) * VEC);
+        if constexpr (SHIFT) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                const int j = v * VEC - shift + i;
+                if (w && j >= 0 && j < cols) a[i] = to_f(w[j]);
+            }
+        } else {
+            if (w && v < nvec) load_f<false>(a, w + static_cast<int64_t>(v) * VEC);
+        }
 #pragma unroll
         for (int i = 0; i < VEC; ++i) one[s * VEC + i] = a[i];
     }
 }
 
-// The pairs back into pieces of a row.
-template <int VEC, int E, typename T>
-__device__ __forceinline__ void put_pairs(T* row, const float2 (&f)[E / 2], int lane, int lanes, int nvec)
+// Which of this thread's elements are in the row.
+template <int VEC, int E>
+__device__ __forceinline__ uint32_t valid_elements(int lane, int lanes, int cols, int shift)
 {
-    row += static_cast<int64_t>(lane) * VEC;
+    uint32_t bits = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int j = (e / VEC * lanes + lane) * VEC - shift + e % VEC;
+        if (j >= 0 && j < cols) bits |= 1u << e;
+    }
+    return bits;
+}
+
+// Elements that are not in the row become x.
+template <int E>
+__device__ __forceinline__ void fill_invalid(float2 (&f)[E / 2], uint32_t valid, float x)
+{
+    if (valid == (E == 32 ? 0xffffffffu : (1u << (E & 31)) - 1u)) return;
+#pragma unroll
+    for (int j = 0; j < E / 2; ++j) {
+        if (!((valid >> (2 * j)) & 1u)) f[j].x = x;
+        if (!((valid >> (2 * j + 1)) & 1u)) f[j].y = x;
+    }
+}
+
+// The pairs back into pieces of a row.
+template <int VEC, int E, bool SHIFT, typename T>
+__device__ __forceinline__ void put_pairs(T* row, const float2 (&f)[E / 2], int lane, int lanes, int nvec, uint32_t valid, int shift)
+{
+    row += static_cast<int64_t>(lane) * VEC - (SHIFT ? shift : 0);
 #pragma unroll
     for (int s = 0; s < E / VEC; ++s) {
-        if (s * lanes + lane < nvec) {
+        if constexpr (SHIFT) {
+            const uint32_t bits = (valid >> (s * VEC)) & ((1u << VEC) - 1u);
+            Raw<T, VEC> r;
+#pragma unroll
+            for (int i = 0; i < VEC; i += 2) set_pair(r.e + i, f[(s * VEC + i) / 2]);
+            if (bits == (1u << VEC) - 1u) {
+                store_raw<true>(row + s * lanes * VEC, r);
+            } else if (bits) {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i)
+                    if ((bits >> i) & 1u) row[s * lanes * VEC + i] = r.e[i];
+            }
+        } else if (s * lanes + lane < nvec) {
             Raw<T, VEC> r;
             if constexpr (VEC == 1) {
                 r.e[0] = from_f<T>(s & 1 ? f[s / 2].y : f[s / 2].x);
@@ -172,8 +254,10 @@ __device__ __forceinline__ void put_pairs(T* row, const float2 (&f)[E / 2], int 
 // row costs a thread beside its elements (two sums over the warp, one over the block) is as
 // much as 16 elements, so rows of more than a warp get 32; pairs of elements share an
 // instruction.  What bounds it is the instructions, not the memory, when rows are of 16 bits.
-template <typename T, typename W, int VEC, int E, bool WARP>
-__global__ void __maxnreg__(E == 32 || VEC == 1 ? 128 : 80)
+// SHIFT: rows that start anywhere, the same distance behind a 16-byte boundary in x and y.
+// The distance is that of every row a thread sees: the grid makes steps of whole periods.
+template <typename T, typename W, int VEC, int E, bool WARP, bool SHIFT>
+__global__ void __maxnreg__(E == 32 || VEC == 1 || SHIFT ? 128 : 80)
 ln_forward_kernel(T* y, int64_t ldy, float* __restrict__ mean_out, float* __restrict__ rstd_out, const T* x,
                   int64_t ldx, const W* __restrict__ w, const W* __restrict__ b, int64_t rows, int cols, float eps,
                   int lanes)
@@ -187,12 +271,14 @@ ln_forward_kernel(T* y, int64_t ldy, float* __restrict__ mean_out, float* __rest
     const int lane = WARP ? (threadIdx.x & (lanes - 1)) : threadIdx.x;
     const int64_t group = WARP ? (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / lanes : blockIdx.x;
     const int64_t groups = WARP ? static_cast<int64_t>(gridDim.x) * blockDim.x / lanes : gridDim.x;
-    const int nvec = cols / VEC;
+    const int shift = SHIFT ? row_shift(x, ldx, group) : 0, nvec = SHIFT ? (cols + shift + VEC - 1) / VEC : cols / VEC;
+    const uint32_t valid = SHIFT ? valid_elements<VEC, E>(lane, lanes, cols, shift) : 0;
     const float inv_n = 1.0f / static_cast<float>(cols);
     // elements in this thread's warp (or group)
-    int mine = 0;
+    int mine = SHIFT ? __popc(valid) : 0;
 #pragma unroll
-    for (int s = 0; s < NV; ++s) mine += s * lanes + lane < nvec ? VEC : 0;
+    for (int s = 0; s < NV; ++s)
+        if (!SHIFT) mine += s * lanes + lane < nvec ? VEC : 0;
     const float warp_n = lanes_sum(static_cast<float>(mine), WARP ? lanes : 32);
     const float warp_inv = warp_n > 0.0f ? 1.0f / warp_n : 0.0f;
     if (!WARP && (threadIdx.x & 31) == 0) count[threadIdx.x >> 5] = make_float2(warp_n, warp_inv);   // (read behind a barrier)
@@ -204,26 +290,30 @@ ln_forward_kernel(T* y, int64_t ldy, float* __restrict__ mean_out, float* __rest
     // every lane of a warp makes the same number of trips: the shuffles name all of them
     const int64_t first = WARP ? group - (threadIdx.x & 31) / lanes : group;
     const int64_t off = group - first;
+    auto request = [&](int64_t r, int stage) {
+        if constexpr (SHIFT) px.request_shifted(x + r * ldx, r < rows, r * ldx < shift, stage, lane, lanes, nvec, cols, shift);
+        else px.request(x + r * ldx, r < rows, stage, lane, lanes, nvec);
+    };
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) {
         const int64_t r = first + k * groups + off;
-        px.request(x + r * ldx, r < rows, k, lane, lanes, nvec);
+        request(r, k);
         if (P::ASYNC) ptx::cp_async_commit();
     }
     float2 wf[E / 2], bf[E / 2];
-    get_weights<VEC, E>(wf, w, 1.0f, lane, lanes, nvec);
-    get_weights<VEC, E>(bf, b, 0.0f, lane, lanes, nvec);
+    get_weights<VEC, E, SHIFT>(wf, w, 1.0f, lane, lanes, nvec, cols, shift);
+    get_weights<VEC, E, SHIFT>(bf, b, 0.0f, lane, lanes, nvec, cols, shift);
     int stage = 0, flip = 0;
     for (int64_t r0 = first; r0 < rows; r0 += groups) {
         const int64_t r = r0 + off;
         const bool has = r < rows;
         if constexpr (P::ASYNC) ptx::cp_async_wait<AHEAD - 1>();
-        else px.request(x + r * ldx, has, 0, lane, lanes, nvec);
+        else request(r, 0);
+        if constexpr (SHIFT) px.clean(stage, lane, shift);
         float2 f[E / 2];
         get_pairs<VEC, E, P, T>(f, px, stage);
         if constexpr (P::ASYNC) {
-            const int64_t rn = r + AHEAD * groups;
-            px.request(x + rn * ldx, rn < rows, (stage + AHEAD) % P::STAGES, lane, lanes, nvec);
+            request(r + AHEAD * groups, (stage + AHEAD) % P::STAGES);
             ptx::cp_async_commit();
             stage = stage + 1 == P::STAGES ? 0 : stage + 1;
         }
@@ -233,9 +323,10 @@ ln_forward_kernel(T* y, int64_t ldy, float* __restrict__ mean_out, float* __rest
         const float sum = lanes_sum(s2.x + s2.y, WARP ? lanes : 32);
         const float near = sum * warp_inv;               // the mean over this warp's elements
         float2 q2 = both(0.0f);
+        if constexpr (SHIFT) fill_invalid<E>(f, valid, near);    // beyond the row: no difference
 #pragma unroll
         for (int s = 0; s < NV; s += VEC == 1 ? 2 : 1) {
-            const bool in = s * lanes + lane < nvec;
+            const bool in = SHIFT || s * lanes + lane < nvec;
             if constexpr (VEC == 1) {
                 float2 g = f[s / 2];                     // beyond the row: no difference
                 if (!in) g.x = near;
@@ -273,7 +364,7 @@ ln_forward_kernel(T* y, int64_t ldy, float* __restrict__ mean_out, float* __rest
         }
 #pragma unroll
         for (int j = 0; j < E / 2; ++j) f[j] = fma2(mul2(add2(f[j], both(-mean)), both(rstd)), wf[j], bf[j]);
-        put_pairs<VEC, E>(y + r * ldy, f, lane, lanes, nvec);
+        put_pairs<VEC, E, SHIFT>(y + r * ldy, f, lane, lanes, nvec, valid, shift);
     }
 }
 
@@ -342,7 +433,7 @@ ln_forward_long_kernel(T* y, int64_t ldy, float* __restrict__ mean_out, float* _
 
 // partial: [2][gridDim.x][cols] column sums of this block's rows (dweight, then dbias), or null.
 // Dynamic shared memory: the pieces of x and dy, and later (WARP, partial != null) 2 * cols floats.
-template <typename T, typename W, int VEC, bool WARP>
+template <typename T, typename W, int VEC, bool WARP, bool SHIFT>
 __global__ void __launch_bounds__(MAX_THREADS)
 ln_backward_kernel(T* dx, int64_t lddx, float* __restrict__ partial, const T* dy, int64_t lddy, const T* x,
                    int64_t ldx, const W* __restrict__ w, const float* __restrict__ mean_in,
@@ -355,7 +446,8 @@ ln_backward_kernel(T* dx, int64_t lddx, float* __restrict__ partial, const T* dy
     const int lane = WARP ? (threadIdx.x & (lanes - 1)) : threadIdx.x;
     const int64_t group = WARP ? (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / lanes : blockIdx.x;
     const int64_t groups = WARP ? static_cast<int64_t>(gridDim.x) * blockDim.x / lanes : gridDim.x;
-    const int nvec = cols / VEC;
+    const int shift = SHIFT ? row_shift(x, ldx, group) : 0, nvec = SHIFT ? (cols + shift + VEC - 1) / VEC : cols / VEC;
+    const uint32_t valid = valid_elements<VEC, EPT>(lane, lanes, cols, shift);
     const float inv_n = 1.0f / static_cast<float>(cols);
     P px, py;
     px.init(smem, lane, lanes, nvec);
@@ -365,8 +457,13 @@ ln_backward_kernel(T* dx, int64_t lddx, float* __restrict__ partial, const T* dy
     const int64_t first = WARP ? group - (threadIdx.x & 31) / lanes : group;
     const int64_t off = group - first;
     auto request = [&](int64_t r, int stage) {
-        px.request(x + r * ldx, r < rows, stage, lane, lanes, nvec);
-        py.request(dy + r * lddy, r < rows, stage, lane, lanes, nvec);
+        if constexpr (SHIFT) {
+            px.request_shifted(x + r * ldx, r < rows, r * ldx < shift, stage, lane, lanes, nvec, cols, shift);
+            py.request_shifted(dy + r * lddy, r < rows, r * lddy < shift, stage, lane, lanes, nvec, cols, shift);
+        } else {
+            px.request(x + r * ldx, r < rows, stage, lane, lanes, nvec);
+            py.request(dy + r * lddy, r < rows, stage, lane, lanes, nvec);
+        }
         if (P::ASYNC) ptx::cp_async_commit();
     };
 #pragma unroll
@@ -374,7 +471,7 @@ ln_backward_kernel(T* dx, int64_t lddx, float* __restrict__ partial, const T* dy
     float2 dw2[EPT / 2], db2[EPT / 2], wf[EPT / 2];
 #pragma unroll
     for (int j = 0; j < EPT / 2; ++j) dw2[j] = db2[j] = both(0.0f);
-    get_weights<VEC, EPT>(wf, w, 1.0f, lane, lanes, nvec);
+    get_weights<VEC, EPT, SHIFT>(wf, w, 1.0f, lane, lanes, nvec, cols, shift);
     float mean_next = first + off < rows ? mean_in[first + off] : 0.0f;
     float rstd_next = first + off < rows ? rstd_in[first + off] : 0.0f;
     int stage = 0, flip = 0;
@@ -384,17 +481,20 @@ ln_backward_kernel(T* dx, int64_t lddx, float* __restrict__ partial, const T* dy
         const float mean = mean_next, rstd = rstd_next;
         if constexpr (P::ASYNC) ptx::cp_async_wait<AHEAD - 1>();
         else request(r, 0);
+        if constexpr (SHIFT) {
+            px.clean(stage, lane, shift);
+            py.clean(stage, lane, shift);
+        }
         float2 h[EPT / 2], d[EPT / 2], a1 = both(0.0f), a2 = both(0.0f);
         if (!WARP || has) {
-            // beyond the row dy is zero, and so is all that is added up: h must be finite there, and
-            // (0 - mean) rstd need not be where the row itself is (a constant one of large numbers)
             get_pairs<VEC, EPT, P, T>(h, px, stage);
             get_pairs<VEC, EPT, P, T>(d, py, stage);
+            // beyond the row dy is zero, and so is all that is added up: h must be finite there, and
+            // (0 - mean) rstd need not be where the row itself is (a constant one of large numbers)
+            fill_invalid<EPT>(h, valid, mean);
 #pragma unroll
             for (int j = 0; j < EPT / 2; ++j) {
-                const int s0 = 2 * j / VEC, s1 = (2 * j + 1) / VEC;
-                const float2 by = make_float2(s0 * lanes + lane < nvec ? rstd : 0.0f, s1 * lanes + lane < nvec ? rstd : 0.0f);
-                h[j] = mul2(add2(h[j], both(-mean)), by);
+                h[j] = mul2(add2(h[j], both(-mean)), both(rstd));
                 dw2[j] = fma2(d[j], h[j], dw2[j]);
                 db2[j] = add2(db2[j], d[j]);
                 d[j] = mul2(d[j], wf[j]);                // from here on dy * weight
@@ -431,8 +531,15 @@ ln_backward_kernel(T* dx, int64_t lddx, float* __restrict__ partial, const T* dy
 #pragma unroll
                 for (int s = 0; s < NV; ++s) {
                     if (s * lanes + lane >= nvec) continue;
+                    const T* from = dr + static_cast<int64_t>(s * lanes + lane) * VEC - shift;
+                    const uint32_t bits = (valid >> (s * VEC)) & ((1u << VEC) - 1u);
                     float o[VEC];
-                    load_f<true>(o, dr + static_cast<int64_t>(s * lanes + lane) * VEC);
+                    if (!SHIFT || bits == (1u << VEC) - 1u) {
+                        load_f<true>(o, from);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i) o[i] = (bits >> i) & 1u ? to_f(from[i]) : 0.0f;
+                    }
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) {
                         float2& t = d[(s * VEC + i) / 2];
@@ -440,7 +547,7 @@ ln_backward_kernel(T* dx, int64_t lddx, float* __restrict__ partial, const T* dy
                     }
                 }
             }
-            put_pairs<VEC, EPT>(dr, d, lane, lanes, nvec);
+            put_pairs<VEC, EPT, SHIFT>(dr, d, lane, lanes, nvec, valid, shift);
         }
     }
     if (!partial) return;
@@ -455,8 +562,9 @@ ln_backward_kernel(T* dx, int64_t lddx, float* __restrict__ partial, const T* dy
             if (v >= nvec) continue;
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-                pw[v * VEC + i] = dw[s * VEC + i];
-                pb[v * VEC + i] = db[s * VEC + i];
+                if (SHIFT && !((valid >> (s * VEC + i)) & 1u)) continue;
+                pw[v * VEC - shift + i] = dw[s * VEC + i];
+                pb[v * VEC - shift + i] = db[s * VEC + i];
             }
         }
         return;
@@ -475,8 +583,9 @@ ln_backward_kernel(T* dx, int64_t lddx, float* __restrict__ partial, const T* dy
             if (v >= nvec) continue;
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-                cols_sum[v * VEC + i] += dw[s * VEC + i];
-                cols_sum[cols + v * VEC + i] += db[s * VEC + i];
+                if (SHIFT && !((valid >> (s * VEC + i)) & 1u)) continue;
+                cols_sum[v * VEC - shift + i] += dw[s * VEC + i];
+                cols_sum[cols + v * VEC - shift + i] += db[s * VEC + i];
             }
         }
     }
@@ -663,6 +772,24 @@ int access_width(int64_t cols, const void* w, const void* b, std::initializer_li
 template <int N>
 using Int = std::integral_constant<int, N>;
 
+// Whether the rows of all arrays start at the same distance from a 16-byte boundary, row by row.
+template <typename T>
+bool same_shift(std::initializer_list<std::pair<const void*, int64_t>> arrays)
+{
+    const auto& a = *arrays.begin();
+    for (const auto& b : arrays)
+        if ((reinterpret_cast<uintptr_t>(a.first) - reinterpret_cast<uintptr_t>(b.first)) % 16 != 0 ||
+            (a.second - b.second) % static_cast<int64_t>(16 / sizeof(T)) != 0)
+            return false;
+    return true;
+}
+
+// Elements of the pieces that a row may touch, whatever its shift.
+int64_t shifted_span(int64_t cols, int vec) { return (cols + 2 * vec - 2) / vec * vec; }
+
+// Blocks for rows with a shift: every thread's steps are whole periods of it, at most 8 rows.
+int64_t whole_periods(int64_t blocks, int64_t wanted) { return blocks < wanted ? blocks / 8 * 8 : wanted; }
+
 // f(Int<vec>{}) for an access width of access_width()
 template <typename T, typename F>
 int with_width(int vec, F f)
@@ -717,7 +844,9 @@ extern "C" int sb200_layer_norm(sb200_ctx* ctx, void* y, int64_t ldy, float* mea
     if (!ctx || rows < 0 || cols < 1 || ldx < cols || ldy < cols || !(eps >= 0.0f)) return SB200_ERR_INVALID_ARG;
     if (const int rc = check_types(type, weight_type)) return rc;
     if (rows == 0) return SB200_OK;
-    if (!x || !y) return SB200_ERR_INVALID_ARG;
+    if (!x || !y || !aligned_to(x, type_bytes(type)) || !aligned_to(y, type_bytes(type)) || !aligned_to(weight, type_bytes(weight_type)) ||
+        !aligned_to(bias, type_bytes(weight_type)) || !aligned_to(mean, 4) || !aligned_to(rstd, 4))
+        return SB200_ERR_INVALID_ARG;
     DeviceGuard dev(ctx->device);
     if (!dev.ok) return SB200_ERR_CUDA;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
@@ -725,6 +854,26 @@ extern "C" int sb200_layer_norm(sb200_ctx* ctx, void* y, int64_t ldy, float* mea
         using T = decltype(t);
         using W = decltype(wt);
         const int width = access_width<T, W>(cols, weight, bias, {{x, ldx}, {y, ldy}});
+        if constexpr (sizeof(T) == 2) {
+            // odd rows (4-byte accesses, where they fit, are better: 16384 x 4094 bf16 71 us, 137 in this way)
+            constexpr int FULL = 16 / static_cast<int>(sizeof(T));
+            const int64_t span = shifted_span(cols, FULL);
+            if (width == 1 && same_shift<T>({{x, ldx}, {y, ldy}}) && span <= 32 * MAX_THREADS) {
+                auto launch = [&](auto kern, auto e) -> int {
+                    const Shape s = shape_of(rows, span, FULL, decltype(e)::value);
+                    const int smem = s.block * Pieces<T, FULL, decltype(e)::value>::SMEM;
+                    const int64_t most = resident_blocks(ctx, kern, s.block, smem);
+                    if (most < 8) return SB200_ERR_CUDA;
+                    return launch_after(ctx, kern.run, static_cast<unsigned>(whole_periods(most, s.blocks)), s.block, smem, stream, static_cast<T*>(y),
+                                        ldy, mean, rstd, static_cast<const T*>(x), ldx, static_cast<const W*>(weight), static_cast<const W*>(bias),
+                                        rows, static_cast<int>(cols), eps, s.lanes);
+                };
+                // 16 elements a thread as far as they go (the masks of 32 do not fit the registers: 4095 columns 139 us, 128 with 16)
+                if (span <= 16 * 32) return launch(Kernel<ln_forward_kernel<T, W, FULL, 16, true, true>>{}, Int<16>{});
+                if (span <= 16 * MAX_THREADS) return launch(Kernel<ln_forward_kernel<T, W, FULL, 16, false, true>>{}, Int<16>{});
+                return launch(Kernel<ln_forward_kernel<T, W, FULL, 32, false, true>>{}, Int<32>{});
+            }
+        }
         return with_width<T>(width, [&](auto v) -> int {
             constexpr int VEC = decltype(v)::value;
             // 32 elements a thread for rows of more than 512 columns, so that a warp holds 1024;
@@ -744,13 +893,13 @@ extern "C" int sb200_layer_norm(sb200_ctx* ctx, void* y, int64_t ldy, float* mea
             const int n = static_cast<int>(cols);
             if (many) {
                 const int smem = s.block * Pieces<T, VEC, MANY>::SMEM;
-                if (s.lanes <= 32) return launch(Kernel<ln_forward_kernel<T, W, VEC, MANY, true>>{}, smem, n, eps, s.lanes);
-                return launch(Kernel<ln_forward_kernel<T, W, VEC, MANY, false>>{}, smem, n, eps, s.lanes);
+                if (s.lanes <= 32) return launch(Kernel<ln_forward_kernel<T, W, VEC, MANY, true, false>>{}, smem, n, eps, s.lanes);
+                return launch(Kernel<ln_forward_kernel<T, W, VEC, MANY, false, false>>{}, smem, n, eps, s.lanes);
             }
             const int smem = s.block * Pieces<T, VEC, 16>::SMEM;
-            if (s.lanes <= 32) return launch(Kernel<ln_forward_kernel<T, W, VEC, 16, true>>{}, smem, n, eps, s.lanes);
+            if (s.lanes <= 32) return launch(Kernel<ln_forward_kernel<T, W, VEC, 16, true, false>>{}, smem, n, eps, s.lanes);
             if constexpr (WIDE) return SB200_ERR_INVALID_ARG;    // (not reached: such rows have 32 elements a thread)
-            else return launch(Kernel<ln_forward_kernel<T, W, VEC, 16, false>>{}, smem, n, eps, s.lanes);
+            else return launch(Kernel<ln_forward_kernel<T, W, VEC, 16, false, false>>{}, smem, n, eps, s.lanes);
         });
     });
 }
@@ -771,6 +920,11 @@ extern "C" int sb200_layer_norm_backward(sb200_ctx* ctx, void* dx, int64_t lddx,
     if (!ctx || rows < 0 || cols < 1 || ldx < cols || lddy < cols || (dx && lddx < cols)) return SB200_ERR_INVALID_ARG;
     if (const int rc = check_types(type, weight_type)) return rc;
     if (rows > 0 && (!x || !dy || !mean || !rstd)) return SB200_ERR_INVALID_ARG;
+    for (const void* at : {static_cast<const void*>(x), dy, static_cast<const void*>(dx)})
+        if (!aligned_to(at, type_bytes(type))) return SB200_ERR_INVALID_ARG;
+    for (const void* at : {weight, static_cast<const void*>(dweight), static_cast<const void*>(dbias)})
+        if (!aligned_to(at, type_bytes(weight_type))) return SB200_ERR_INVALID_ARG;
+    if (!aligned_to(mean, 4) || !aligned_to(rstd, 4)) return SB200_ERR_INVALID_ARG;
     const bool sums = dweight || dbias;
     if (sums && (!workspace || !aligned_to(workspace, 16) ||
                  workspace_bytes < sb200_layer_norm_backward_workspace(ctx, rows, cols)))
@@ -792,42 +946,57 @@ extern "C" int sb200_layer_norm_backward(sb200_ctx* ctx, void* dx, int64_t lddx,
             const int width = dx ? access_width<T, W>(cols, weight, nullptr, {{x, ldx}, {dy, lddy}, {dx, lddx}})
                                  : access_width<T, W>(cols, weight, nullptr, {{x, ldx}, {dy, lddy}});
             const int64_t bound = backward_parts(ctx->sm_count, rows, cols);
-            const int rc = with_width<T>(width, [&](auto v) -> int {
+            constexpr int FULL = 16 / static_cast<int>(sizeof(T));
+            const int64_t span = shifted_span(cols, FULL);
+            const std::pair<const void*, int64_t> out{dx ? dx : x, dx ? lddx : ldx};
+            const bool shifted = width == 1 && span <= REGISTER_COLS && same_shift<T>({{x, ldx}, {dy, lddy}, out});
+            const int n = static_cast<int>(cols);
+            auto launch = [&](auto kern, auto v, auto shift) -> int {
                 constexpr int VEC = decltype(v)::value;
-                const Shape s = shape_of(rows, cols, VEC, EPT);
-                if (cols > REGISTER_COLS) {
-                    // the column sums first: dx may overwrite dy
-                    if (sums) {
-                        parts = static_cast<int>(bound);
-                        const dim3 grid(static_cast<unsigned>((cols + 255) / 256), static_cast<unsigned>(parts));
-                        ln_backward_long_cols_kernel<T><<<grid, 256, 0, stream>>>(partial, yp, lddy, xp, ldx, mean, rstd, rows, cols);
-                        ctx->launches += 1;
-                    }
-                    if (dx) {
-                        Kernel<ln_backward_long_kernel<T, W, VEC>> kern;
-                        const int64_t most = resident_blocks(ctx, kern, s.block, 0);
-                        if (most < 1) return SB200_ERR_CUDA;
-                        kern.run<<<static_cast<unsigned>(s.blocks < most ? s.blocks : most), s.block, 0, stream>>>(
-                            dxp, lddx, yp, lddy, xp, ldx, wp, mean, rstd, rows, cols, accumulate_dx);
-                        ctx->launches += 1;
-                    }
-                    return SB200_OK;
+                constexpr bool SHIFT = decltype(shift)::value;
+                const Shape s = shape_of(rows, SHIFT ? span : cols, VEC, EPT);
+                int smem = 2 * s.block * Pieces<T, VEC, EPT>::SMEM;
+                if (s.lanes <= 32 && smem < 2 * 32 * EPT * 4) smem = 2 * 32 * EPT * 4;      // column sums of such rows
+                const int64_t most = resident_blocks(ctx, kern, s.block, smem);
+                if (most < 8) return SB200_ERR_CUDA;
+                const int64_t grid = most < bound ? most : bound;
+                parts = static_cast<int>(SHIFT ? whole_periods(grid, s.blocks) : s.blocks < grid ? s.blocks : grid);
+                return launch_after(ctx, kern.run, static_cast<unsigned>(parts), s.block, smem, stream, dxp, lddx, partial, yp, lddy, xp, ldx, wp, mean, rstd,
+                                    rows, n, accumulate_dx, s.lanes);
+            };
+            auto any = [&]() -> int {
+                if constexpr (sizeof(T) == 2) {
+                    if (shifted)
+                        return shape_of(rows, span, FULL, EPT).lanes <= 32
+                                   ? launch(Kernel<ln_backward_kernel<T, W, FULL, true, true>>{}, Int<FULL>{}, std::true_type{})
+                                   : launch(Kernel<ln_backward_kernel<T, W, FULL, false, true>>{}, Int<FULL>{}, std::true_type{});
                 }
-                const int n = static_cast<int>(cols);
-                auto launch = [&](auto kern) -> int {
-                    int smem = 2 * s.block * Pieces<T, VEC, EPT>::SMEM;
-                    if (s.lanes <= 32 && smem < 2 * 32 * EPT * 4) smem = 2 * 32 * EPT * 4;      // column sums of such rows
-                    const int64_t most = resident_blocks(ctx, kern, s.block, smem);
-                    if (most < 1) return SB200_ERR_CUDA;
-                    int64_t grid = s.blocks < most ? s.blocks : most;
-                    if (grid > bound) grid = bound;
-                    parts = static_cast<int>(grid);
-                    return launch_after(ctx, kern.run, static_cast<unsigned>(grid), s.block, smem, stream, dxp, lddx, partial, yp, lddy, xp, ldx, wp, mean, rstd,
-                                        rows, n, accumulate_dx, s.lanes);
-                };
-                return s.lanes <= 32 ? launch(Kernel<ln_backward_kernel<T, W, VEC, true>>{}) : launch(Kernel<ln_backward_kernel<T, W, VEC, false>>{});
-            });
-            if (rc) return rc;
+                return with_width<T>(width, [&](auto v) -> int {
+                    constexpr int VEC = decltype(v)::value;
+                    const Shape s = shape_of(rows, cols, VEC, EPT);
+                    if (cols > REGISTER_COLS) {
+                        // the column sums first: dx may overwrite dy
+                        if (sums) {
+                            parts = static_cast<int>(bound);
+                            const dim3 grid(static_cast<unsigned>((cols + 255) / 256), static_cast<unsigned>(parts));
+                            ln_backward_long_cols_kernel<T><<<grid, 256, 0, stream>>>(partial, yp, lddy, xp, ldx, mean, rstd, rows, cols);
+                            ctx->launches += 1;
+                        }
+                        if (dx) {
+                            Kernel<ln_backward_long_kernel<T, W, VEC>> kern;
+                            const int64_t most = resident_blocks(ctx, kern, s.block, 0);
+                            if (most < 1) return SB200_ERR_CUDA;
+                            kern.run<<<static_cast<unsigned>(s.blocks < most ? s.blocks : most), s.block, 0, stream>>>(
+                                dxp, lddx, yp, lddy, xp, ldx, wp, mean, rstd, rows, cols, accumulate_dx);
+                            ctx->launches += 1;
+                        }
+                        return SB200_OK;
+                    }
+                    return s.lanes <= 32 ? launch(Kernel<ln_backward_kernel<T, W, VEC, true, false>>{}, v, std::false_type{})
+                                         : launch(Kernel<ln_backward_kernel<T, W, VEC, false, false>>{}, v, std::false_type{});
+                });
+            };
+            if (const int rc = any()) return rc;
         }
         if (sums) {
             const dim3 grid(static_cast<unsigned>((cols + 31) / 32), 2);

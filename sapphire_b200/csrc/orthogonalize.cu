@@ -940,7 +940,7 @@ extern "C" int sb200_orthogonalize(sb200_ctx* ctx, void* out, int64_t ldo, int64
     if (rows > MAX_SIDE || cols > MAX_SIDE || batch > 65535 || steps > MAX_STEPS) return SB200_ERR_TOO_LARGE;
     if (!bounded(a, b, c, steps)) return SB200_ERR_UNSUPPORTED;
     if (rows == 0 || cols == 0 || batch == 0) return SB200_OK;
-    if (!out || !g) return SB200_ERR_INVALID_ARG;
+    if (!out || !g || !aligned_to(out, type_bytes(type)) || !aligned_to(g, type_bytes(type))) return SB200_ERR_INVALID_ARG;
     const OrthPlan q = plan_orth(rows, cols, batch, type);
     if (!workspace || workspace_bytes < q.total) return SB200_ERR_INVALID_ARG;
     DeviceGuard dev(ctx->device);

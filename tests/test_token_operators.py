@@ -58,6 +58,18 @@ REFUSED = [
     (embedding, dict(table=None), L.ERR_INVALID_ARG),
     (embedding, dict(ids=None), L.ERR_INVALID_ARG),
     (embedding, dict(ids=P + 4), L.ERR_INVALID_ARG),
+    (embedding, dict(out=P + 2), L.ERR_INVALID_ARG),
+    (embedding, dict(table=P + 1, tt=L.BF16, ta=L.BF16), L.ERR_INVALID_ARG),
+    (embedding_backward, dict(dtable=P + 2), L.ERR_INVALID_ARG),
+    (embedding_backward, dict(dout=P + 1, ta=L.F16), L.ERR_INVALID_ARG),
+    (layer_norm, dict(x=P + 2), L.ERR_INVALID_ARG),
+    (layer_norm, dict(y=P + 1, t=L.BF16), L.ERR_INVALID_ARG),
+    (layer_norm_backward, dict(dy=P + 2), L.ERR_INVALID_ARG),
+    (layer_norm_backward, dict(dx=P + 1, t=L.F16), L.ERR_INVALID_ARG),
+    (layer_norm_backward, dict(dw=P + 2), L.ERR_INVALID_ARG),
+    (layer_norm_backward, dict(mean=P + 2), L.ERR_INVALID_ARG),
+    (orthogonalize, dict(g=P + 2), L.ERR_INVALID_ARG),
+    (orthogonalize, dict(out=P + 1, t=L.BF16), L.ERR_INVALID_ARG),
     (embedding, dict(n=(1 << 30) + 1), L.ERR_TOO_LARGE),
     (embedding, dict(vocab=(1 << 31) - 1), L.ERR_TOO_LARGE),
     (embedding, dict(cols=(1 << 20) + 1, ldo=1 << 21, ldt=1 << 21), L.ERR_TOO_LARGE),

@@ -311,6 +311,67 @@ def test_layer_norm_strides_and_in_place(ctx, t, cols, pitch, offset):
           2 * half_step(t) * dx.double().abs() * 1.01 + 4 * U * dx.double().abs() + tiny(t))
 
 
+@pytest.mark.parametrize("t,wt", LN_TYPES)
+@pytest.mark.parametrize("rows,cols,pitch,offset", [(3, 1, 1, 5), (40, 1, 1, 0), (700, 3, 3, 1), (100, 5, 8, 3), (40, 17, 17, 7), (9000, 63, 63, 0),
+                                                    (20, 505, 505, 2), (20, 506, 508, 1), (5000, 1001, 1001, 0), (30, 1024, 1027, 5),
+                                                    (1000, 4003, 4003, 0), (9, 8185, 8185, 3), (9, 8187, 8190, 1), (5, 16376, 16379, 1)])
+def test_layer_norm_rows_that_start_anywhere(ctx, t, wt, rows, cols, pitch, offset):
+    """Rows at the same odd distances in all arrays give what aligned rows give, up to the order
+    of the sums, in place too, and nothing around them is read into a sum or written."""
+    g = gen(rows + cols)
+    x = randn(g, rows, cols, dtype=t, pitch=pitch, offset=offset)
+    dy = randn(g, rows, cols, dtype=t, pitch=pitch, offset=offset)
+    w, b = randn(g, cols, dtype=wt), randn(g, cols, dtype=wt)
+
+    def like():
+        flat = torch.full((rows * pitch + offset + 16,), 7.0, dtype=t, device=DEV)
+        return flat, flat[offset:offset + rows * pitch].view(rows, pitch)[:, :cols]
+
+    eps = 1e-3
+    flat, y = like()
+    _, mean, rstd = ops.layer_norm(ctx, x, w, b, eps=eps, out=y)
+    xr, m, r, h, wr, br = ln_reference(x, w, b, eps)
+    D = depth(cols) + 8
+    dm = D * U * xr.abs().mean(-1, keepdim=True)
+    check(mean, m[:, 0], dm[:, 0])
+    dr = (D * U + dm ** 2 * r ** 2) * r
+    check(rstd, r[:, 0], dr[:, 0])
+    want = h * wr + br
+    tol = wr.abs() * (r * dm + h.abs() * (dr / r + 4 * U)) + 4 * U * (br.abs() + want.abs())
+    check(y, want, tol + half_step(t) * (want.abs() + tol) * 1.001 + tiny(t))
+    kept = torch.ones_like(flat, dtype=torch.bool)
+    kept[offset:offset + rows * pitch].view(rows, pitch)[:, :cols] = False
+    assert (flat[kept] == 7.0).all()
+
+    flat, dx = like()
+    dx.copy_(x)
+    dx0 = x.cpu().double()
+    got, dw, db = ops.layer_norm_backward(ctx, dy, x, mean, rstd, w, dx=dx, accumulate_dx=True)
+    assert (flat[kept] == 7.0).all()
+    m, r = mean.cpu().double()[:, None], rstd.cpu().double()[:, None]       # the call's own inputs
+    d = dy.cpu().double()
+    h = (xr - m) * r
+    gw = d * wr
+    m1, m2 = gw.mean(-1, keepdim=True), (gw * h).mean(-1, keepdim=True)
+    want = r * (gw - m1 - h * m2) + dx0
+    D = (depth(cols) + 10) * U
+    size = r * (gw.abs() * 6 * U + D * gw.abs().mean(-1, keepdim=True) + h.abs() * (D * (gw * h).abs().mean(-1, keepdim=True)) +
+                6 * U * (m1.abs() + (h * m2).abs())) + 2 * U * want.abs()
+    check(got, want, size + half_step(t) * (want.abs() + size) * 1.001 + tiny(t))
+    R = (rows + 70) * U
+    for out, terms in ((dw, d * h), (db, d)):
+        tol = (R + 4 * U) * terms.abs().sum(0) + 2 * U * terms.sum(0).abs()
+        check(out, terms.sum(0), tol + half_step(wt) * (terms.sum(0).abs() + tol) * 1.001 + tiny(wt))
+    # in place
+    z = y.clone() if offset == 0 and pitch == cols else y
+    plain, _, _ = ops.layer_norm_backward(ctx, dy, x, mean, rstd, w)
+    over = dy
+    ops.layer_norm_backward(ctx, over, x, mean, rstd, w, dx=over)
+    check(over, plain.double().cpu(), 4 * size + 2 * half_step(t) * (plain.double().cpu().abs() + size) + tiny(t))
+    ops.layer_norm(ctx, x, w, b, eps=eps, out=x)
+    assert torch.equal(x, z)
+
+
 def test_layer_norm_without_weights_and_leading_dimensions(ctx):
     g = gen(8)
     x = randn(g, 12, 96).view(3, 4, 96)
