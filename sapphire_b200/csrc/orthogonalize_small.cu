@@ -14,7 +14,8 @@
 //     distributed shared memory, splits the sums into parts and stores them in every CTA
 //   B = b A + c A A by every CTA for itself
 //   X = a X + B X on the CTA's columns
-// Products, parts and roundings are those of the general way.
+// Products, parts and roundings are those of the general way with two parts, for bf16 too: the
+// products are too short to gain from one.
 #include <type_traits>
 
 #include "gemm_common.cuh"
@@ -48,7 +49,7 @@ __device__ __forceinline__ int small_piece(int r, int c8)
     return (c8 >> 3) * SMALL_TILE + r * 128 + (((c8 & 7) ^ (r & 7)) << 4);
 }
 
-template <typename T, bool SPLIT>
+template <typename T>
 __global__ void __launch_bounds__(SMALL_THREADS, 1) orth_small_kernel(const SmallParams p)
 {
     extern __shared__ uint8_t smem_raw[];
@@ -154,40 +155,49 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) orth_small_kernel(const Smal
         ptx::tc_fence_after_sync();
     };
     const uint32_t x_at = ptx::smem_u32(x), a_at = ptx::smem_u32(am);
-
-    for (int step = 0; step < p.q.steps; ++step) {
-        // ---- partial X X^T: a chain of accumulations per 64 columns, each with an accumulator of
-        // its own.  Small terms come first in every chain here: the tensor core cuts what it
-        // adds at the accumulator's last place, which matters only once hi.hi has begun.
-        const int chains = p.W / 64;
-        run([&]() {
-            constexpr uint32_t idesc = ptx::make_idesc_f16(128, 128, 0, 0);
-            for (int kb = 0; kb < chains; ++kb) {
-                const uint32_t at = x_at + kb * SMALL_TILE;
+    // One chain of accumulations into d: `count` times 16 of k.  Small terms come first: the
+    // tensor core cuts what it adds at the accumulator's last place, which matters only once
+    // hi.hi has begun.  Chains have 32 of k: with 64 the result of narrow matrices (68 x 3567)
+    // was off by 2.0e-6, twice as much as fp32 arithmetic.
+    auto chain = [&](uint32_t d, uint32_t a_step, uint32_t a_part, uint32_t a, uint32_t b, uint32_t b_part, uint32_t idesc, uint32_t b_step,
+                     uint32_t b_lbo, int count) {
 #pragma unroll
-                for (int pass = 0; pass < (SPLIT ? 3 : 1); ++pass) {
-                    const uint32_t pa = at + (SPLIT && pass == 1 ? SMALL_X_PART : 0), pb = at + (SPLIT && pass == 0 ? SMALL_X_PART : 0);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        ptx::mma_f16(tmem + kb * 128, ptx::make_smem_desc(pa + k * 32, 16u, 1024u, ptx::LAYOUT_SW128),
-                                     ptx::make_smem_desc(pb + k * 32, 16u, 1024u, ptx::LAYOUT_SW128), idesc, pass > 0 || k > 0);
-                }
-            }
-        });
-        float acc[32];
-        {
+        for (int pass = 0; pass < 3; ++pass) {
+            const uint32_t pa = a + (pass == 1 ? a_part : 0), pb = b + (pass == 0 ? b_part : 0);
+            for (int k = 0; k < count; ++k)
+                ptx::mma_f16(d, ptx::make_smem_desc(pa + k * a_step, 16u, 1024u, ptx::LAYOUT_SW128),
+                             ptx::make_smem_desc(pb + k * b_step, b_lbo, 1024u, ptx::LAYOUT_SW128), idesc, pass > 0 || k > 0);
+        }
+    };
+    auto add_chains = [&](float (&to)[32], int col, int count, int pitch) {
+#pragma unroll 1
+        for (int c = 0; c < count; ++c) {
             uint32_t u[32];
-            ptx::tmem_ld_32x32(lane_base + group * 32, u);
+            ptx::tmem_ld_32x32(lane_base + c * pitch + col, u);
             ptx::tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 32; ++j) acc[j] = __uint_as_float(u[j]);
-#pragma unroll 1
-            for (int kb = 1; kb < chains; ++kb) {
-                ptx::tmem_ld_32x32(lane_base + kb * 128 + group * 32, u);
-                ptx::tmem_ld_wait();
+            for (int j = 0; j < 32; ++j) to[j] = __fadd_rn(to[j], __uint_as_float(u[j]));
+        }
+    };
+    const int k_chains = p.R > 64 ? 4 : 2;       // of the products over R
+
+    for (int step = 0; step < p.q.steps; ++step) {
+        // ---- partial X X^T, a chain per 32 columns, four at a time
+        float acc[32];
 #pragma unroll
-                for (int j = 0; j < 32; ++j) acc[j] = __fadd_rn(acc[j], __uint_as_float(u[j]));
-            }
+        for (int j = 0; j < 32; ++j) acc[j] = 0.0f;
+        const int chains = p.W / 32;
+#pragma unroll 1
+        for (int c0 = 0; c0 < chains; c0 += 4) {
+            const int count = min(4, chains - c0);
+            run([&]() {
+                constexpr uint32_t idesc = ptx::make_idesc_f16(128, 128, 0, 0);
+                for (int c = 0; c < count; ++c) {
+                    const uint32_t at = x_at + ((c0 + c) >> 1) * SMALL_TILE + ((c0 + c) & 1) * 64;
+                    chain(tmem + c * 128, 32, SMALL_X_PART, at, at, SMALL_X_PART, idesc, 32, 16u, 2);
+                }
+            });
+            add_chains(acc, group * 32, count, 128);
         }
         if (p.ctas == 1) {
 #pragma unroll
@@ -197,7 +207,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) orth_small_kernel(const Smal
                 for (int e = 0; e < 8; ++e) acc[c * 8 + e] *= ORTH_INV_SCALE;
                 split_f16(acc + c * 8, hi, lo);
                 store_raw<false>(reinterpret_cast<f16*>(am + small_piece(row, group * 4 + c)), hi);
-                if (SPLIT) store_raw<false>(reinterpret_cast<f16*>(am + SMALL_A_PART + small_piece(row, group * 4 + c)), lo);
+                store_raw<false>(reinterpret_cast<f16*>(am + SMALL_A_PART + small_piece(row, group * 4 + c)), lo);
             }
         } else {
             // [128 rows][32 pieces of four], a row's pieces permuted by its number
@@ -238,69 +248,50 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) orth_small_kernel(const Smal
                 for (int s = 0; s < p.ctas; ++s) {
                     const uint32_t to = ptx::map_to_cta(at, s);
                     ptx::st_cluster_b64(to, *reinterpret_cast<const uint2*>(hi[k].e));
-                    if (SPLIT) ptx::st_cluster_b64(to + SMALL_A_PART, *reinterpret_cast<const uint2*>(lo[k].e));
+                    ptx::st_cluster_b64(to + SMALL_A_PART, *reinterpret_cast<const uint2*>(lo[k].e));
                 }
             }
             ptx::cluster_sync();
         }
 
-        // ---- B = b A + c A A in A's place (with one part, a on the diagonal)
+        // ---- B = b A + c A A in A's place
         run([&]() {
             constexpr uint32_t idesc = ptx::make_idesc_f16(128, 128, 0, 0);
-#pragma unroll
-            for (int pass = 0; pass < (SPLIT ? 3 : 1); ++pass) {
-#pragma unroll
-                for (int kb = 0; kb < 2; ++kb) {
-                    const uint32_t at = a_at + kb * SMALL_TILE;
-                    const uint32_t pa = at + (SPLIT && pass == 1 ? SMALL_A_PART : 0), pb = at + (SPLIT && pass == 0 ? SMALL_A_PART : 0);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        ptx::mma_f16(tmem, ptx::make_smem_desc(pa + k * 32, 16u, 1024u, ptx::LAYOUT_SW128),
-                                     ptx::make_smem_desc(pb + k * 32, 16u, 1024u, ptx::LAYOUT_SW128), idesc, pass > 0 || kb > 0 || k > 0);
-                }
+            for (int c = 0; c < k_chains; ++c) {
+                const uint32_t at = a_at + (c >> 1) * SMALL_TILE + (c & 1) * 64;
+                chain(tmem + c * 128, 32, SMALL_A_PART, at, at, SMALL_A_PART, idesc, 32, 16u, 2);
             }
         });
         {
-            uint32_t u[32];
-            ptx::tmem_ld_32x32(lane_base + group * 32, u);
-            ptx::tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) acc[j] = 0.0f;
+            add_chains(acc, group * 32, k_chains, 128);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 f16* at = reinterpret_cast<f16*>(am + small_piece(row, group * 4 + c));
                 float h[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
                 Raw<f16, 8> hi, lo;
-                if (SPLIT) {
-                    load_raw<false>(lo, at + SMALL_A_PART / 2);
-                    join_f16(h, lo);
-                }
+                load_raw<false>(lo, at + SMALL_A_PART / 2);
+                join_f16(h, lo);
                 load_raw<false>(hi, at);
                 join_f16(h, hi);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    h[e] = fmaf(p.q.b, h[e], __uint_as_float(u[c * 8 + e]) * (p.q.c * ORTH_INV_SCALE));
-                    if (!SPLIT && row == group * 32 + c * 8 + e) h[e] += p.q.a * ORTH_SCALE;
-                }
+                for (int e = 0; e < 8; ++e) h[e] = fmaf(p.q.b, h[e], acc[c * 8 + e] * (p.q.c * ORTH_INV_SCALE));
                 split_f16(h, hi, lo);
                 store_raw<false>(at, hi);
-                if (SPLIT) store_raw<false>(at + SMALL_A_PART / 2, lo);
+                store_raw<false>(at + SMALL_A_PART / 2, lo);
             }
         }
 
         // ---- X = a X + B X on this CTA's columns
+        // (where W columns leave room for two accumulators only, chains of 64 rows)
+        const int merged = k_chains * p.W > 512 ? 2 : 1, x_chains = k_chains / merged;
         run([&]() {
             const uint32_t idesc = ptx::make_idesc_f16(128, p.W, 0, 1);
-#pragma unroll
-            for (int pass = 0; pass < (SPLIT ? 3 : 1); ++pass) {
-#pragma unroll
-                for (int kb = 0; kb < 2; ++kb) {
-                    const uint32_t pa = a_at + kb * SMALL_TILE + (SPLIT && pass == 1 ? SMALL_A_PART : 0);
-                    const uint32_t pb = x_at + kb * 64 * 128 + (SPLIT && pass == 0 ? SMALL_X_PART : 0);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        ptx::mma_f16(tmem, ptx::make_smem_desc(pa + k * 32, 16u, 1024u, ptx::LAYOUT_SW128),
-                                     ptx::make_smem_desc(pb + k * 16 * 128, SMALL_TILE, 1024u, ptx::LAYOUT_SW128), idesc,
-                                     pass > 0 || kb > 0 || k > 0);
-                }
+            for (int c = 0; c < x_chains; ++c) {
+                const int first = c * merged;    // in units of 32 rows
+                chain(tmem + c * p.W, 32, SMALL_A_PART, a_at + (first >> 1) * SMALL_TILE + (first & 1) * 64, x_at + first * 32 * 128,
+                      SMALL_X_PART, idesc, 16 * 128, SMALL_TILE, 2 * merged);
             }
         });
         const bool last = step + 1 == p.q.steps;
@@ -308,9 +299,16 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) orth_small_kernel(const Smal
 #pragma unroll 1
         for (int j = 0; j < width; j += 16) {
             uint32_t u[16];
-            ptx::tmem_ld_32x16(lane_base + group * width + j, u);
-            ptx::tmem_ld_wait();
             float y[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) y[e] = 0.0f;
+#pragma unroll 1
+            for (int c = 0; c < x_chains; ++c) {
+                ptx::tmem_ld_32x16(lane_base + c * p.W + group * width + j, u);
+                ptx::tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 16; ++e) y[e] = __fadd_rn(y[e], __uint_as_float(u[e]));
+            }
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 f16* at = reinterpret_cast<f16*>(x + small_piece(row, (group * width + j) / 8 + c));
@@ -318,12 +316,10 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) orth_small_kernel(const Smal
                 Raw<f16, 8> hi, lo;
                 load_raw<false>(lo, at + SMALL_X_PART / 2);
                 join_f16(h, lo);
-                if (SPLIT) {
-                    load_raw<false>(hi, at);
-                    join_f16(h, hi);
-                }
+                load_raw<false>(hi, at);
+                join_f16(h, hi);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) h[e] = fmaf(p.q.a, h[e], __uint_as_float(u[c * 8 + e]) * ORTH_INV_SCALE);
+                for (int e = 0; e < 8; ++e) h[e] = fmaf(p.q.a, h[e], y[c * 8 + e] * ORTH_INV_SCALE);
                 if (!last) {
                     split_f16(h, hi, lo);
                     store_raw<false>(at, hi);
@@ -367,7 +363,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) orth_small_kernel(const Smal
     }
 }
 
-template <typename T, bool SPLIT>
+template <typename T>
 cudaLaunchConfig_t small_config(cudaLaunchAttribute (&attr)[2], int64_t batch, int ctas, cudaStream_t stream)
 {
     cudaLaunchConfig_t cfg = {};
@@ -387,17 +383,17 @@ cudaLaunchConfig_t small_config(cudaLaunchAttribute (&attr)[2], int64_t batch, i
 }
 
 // The largest cluster this kernel can have on the context's device: 16, 8, or 0 (asked once).
-template <typename T, bool SPLIT>
+template <typename T>
 int largest_cluster(const sb200_ctx* ctx)
 {
     static int known[16] = {};                   // + 1
     if (ctx->device < 16 && known[ctx->device]) return known[ctx->device] - 1;
-    auto kern = orth_small_kernel<T, SPLIT>;
+    auto kern = orth_small_kernel<T>;
     int most = 0;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMALL_SMEM) == cudaSuccess) {
         most = 8;
         cudaLaunchAttribute attr[2];
-        cudaLaunchConfig_t cfg = small_config<T, SPLIT>(attr, 1, 16, nullptr);
+        cudaLaunchConfig_t cfg = small_config<T>(attr, 1, 16, nullptr);
         cfg.numAttrs = 1;
         int fit = 0;
         if (cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
@@ -409,13 +405,11 @@ int largest_cluster(const sb200_ctx* ctx)
     return most;
 }
 
-// f(T{}, std::bool_constant<two parts>{}) for an element type of the ABI
+// f(T{}) for an element type of the ABI
 template <typename F>
 int with_small_type(int type, F f)
 {
-    if (type == SB200_F32) return f(float{}, std::true_type{});
-    if (type == SB200_F16) return f(f16{}, std::true_type{});
-    return f(bf16{}, std::false_type{});
+    return type == SB200_F32 ? f(float{}) : type == SB200_F16 ? f(f16{}) : f(bf16{});
 }
 
 }  // namespace
@@ -424,17 +418,16 @@ bool orthogonalize_small_fits(const sb200_ctx* ctx, const OrthCall& q)
 {
     const int64_t r = q.rows < q.cols ? q.rows : q.cols, c = q.rows < q.cols ? q.cols : q.rows;
     if (r > 128 || c > SMALL_W * SMALL_CTAS) return false;
-    return with_small_type(q.type, [&](auto t, auto split) -> int {
-        const int most = largest_cluster<decltype(t), decltype(split)::value>(ctx);
+    return with_small_type(q.type, [&](auto t) -> int {
+        const int most = largest_cluster<decltype(t)>(ctx);
         return c <= static_cast<int64_t>(SMALL_W) * most;
     });
 }
 
 int launch_orthogonalize_small(sb200_ctx* ctx, const OrthCall& q, cudaStream_t stream)
 {
-    return with_small_type(q.type, [&](auto t, auto split) -> int {
+    return with_small_type(q.type, [&](auto t) -> int {
         using T = decltype(t);
-        constexpr bool SPLIT = decltype(split)::value;
         SmallParams p{};
         p.q = q;
         p.tall = q.rows > q.cols;
@@ -444,14 +437,14 @@ int launch_orthogonalize_small(sb200_ctx* ctx, const OrthCall& q, cudaStream_t s
         // as much: one CTA up to 256 columns, then as many as give each 128.
         p.ctas = 1;
         if (p.C > SMALL_W)
-            while (p.ctas < largest_cluster<T, SPLIT>(ctx) && p.ctas * 128 < p.C) p.ctas *= 2;
+            while (p.ctas < largest_cluster<T>(ctx) && p.ctas * 128 < p.C) p.ctas *= 2;
         p.W = ((p.C + p.ctas - 1) / p.ctas + 63) / 64 * 64;
         p.status = ctx->d_status;
         p.wait_limit_ns = ctx->wait_limit_ns;
         p.test_stall_kb = ctx->test_stall_kb;
         cudaLaunchAttribute attr[2];
-        const cudaLaunchConfig_t cfg = small_config<T, SPLIT>(attr, q.batch, p.ctas, stream);
-        const cudaError_t err = cudaLaunchKernelEx(&cfg, orth_small_kernel<T, SPLIT>, p);
+        const cudaLaunchConfig_t cfg = small_config<T>(attr, q.batch, p.ctas, stream);
+        const cudaError_t err = cudaLaunchKernelEx(&cfg, orth_small_kernel<T>, p);
         ctx->launches += 1;
         return err == cudaSuccess && cudaGetLastError() == cudaSuccess ? SB200_OK : SB200_ERR_CUDA;
     });
