@@ -159,26 +159,30 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) orth_small_kernel(const Smal
     // tensor core cuts what it adds at the accumulator's last place, which matters only once
     // hi.hi has begun.  Chains have 32 of k: with 64 the result of narrow matrices (68 x 3567)
     // was off by 2.0e-6, twice as much as fp32 arithmetic.
-    auto chain = [&](uint32_t d, uint32_t a_step, uint32_t a_part, uint32_t a, uint32_t b, uint32_t b_part, uint32_t idesc, uint32_t b_step,
-                     uint32_t b_lbo, int count) {
+    auto chain = [&](uint32_t d, uint32_t a_part, uint32_t a, uint32_t b, uint32_t b_part, uint32_t idesc, uint32_t b_step, uint32_t b_lbo,
+                     auto count) {
 #pragma unroll
         for (int pass = 0; pass < 3; ++pass) {
             const uint32_t pa = a + (pass == 1 ? a_part : 0), pb = b + (pass == 0 ? b_part : 0);
-            for (int k = 0; k < count; ++k)
-                ptx::mma_f16(d, ptx::make_smem_desc(pa + k * a_step, 16u, 1024u, ptx::LAYOUT_SW128),
+#pragma unroll
+            for (int k = 0; k < decltype(count)::value; ++k)
+                ptx::mma_f16(d, ptx::make_smem_desc(pa + k * 32, 16u, 1024u, ptx::LAYOUT_SW128),
                              ptx::make_smem_desc(pb + k * b_step, b_lbo, 1024u, ptx::LAYOUT_SW128), idesc, pass > 0 || k > 0);
         }
     };
     auto add_chains = [&](float (&to)[32], int col, int count, int pitch) {
 #pragma unroll 1
-        for (int c = 0; c < count; ++c) {
-            uint32_t u[32];
+        for (int c = 0; c < count; c += 2) {     // (an even number: two loads under way)
+            uint32_t u[32], v[32];
             ptx::tmem_ld_32x32(lane_base + c * pitch + col, u);
+            ptx::tmem_ld_32x32(lane_base + (c + 1) * pitch + col, v);
             ptx::tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 32; ++j) to[j] = __fadd_rn(to[j], __uint_as_float(u[j]));
+            for (int j = 0; j < 32; ++j) to[j] = __fadd_rn(__fadd_rn(to[j], __uint_as_float(u[j])), __uint_as_float(v[j]));
         }
     };
+    using Two = std::integral_constant<int, 2>;
+    using Four = std::integral_constant<int, 4>;
     const int k_chains = p.R > 64 ? 4 : 2;       // of the products over R
 
     for (int step = 0; step < p.q.steps; ++step) {
@@ -194,7 +198,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) orth_small_kernel(const Smal
                 constexpr uint32_t idesc = ptx::make_idesc_f16(128, 128, 0, 0);
                 for (int c = 0; c < count; ++c) {
                     const uint32_t at = x_at + ((c0 + c) >> 1) * SMALL_TILE + ((c0 + c) & 1) * 64;
-                    chain(tmem + c * 128, 32, SMALL_X_PART, at, at, SMALL_X_PART, idesc, 32, 16u, 2);
+                    chain(tmem + c * 128, SMALL_X_PART, at, at, SMALL_X_PART, idesc, 32, 16u, Two{});
                 }
             });
             add_chains(acc, group * 32, count, 128);
@@ -259,7 +263,7 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) orth_small_kernel(const Smal
             constexpr uint32_t idesc = ptx::make_idesc_f16(128, 128, 0, 0);
             for (int c = 0; c < k_chains; ++c) {
                 const uint32_t at = a_at + (c >> 1) * SMALL_TILE + (c & 1) * 64;
-                chain(tmem + c * 128, 32, SMALL_A_PART, at, at, SMALL_A_PART, idesc, 32, 16u, 2);
+                chain(tmem + c * 128, SMALL_A_PART, at, at, SMALL_A_PART, idesc, 32, 16u, Two{});
             }
         });
         {
@@ -290,24 +294,26 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) orth_small_kernel(const Smal
             const uint32_t idesc = ptx::make_idesc_f16(128, p.W, 0, 1);
             for (int c = 0; c < x_chains; ++c) {
                 const int first = c * merged;    // in units of 32 rows
-                chain(tmem + c * p.W, 32, SMALL_A_PART, a_at + (first >> 1) * SMALL_TILE + (first & 1) * 64, x_at + first * 32 * 128,
-                      SMALL_X_PART, idesc, 16 * 128, SMALL_TILE, 2 * merged);
+                const uint32_t a = a_at + (first >> 1) * SMALL_TILE + (first & 1) * 64, b = x_at + first * 32 * 128;
+                if (merged == 2) chain(tmem + c * p.W, SMALL_A_PART, a, b, SMALL_X_PART, idesc, 16 * 128, SMALL_TILE, Four{});
+                else chain(tmem + c * p.W, SMALL_A_PART, a, b, SMALL_X_PART, idesc, 16 * 128, SMALL_TILE, Two{});
             }
         });
         const bool last = step + 1 == p.q.steps;
         const int width = p.W / 4;               // columns of this warp
 #pragma unroll 1
         for (int j = 0; j < width; j += 16) {
-            uint32_t u[16];
             float y[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) y[e] = 0.0f;
 #pragma unroll 1
-            for (int c = 0; c < x_chains; ++c) {
+            for (int c = 0; c < x_chains; c += 2) {
+                uint32_t u[16], v[16];
                 ptx::tmem_ld_32x16(lane_base + c * p.W + group * width + j, u);
+                ptx::tmem_ld_32x16(lane_base + (c + 1) * p.W + group * width + j, v);
                 ptx::tmem_ld_wait();
 #pragma unroll
-                for (int e = 0; e < 16; ++e) y[e] = __fadd_rn(y[e], __uint_as_float(u[e]));
+                for (int e = 0; e < 16; ++e) y[e] = __fadd_rn(__fadd_rn(y[e], __uint_as_float(u[e])), __uint_as_float(v[e]));
             }
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
