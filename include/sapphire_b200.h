@@ -647,7 +647,8 @@ int sb200_layer_norm_backward(sb200_ctx* ctx, void* dx, int64_t lddx, void* dwei
  * out = X.  The usual coefficients 3.4445, -4.7750, 2.0315 and five steps bring the
  * singular values near one.  g and out are of `type` and may be the same matrix.
  * SB200_F32 and SB200_F16 are computed to about fp32 accuracy (operands in two fp16
- * parts, 22 bits); SB200_BF16 with operands of 11 bits, its own result having 8.
+ * parts, 22 bits); SB200_BF16, its own result having 8, with operands of 11 bits
+ * where both sides are longer than 128.
  * Coefficients that let a singular value s, or |b s^2 + c s^4| with or without a in
  * front, pass about 7 on the way are refused (SB200_ERR_UNSUPPORTED).  Limits
  * (SB200_ERR_TOO_LARGE): sides <= 2^20, batch <= 65535, steps <= 64.  The waits inside

@@ -14,7 +14,8 @@
 // its pieces of the next rows on the way into shared memory (its own slots, so nothing
 // but the thread itself waits for them): the memory system always has several rows a
 // block to work on, which one row at a time in registers does not give it (65536 x 4096
-// bf16 forward: 291 us).  In the backward pass every thread keeps the column sums of its
+// bf16 forward: 291 us, so 180 to 192 or 5.6 to 6.0 TB/s; 32768 x 4096 fp32 backward: 240 us,
+// 6.7 TB/s).  In the backward pass every thread keeps the column sums of its
 // columns in registers over all the rows its block sees, writes one partial sum a block,
 // and a second kernel adds the partials in block order: no atomics, the same bits run to
 // run.  Rows that 16-byte accesses do not fit take 4-byte ones.  Odd rows of 16-bit elements

@@ -17,10 +17,13 @@
 //     so a chain of accumulations ends after CHUNK_KB k-blocks and the chains are added
 //     in registers.  a X is added in the epilogue: inside the chains it would triple
 //     their error.
-//   bf16 input: the products take the hi parts alone (11 bits; the result keeps 8), with
+//   bf16 input (both sides longer than 128): the products take the hi parts alone (11 bits; the result keeps 8), with
 //     X = (a + B) hi + a lo: a stands on the diagonal of B, which saves reading hi again.
 //     X has both parts because rounding X itself every step would feed the small singular
 //     directions, which a step multiplies by a, with the rounding errors of the large ones.
+//
+// Five steps take 150 us for 784 x 512 fp32, 473 to 505 us for 4 x 1024 x 4096 bf16 and 3.6 ms
+// for 4096 x 4096 fp32 (1375 GFLOP in triangles, 382 TFLOP/s, three times that as fp16 products).
 //
 // A and A A are symmetric: only tiles on and above the diagonal are computed, and a tile
 // above it is also stored transposed.  X X^T and A A read both operands along k; B X reads

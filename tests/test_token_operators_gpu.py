@@ -533,6 +533,14 @@ def test_orthogonalize_large(ctx, t, rows, cols):
     assert rel(out, x.mT if rows > cols else x) <= ns_tolerance(t)
 
 
+@pytest.mark.parametrize("batch,rows,cols", [(1, 45, 813), (3, 128, 128), (2, 700, 100), (1, 17, 4096)])
+def test_orthogonalize_narrow_bf16(ctx, batch, rows, cols):
+    """With a side of at most 128 the operands have 22 bits for bf16 too: what is left is the
+    bar of the fp32-accurate products and the result's own rounding."""
+    g = gradient(gen(rows + cols), batch, rows, cols, dtype=BF16)
+    assert rel(ops.orthogonalize(ctx, g), ns_reference(g)) <= 1e-5 + half_step(BF16)
+
+
 def test_orthogonalize_strides_steps_and_in_place(ctx):
     g = gen(4)
     wide = gradient(g, 90, 200)
