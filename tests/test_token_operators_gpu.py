@@ -656,6 +656,33 @@ def test_captured_products_and_long_sorts(ctx, rows, cols):
     ctx.check_device_status()
 
 
+def test_two_streams_at_once(ctx):
+    """Calls of one context on two streams, in flight together: nothing of theirs is shared."""
+    g = gen(15)
+    ms = [gradient(g, 300, 700), gradient(g, 2304, 2500), gradient(g, 100, 900)]
+    ids = [token_ids(g, n, 3000, torch.int64).to(DEV) for n in (20000, 5000)]
+    douts = [randn(g, len(i), 136) for i in ids]
+    x, w = randn(g, 4001, 999, dtype=BF16), randn(g, 999)
+
+    def work():
+        out = [ops.orthogonalize(ctx, m) for m in ms]
+        out += [ops.embedding_backward(ctx, torch.empty(3000, 136, device=DEV), d, i) for d, i in zip(douts, ids)]
+        y, mean, rstd = ops.layer_norm(ctx, x, w)
+        return out + [y, *ops.layer_norm_backward(ctx, y, x, mean, rstd, w)]
+
+    want = work()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for _ in range(4):
+        for st in streams:
+            with torch.cuda.stream(st):
+                got.append(work())
+    torch.cuda.synchronize()
+    ctx.check_device_status()
+    assert all(torch.equal(p, q) for out in got for p, q in zip(out, want))
+
+
 def test_offsets_beyond_32_bits(ctx):
     """Rows so far apart that the last ones start more than 2^32 elements in."""
     g = gen(14)
