@@ -774,7 +774,7 @@ OrthPlan plan_orth(int64_t rows, int64_t cols, int64_t batch, int type)
     q.batch = batch;
     q.ldx = (q.C + 63) / 64 * 64;
     q.lda = (q.R + 63) / 64 * 64;
-    q.split = type != SB200_BF16;
+    q.split = type != SB200_BF16 || q.R <= 128;  // whichever kernel a narrow matrix takes, its operands have 22 bits
     int64_t at = 0;
     auto take = [&](int64_t bytes) { const int64_t o = at; at += (bytes + 255) / 256 * 256; return o; };
     for (int i = 0; i < 2; ++i) q.x[i] = take(2 * batch * q.R * q.ldx * 2);

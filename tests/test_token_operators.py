@@ -161,6 +161,15 @@ def test_workspace_sizes(fake):
     assert lib.sb200_orthogonalize_workspace(512, 784, 1, L.F32) >= 2 * (4 * 512 * 784 + 4 * 512 * 512)
 
 
+def test_workspace_of_narrow_bf16(fake):
+    """With a side of at most 128 every operand has two parts, for bf16 as for fp32; with both
+    sides longer A and B have one."""
+    size = L.lib().sb200_orthogonalize_workspace
+    for rows, cols in ((128, 4097), (45, 6000), (6000, 100), (1, 5000)):
+        assert size(rows, cols, 2, L.BF16) == size(rows, cols, 2, L.F32)
+    assert size(129, 4097, 2, L.BF16) < size(129, 4097, 2, L.F32)
+
+
 @pytest.mark.skipif(torch.cuda.is_available(), reason="would launch on a stand-in context")
 def test_valid_calls_reach_the_device_and_fail_there(fake):
     """The checks let these pass: without a device the next thing is a CUDA error."""

@@ -541,6 +541,17 @@ def test_orthogonalize_narrow_bf16(ctx, batch, rows, cols):
     assert rel(ops.orthogonalize(ctx, g), ns_reference(g)) <= 1e-5 + half_step(BF16)
 
 
+@pytest.mark.parametrize("batch,rows,cols", [(1, 128, 4097), (1, 45, 6000), (2, 4500, 100), (1, 128, 4096)])
+def test_orthogonalize_narrow_bf16_of_any_length(ctx, batch, rows, cols):
+    """22 bits whichever kernel such a matrix takes.  A result d away from the definition rounds
+    to another number than it with a probability of |d| / spacing, and is then one spacing off:
+    the squares add up to sum |d| spacing <= 1e-5 |x| 2^-7 |x| (operands of 11 bits: 2e-3 |x|)."""
+    g = gradient(gen(rows + cols), batch, rows, cols, dtype=BF16)
+    out = ops.orthogonalize(ctx, g)
+    ctx.check_device_status()
+    assert rel(out, ns_reference(g).to(BF16)) <= (1e-5 * 2.0 ** -7) ** 0.5
+
+
 def test_orthogonalize_strides_steps_and_in_place(ctx):
     g = gen(4)
     wide = gradient(g, 90, 200)
