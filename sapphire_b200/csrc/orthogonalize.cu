@@ -45,6 +45,7 @@ constexpr int MMA_K = 16;
 constexpr int TILE_BYTES = 128 * KB * 2;         // 128 rows (or columns) x 64 k
 constexpr int MN_CHUNK_BYTES = 64 * KB * 2;      // MN-major: 64 k rows x 64 columns
 constexpr int CHUNK_KB = 2;                      // k-blocks per accumulation chain with two parts (1 in the sliced kernel)
+constexpr int LONG_CHAIN_KB = 64;                // of X X^T with one part: 256 accumulations lose 2.4e-5 of a sum of positive terms
 constexpr float SCALE = ORTH_SCALE, INV_SCALE = ORTH_INV_SCALE;
 constexpr double LARGEST = 7.5;                  // of a singular value: 7.5 * 2^13 < 65504
 constexpr int EPI_WARPS = 16;
@@ -412,7 +413,7 @@ orth_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             if constexpr (PAIR && (READS_HI || READS_LO)) {
                 if (blocks > 0) fetch(0);        // travels while the products run
             }
-            if (SPLIT || !PAIR) {
+            if (SPLIT || !PAIR || (WHAT == GRAM && p.chunk_kb < p.num_kb)) {
                 // chains of accumulations are added here, rounded to nearest
                 float sum[COLS];
 #pragma unroll
@@ -867,7 +868,11 @@ template <int WHAT>
 int product(sb200_ctx* ctx, bool split, const OrthMaps& m, OrthParams p, cudaStream_t stream)
 {
     p.slices = slices_for(ctx, p.rows, p.cols, p.batch, p.num_kb, WHAT != APPLY, split);
-    p.chunk_kb = !split ? p.num_kb : p.slices == 0 ? CHUNK_KB : 1;
+    // One part: X X^T runs over the longer side, up to 2^20, and its diagonal adds positive terms alone, so that
+    // what the chain cuts off goes to one side: 3.0e-3 of a sum over 2^19 columns in a single chain (measured,
+    // 0.8 x 2^-23 an accumulation).  The others run over the shorter side; where that is 2^16 (X in its parts
+    // and copies then takes 69 GB) a chain loses 4e-4, less than the half step of its fp16 operands.
+    p.chunk_kb = split ? (p.slices == 0 ? CHUNK_KB : 1) : WHAT == GRAM && p.num_kb > LONG_CHAIN_KB ? LONG_CHAIN_KB : p.num_kb;
     if (p.slices == 0)
         return split ? launch_product<WHAT, true, true>(ctx, m, p, stream) : launch_product<WHAT, true, false>(ctx, m, p, stream);
     return split ? launch_product<WHAT, false, true>(ctx, m, p, stream) : launch_product<WHAT, false, false>(ctx, m, p, stream);

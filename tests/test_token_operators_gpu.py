@@ -552,6 +552,31 @@ def test_orthogonalize_narrow_bf16_of_any_length(ctx, batch, rows, cols):
     assert rel(out, ns_reference(g).to(BF16)) <= (1e-5 * 2.0 ** -7) ** 0.5
 
 
+@pytest.mark.parametrize("rows", [2048, 2304])
+def test_orthogonalize_bf16_long_sums(ctx, rows):
+    """X X^T over 2^19 columns whose terms are all positive: the tensor core cuts every
+    accumulation, so one chain over all of them loses 3.0e-3 of the sum, always to one side.
+    (2048 rows take tiles of one SM, 2304 of pairs.)
+
+    The rows are s_i times orthogonal signs, so with a = c = 0, b = 1 a step gives
+    x_ij * (2^19 x_ij^2).  A row's result has the rounding of x (half a step of fp16, three
+    times over), of A and of the result; their mean over the rows has a deviation of a
+    rows^1/2-th of that, four of which are allowed, and a chain of at most 256 accumulations
+    may lose four units of 2^-23 each."""
+    g, cols = gen(rows), 1 << 19
+    signs = torch.ones(1, 1, device=DEV)
+    while signs.shape[0] < 4096:
+        signs = torch.cat([torch.cat([signs, signs], 1), torch.cat([signs, -signs], 1)], 0)
+    signs = signs[:rows]
+    s = (1 + torch.rand(rows, generator=g)).to(BF16).to(DEV)
+    out = ops.orthogonalize(ctx, (signs * s[:, None]).to(BF16).repeat(1, cols // 4096), steps=1, coefficients=(0.0, 1.0, 0.0))
+    ctx.check_device_status()
+    x = s.double() / (cols * s.double().square().sum()).sqrt()
+    off = (out[:, -4096:].double() * signs / (cols * x ** 3)[:, None]).mean() - 1
+    spread = (half_step(BF16) ** 2 + (3 * half_step(F16)) ** 2 + half_step(F16) ** 2) ** 0.5 / 3 ** 0.5
+    assert abs(float(off)) <= 256 * 4 * 2.0 ** -23 + 4 * spread / rows ** 0.5
+
+
 def test_orthogonalize_strides_steps_and_in_place(ctx):
     g = gen(4)
     wide = gradient(g, 90, 200)
