@@ -21,9 +21,16 @@
 //     X = (a + B) hi + a lo: a stands on the diagonal of B, which saves reading hi again.
 //     X has both parts because rounding X itself every step would feed the small singular
 //     directions, which a step multiplies by a, with the rounding errors of the large ones.
+//     Why one part: the three roundings a step (of X, A and B; each adds about as much) leave
+//     the result off by 0.6e-3 to 1.2e-3 (2-norm), less than its own rounding to bf16, 1.66e-3;
+//     together 1.78e-3 to 2.07e-3 where two parts, and fp32 arithmetic, give 1.66e-3.  Two parts
+//     take three products: 1.02 ms instead of 0.47 for 4 x 1024 x 4096, 3.64 instead of 1.28 for
+//     4096 x 4096, 157 us instead of 121 for 2 x 153 x 188.  Dropping one of the roundings alone
+//     saves little of the error.  Who needs more than this has the fp32 call.
 //
-// Five steps take 150 us for 784 x 512 fp32, 473 to 505 us for 4 x 1024 x 4096 bf16 and 3.6 ms
-// for 4096 x 4096 fp32 (1375 GFLOP in triangles, 382 TFLOP/s, three times that as fp16 products).
+// Five steps take 150 us for 784 x 512 fp32, 470 to 505 us for 4 x 1024 x 4096 bf16 and 3.6 to
+// 3.8 ms for 4096 x 4096 fp32, by box (1375 GFLOP in triangles, 362 to 382 TFLOP/s, three times
+// that as fp16 products).
 //
 // A and A A are symmetric: only tiles on and above the diagonal are computed, and a tile
 // above it is also stored transposed.  X X^T and A A read both operands along k; B X reads
