@@ -140,11 +140,13 @@ enum { SB200_OPT_SPLIT_EXPLICIT_HI = 1, SB200_OPT_MERGE_MN_BOXES = 2, SB200_OPT_
        SB200_OPT_K_SLICES = 8, SB200_OPT_SPLIT_A_TMEM = 9 };
 int sb200_ctx_set_option(sb200_ctx* ctx, int option, int value);
 
-/* Reads (and clears) the device status word after synchronising the stream.
+/* Reads the device status after synchronising the stream, and clears what it reports.
  * SB200_ERR_DEVICE_TIMEOUT means a bounded wait in a kernel gave up: the results of
  * that launch are undefined.  SB200_ERR_TOKEN_RANGE means an embedding call met a
- * token number beyond the vocabulary and treated it as padding.  The word keeps the
- * first of several events; the context stays usable. */
+ * token number beyond the vocabulary and treated it as padding.  The two are kept
+ * apart: where both happened, in whatever order, the first call reports the timeout
+ * and the next one the token.  Several events of one kind are reported once; the
+ * context stays usable. */
 int sb200_check_device_status(sb200_ctx* ctx, sb200_stream stream);
 
 /*

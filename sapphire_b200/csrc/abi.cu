@@ -187,16 +187,19 @@ extern "C" int sb200_check_device_status(sb200_ctx* ctx, sb200_stream stream_)
     if (!ctx)
         return SB200_ERR_INVALID_ARG;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-    unsigned word = 0;
-    if (cudaMemcpyAsync(&word, ctx->d_status, sizeof(word), cudaMemcpyDeviceToHost, stream) !=
+    unsigned word[2] = {0, 0};
+    static_assert(TOKEN_RANGE_WORD == 1, "both words are read in one copy");
+    if (cudaMemcpyAsync(word, ctx->d_status, sizeof(word), cudaMemcpyDeviceToHost, stream) !=
             cudaSuccess ||
         cudaStreamSynchronize(stream) != cudaSuccess)
         return SB200_ERR_CUDA;
-    if (word == 0)
+    if (word[0] == 0 && word[TOKEN_RANGE_WORD] == 0)
         return SB200_OK;
-    cudaMemsetAsync(ctx->d_status, 0, sizeof(unsigned), stream);
+    // the expired wait first; each call reports and clears one of the two
+    const int which = word[0] ? 0 : TOKEN_RANGE_WORD;
+    cudaMemsetAsync(ctx->d_status + which, 0, sizeof(unsigned), stream);
     cudaStreamSynchronize(stream);
-    return word == FAULT_TOKEN_RANGE ? SB200_ERR_TOKEN_RANGE : SB200_ERR_DEVICE_TIMEOUT;
+    return which ? SB200_ERR_TOKEN_RANGE : SB200_ERR_DEVICE_TIMEOUT;
 }
 
 namespace {

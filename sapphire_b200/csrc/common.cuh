@@ -26,8 +26,7 @@ enum DeviceFault : unsigned {
     FAULT_MMA_WAIT_TMEM = 0x103,   // MMA issuer waiting for a drained accumulator
     FAULT_EPI_WAIT = 0x104,        // epilogue waiting for a finished accumulator
     FAULT_SPLIT_WAIT = 0x105,      // hi/lo split warps waiting for a filled stage
-    FAULT_PEER_WAIT = 0x201,       // gradient exchange waiting for another rank's announcement
-    FAULT_TOKEN_RANGE = 0x301      // embedding: a token number beyond the vocabulary
+    FAULT_PEER_WAIT = 0x201        // gradient exchange waiting for another rank's announcement
 };
 
 struct GemmArgs {
@@ -81,8 +80,12 @@ struct alignas(64) TensorMapSlot {
     uint64_t stamp;        // last use; 0 = empty
 };
 constexpr int TENSOR_MAP_SLOTS = 64;
-// The status allocation: word 0 is the device status word; from SLICE_TICKET_OFFSET on,
-// one ticket counter per output tile of a k-sliced GEMM (zero between launches).
+// The status allocation: word 0 is what a bounded wait that gave up writes; word
+// TOKEN_RANGE_WORD is non-zero once an embedding call met a token number beyond the
+// vocabulary (a word of its own: that call's results are defined, and it must not hide an
+// expired wait); from SLICE_TICKET_OFFSET on, one ticket counter per output tile of a
+// k-sliced GEMM (zero between launches).
+constexpr int TOKEN_RANGE_WORD = 1;
 constexpr int SLICE_TICKET_OFFSET = 16;
 constexpr int SLICE_TICKETS = 240;
 constexpr int STATUS_WORDS = SLICE_TICKET_OFFSET + SLICE_TICKETS;
@@ -93,7 +96,7 @@ struct sb200_ctx {
     int sm_count;
     int last_path;
     int64_t launches;
-    unsigned* d_status;        // device status word
+    unsigned* d_status;        // device status words (STATUS_WORDS of them)
     float* d_workspace;        // scratch for partial column sums / sparse row work
     size_t workspace_bytes;
     int split_explicit_hi;     // 3xTF32: rewrite the high part in shared memory too

@@ -30,7 +30,8 @@ namespace {
 constexpr int LOOKUP_THREADS = 256;
 constexpr int LOOKUP_LANES = 64;         // threads a token at most
 
-__device__ __forceinline__ void report_range(unsigned* status) { atomicCAS(status, 0u, static_cast<unsigned>(FAULT_TOKEN_RANGE)); }
+// Every thread that meets such a number writes the same value.
+__device__ __forceinline__ void report_range(unsigned* token_range) { *token_range = 1u; }
 
 // `lanes` (power of two) threads per token, VEC elements an access.  What counts is how many
 // accesses a thread has under way: eight of one row where rows are long enough (65536 x
@@ -40,7 +41,7 @@ template <typename TT, typename TA, typename I, int VEC, int ROWS>
 __global__ void __launch_bounds__(LOOKUP_THREADS)
 lookup_kernel(TA* __restrict__ out, int64_t ldo, const TT* __restrict__ table, int64_t ldt,
               const I* __restrict__ ids, int64_t n, int64_t vocab, int nvec, float scale, int lanes,
-              unsigned* status)
+              unsigned* token_range)
 {
     const int lane = threadIdx.x & (lanes - 1);
     const int per_block = LOOKUP_THREADS / lanes;
@@ -51,7 +52,7 @@ lookup_kernel(TA* __restrict__ out, int64_t ldo, const TT* __restrict__ table, i
         const int64_t t = t0 + static_cast<int64_t>(k) * per_block;
         id[k] = t < n ? static_cast<int64_t>(ids[t]) : -1;
         if (id[k] >= vocab) {
-            if (lane == 0) report_range(status);
+            if (lane == 0) report_range(token_range);
             id[k] = -1;
         }
     }
@@ -85,10 +86,10 @@ constexpr int SORT_BLOCKS = 64;                              // at most: every b
 
 // The sort key of a token: its vocabulary row, or `vocab` (last) for padding.
 template <typename I>
-__device__ __forceinline__ uint32_t key_of(I id, int64_t vocab, unsigned* status)
+__device__ __forceinline__ uint32_t key_of(I id, int64_t vocab, unsigned* token_range)
 {
     const int64_t v = static_cast<int64_t>(id);
-    if (v >= vocab) report_range(status);
+    if (v >= vocab) report_range(token_range);
     return static_cast<uint32_t>(v < 0 || v >= vocab ? vocab : v);
 }
 
@@ -97,7 +98,7 @@ template <typename I, bool FIRST>
 __global__ void __launch_bounds__(SORT_THREADS)
 sort_count_kernel(uint32_t* __restrict__ counts, uint32_t* __restrict__ touched, const I* __restrict__ ids,
                   const uint32_t* __restrict__ keys, int64_t n, int64_t per_block, int64_t vocab, int shift,
-                  unsigned* status)
+                  unsigned* token_range)
 {
     __shared__ uint32_t hist[DIGITS];
     ptx::griddep_launch_dependents();
@@ -108,7 +109,7 @@ sort_count_kernel(uint32_t* __restrict__ counts, uint32_t* __restrict__ touched,
     for (int64_t i = i0 + threadIdx.x; i < i1; i += SORT_THREADS) {
         uint32_t key;
         if constexpr (FIRST) {
-            key = key_of(ids[i], vocab, status);
+            key = key_of(ids[i], vocab, token_range);
             if (touched && key < vocab) atomicOr(&touched[key >> 5], 1u << (key & 31));
         } else {
             key = keys[i];
@@ -125,7 +126,7 @@ __global__ void __launch_bounds__(SORT_THREADS)
 sort_scatter_kernel(uint32_t* __restrict__ keys_out, uint32_t* __restrict__ pos_out,
                     const uint32_t* __restrict__ counts, const I* __restrict__ ids,
                     const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos, int64_t n,
-                    int64_t per_block, int64_t vocab, int shift, unsigned* status)
+                    int64_t per_block, int64_t vocab, int shift, unsigned* token_range)
 {
     __shared__ uint32_t offset[DIGITS];                      // where this block's next item of a digit goes
     __shared__ unsigned short ahead[SORT_WARPS][DIGITS];     // items of a digit in the warps before, this tile
@@ -173,7 +174,7 @@ sort_scatter_kernel(uint32_t* __restrict__ keys_out, uint32_t* __restrict__ pos_
             key[k] = from[k] = 0;
             if (in) {
                 if constexpr (FIRST) {
-                    key[k] = key_of(ids[i], vocab, status);
+                    key[k] = key_of(ids[i], vocab, token_range);
                     from[k] = static_cast<uint32_t>(i);
                 } else {
                     key[k] = keys[i];
@@ -252,7 +253,7 @@ template <typename I, typename TT, int VEC>
 __global__ void __launch_bounds__(SORT_THREADS)
 sort_small_kernel(uint32_t* __restrict__ keys_out, uint32_t* __restrict__ pos_out, uint32_t* __restrict__ long_runs,
                   const I* __restrict__ ids, int n, int64_t vocab, int passes, TT* __restrict__ dtable, int64_t ldt,
-                  int64_t nvec, unsigned* status)
+                  int64_t nvec, unsigned* token_range)
 {
     ptx::griddep_launch_dependents();
     if (blockIdx.x > 0) {
@@ -281,7 +282,7 @@ sort_small_kernel(uint32_t* __restrict__ keys_out, uint32_t* __restrict__ pos_ou
             const int i = i0 + k * 32;
             key[k] = where[k] = 0;
             if (k < rounds && i < n) {
-                key[k] = pass == 0 ? key_of(ids[i], vocab, status) : skey[i];
+                key[k] = pass == 0 ? key_of(ids[i], vocab, token_range) : skey[i];
                 where[k] = pass == 0 ? i : spos[i];
             }
         }
@@ -628,10 +629,10 @@ int sort_large(sb200_ctx* ctx, const GradPlan& g, unsigned char* ws, const I* id
         uint32_t *kout = u32(g.keys[to]), *pout = u32(g.pos[to]);
         const uint32_t *kin = u32(g.keys[to ^ 1]), *pin = u32(g.pos[to ^ 1]);
         int rc = launch_after(ctx, pass == 0 ? sort_count_kernel<I, true> : sort_count_kernel<I, false>, static_cast<unsigned>(g.blocks), SORT_THREADS, 0, stream,
-                              counts, touched, ids, kin, n, g.per_block, vocab, shift, ctx->d_status);
+                              counts, touched, ids, kin, n, g.per_block, vocab, shift, ctx->d_status + TOKEN_RANGE_WORD);
         if (!rc)
             rc = launch_after(ctx, pass == 0 ? sort_scatter_kernel<I, true> : sort_scatter_kernel<I, false>, static_cast<unsigned>(g.blocks), SORT_THREADS, 0,
-                              stream, kout, pout, counts, ids, kin, pin, n, g.per_block, vocab, shift, ctx->d_status);
+                              stream, kout, pout, counts, ids, kin, pin, n, g.per_block, vocab, shift, ctx->d_status + TOKEN_RANGE_WORD);
         if (rc) return rc;
     }
     *buffer = (g.passes - 1) & 1;
@@ -655,7 +656,7 @@ int launch_grad(sb200_ctx* ctx, const GradPlan& g, unsigned char* ws, TT* dtable
         }
         int64_t fill = accumulate ? 0 : vocab < ctx->sm_count ? vocab : ctx->sm_count - 1;
         kern<<<static_cast<unsigned>(1 + fill), SORT_THREADS, SMALL_SMEM, stream>>>(
-            u32(g.keys[0]), u32(g.pos[0]), u32(g.long_runs), ids, static_cast<int>(n), vocab, g.passes, dtable, ldt, nvec, ctx->d_status);
+            u32(g.keys[0]), u32(g.pos[0]), u32(g.long_runs), ids, static_cast<int>(n), vocab, g.passes, dtable, ldt, nvec, ctx->d_status + TOKEN_RANGE_WORD);
         ctx->launches += 1;
         if (cudaGetLastError() != cudaSuccess) return SB200_ERR_CUDA;
         if (n == 0) return SB200_OK;
@@ -732,7 +733,7 @@ extern "C" int sb200_embedding(sb200_ctx* ctx, void* out, int64_t ldo, const voi
                 const unsigned grid = static_cast<unsigned>((n + per_block - 1) / per_block);
                 lookup_kernel<TT, TA, I, VEC, ROWS><<<grid, LOOKUP_THREADS, 0, stream>>>(
                     static_cast<TA*>(out), ldo, static_cast<const TT*>(table), ldt, static_cast<const I*>(ids), n, vocab,
-                    static_cast<int>(nvec), scale, lanes, ctx->d_status);
+                    static_cast<int>(nvec), scale, lanes, ctx->d_status + TOKEN_RANGE_WORD);
             };
             auto rows = [&](auto id) {
                 if (nvec > LOOKUP_LANES) go(id, Int<1>{});

@@ -118,6 +118,39 @@ def test_embedding_out_of_range_is_reported(ctx):
     assert dt.sum().item() == 16 and dt[0, 0] == 1 and dt[9, 0] == 1
 
 
+@pytest.mark.parametrize("token_first", [True, False])
+@pytest.mark.parametrize("product", ["gemm", "orthogonalize"])
+def test_a_bad_token_hides_no_expired_wait(ctx, product, token_first):
+    """A token number beyond the vocabulary and a wait that runs out are reported each, the
+    wait first, in whatever order they came."""
+    table = torch.ones(10, 8, device=DEV)
+    ids = torch.tensor([3, 10], device=DEV)
+    a = randn(gen(1), 320, 320)                            # (two k-blocks a slice: one of them is held back)
+
+    def stalled():
+        ctx.set_option(L.OPT_WAIT_LIMIT_US, 2000)
+        ctx.set_option(L.OPT_TEST_STALL_KBLOCKS, 1)
+        try:
+            ops.gemm(ctx, a, a) if product == "gemm" else ops.orthogonalize(ctx, a, steps=1)
+            torch.cuda.synchronize()
+        finally:
+            ctx.set_option(L.OPT_TEST_STALL_KBLOCKS, -1)
+            ctx.set_option(L.OPT_WAIT_LIMIT_US, 2000000)
+
+    ctx.check_device_status()
+    if token_first:
+        ops.embedding(ctx, table, ids)
+        stalled()
+    else:
+        stalled()
+        ops.embedding_backward(ctx, table, torch.ones(2, 8, device=DEV), ids)
+    for status in (L.ERR_DEVICE_TIMEOUT, L.ERR_TOKEN_RANGE):
+        with pytest.raises(L.Sb200Error) as e:
+            ctx.check_device_status()
+        assert e.value.status == status
+    ctx.check_device_status()
+
+
 def grad_reference(dout, ids, vocab, scale):
     keep = ids >= 0
     want = torch.zeros(vocab, dout.shape[1], dtype=torch.float64)
