@@ -38,6 +38,7 @@ def im2col(ctx: ops.Context, x: torch.Tensor, kh: int, kw: int, stride: Pair = (
            out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x [N, C, H, W] (contiguous) -> cols [N, C*kh*kw, outR*outC] (``out`` if given:
     contiguous, that shape)."""
+    ops._fp32(x)
     N, Cc, H, W = x.shape
     P = out_size(H, pad[0], dil[0], kh, stride[0]) * out_size(W, pad[1], dil[1], kw, stride[1])
     shape = (N, Cc * kh * kw, P)
@@ -56,6 +57,7 @@ def im2col(ctx: ops.Context, x: torch.Tensor, kh: int, kw: int, stride: Pair = (
 def col2im(ctx: ops.Context, dx: torch.Tensor, cols: torch.Tensor, kh: int, kw: int,
            stride: Pair = (1, 1), pad: Pair = (0, 0), dil: Pair = (1, 1)) -> torch.Tensor:
     """dx [N, C, H, W] (contiguous) += adjoint of im2col applied to cols."""
+    ops._fp32(dx, cols)
     g = _geometry(dx.shape, kh, kw, stride, pad, dil)
     L.check("sb200_col2im", L.lib().sb200_col2im(ctx.handle, dx.data_ptr(), cols.data_ptr(), C.byref(g),
                                                   ops._stream_ptr(ctx.device)))

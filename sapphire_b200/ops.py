@@ -105,6 +105,7 @@ def prepare_gemm(ctx: Context, a: torch.Tensor, b: torch.Tensor, c: Optional[tor
     """The call `gemm` would make, as a `PreparedCall` (result: ``out``)."""
     ba, ra, ca, lda, sa = _mat_geometry(a)
     bb, rb, cb, ldb, sb = _mat_geometry(b)
+    _fp32(bias, colsum_out)
     M, K = (ca, ra) if trans_a else (ra, ca)
     K2, N = (cb, rb) if trans_b else (rb, cb)
     if K != K2:
@@ -193,6 +194,7 @@ def gemm_reduce_scatter(ctx: Context, a: torch.Tensor, b: torch.Tensor, owners, 
     ``store``, stored there (``sb200_gemm_scatter``)."""
     _, ra, ca, lda, _ = _mat_geometry(a)
     _, rb, cb, ldb, _ = _mat_geometry(b)
+    _fp32(colsum_out)
     M, K = (ca, ra) if trans_a else (ra, ca)
     K2, N = (cb, rb) if trans_b else (rb, cb)
     if K != K2:
@@ -208,6 +210,7 @@ def gemm_reduce_scatter(ctx: Context, a: torch.Tensor, b: torch.Tensor, owners, 
 def sum_blocks(ctx: Context, out: torch.Tensor, blocks: torch.Tensor) -> torch.Tensor:
     """out [rows, cols] = blocks[0] + blocks[1] + ... (``blocks``: [n, rows, cols], fp32 adds
     in that order; ``out`` may be ``blocks[0]``)."""
+    _fp32(out, blocks)
     n, rows, cols = blocks.shape
     L.check("sb200_sum_blocks", L.lib().sb200_sum_blocks(
         ctx.handle, out.data_ptr(), out.stride(0), blocks.data_ptr(), n, blocks.stride(0), rows, cols,
@@ -258,6 +261,7 @@ class CsrMatrix:
 def spgemm(ctx: Context, A: CsrMatrix, B: CsrMatrix) -> CsrMatrix:
     """C = A.B with caller-owned (torch) output arrays: symbolic pass, allocate,
     numeric pass."""
+    _fp32(A.val, B.val)
     dev = A.row.device
     a, b = A.as_struct(), B.as_struct()
     row_c = torch.empty(A.M + 1, dtype=torch.int32, device=dev)
@@ -277,6 +281,7 @@ def spgemm(ctx: Context, A: CsrMatrix, B: CsrMatrix) -> CsrMatrix:
 def spgemm_callee_alloc(ctx: Context, A: CsrMatrix, B: CsrMatrix) -> CsrMatrix:
     """The drop-in call: the library allocates C (cudaMalloc); the arrays are
     copied into torch tensors and the library's copies freed."""
+    _fp32(A.val, B.val)
     dev = A.row.device
     a, b, c = A.as_struct(), B.as_struct(), L.Csr()
     L.check("sb200_spgemm_csr", L.lib().sb200_spgemm_csr(
@@ -294,6 +299,7 @@ def spgemm_callee_alloc(ctx: Context, A: CsrMatrix, B: CsrMatrix) -> CsrMatrix:
 
 def dense_to_csr(ctx: Context, dense: torch.Tensor) -> CsrMatrix:
     """2-D fp32 tensor (last dimension contiguous, any row pitch) -> CSR."""
+    _fp32(dense)
     M, N = dense.shape
     c = L.Csr()
     L.check("sb200_dense_to_csr", L.lib().sb200_dense_to_csr(
@@ -312,6 +318,7 @@ def dense_to_csr(ctx: Context, dense: torch.Tensor) -> CsrMatrix:
 
 
 def csr_to_dense(ctx: Context, A: CsrMatrix, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    _fp32(A.val, out)
     if out is None:
         out = torch.empty(A.M, A.N, dtype=torch.float32, device=A.row.device)
     s = A.as_struct()
@@ -327,30 +334,43 @@ def _ew(name, ctx, *args):
     L.check(name, getattr(L.lib(), name)(ctx.handle, *args, _stream_ptr(ctx.device)))
 
 
+def _fp32(*tensors) -> None:
+    """These calls hand addresses on to fp32 kernels: a 16-bit tensor (which the operators
+    of token models produce) would be read and written beyond its end."""
+    for t in tensors:
+        if t is not None and t.dtype != torch.float32:
+            raise TypeError(f"fp32 only, got {t.dtype}")
+
+
 def relu(ctx, x, out=None):
+    _fp32(x, out)
     out = torch.empty_like(x) if out is None else out
     _ew("sb200_relu", ctx, out.data_ptr(), x.data_ptr(), x.numel())
     return out
 
 
 def relu_backward(ctx, dx, dy, x):
+    _fp32(dx, dy, x)
     _ew("sb200_relu_backward", ctx, dx.data_ptr(), dy.data_ptr(), x.data_ptr(), x.numel())
     return dx
 
 
 def softmax(ctx, x, out=None):
+    _fp32(x, out)
     out = torch.empty_like(x) if out is None else out
     _ew("sb200_softmax", ctx, out.data_ptr(), x.data_ptr(), x.numel(), x.shape[-1])
     return out
 
 
 def softmax_backward(ctx, dx, dy, y):
+    _fp32(dx, dy, y)
     _ew("sb200_softmax_backward", ctx, dx.data_ptr(), dy.data_ptr(), y.data_ptr(), y.numel(),
         y.shape[-1])
     return dx
 
 
 def cross_entropy(ctx, prob, label, out=None):
+    _fp32(prob, label, out)
     out = torch.empty(prob.shape[0], dtype=torch.float32, device=prob.device) if out is None else out
     _ew("sb200_cross_entropy", ctx, out.data_ptr(), prob.data_ptr(), label.data_ptr(),
         prob.shape[0], prob.shape[1])
@@ -358,6 +378,7 @@ def cross_entropy(ctx, prob, label, out=None):
 
 
 def cross_entropy_backward(ctx, dx, prob, label):
+    _fp32(dx, prob, label)
     _ew("sb200_cross_entropy_backward", ctx, dx.data_ptr(), prob.data_ptr(), label.data_ptr(),
         prob.shape[0], prob.shape[1])
     return dx
@@ -368,6 +389,7 @@ def softmax_cross_entropy(ctx, logits, label, prob=None, loss=None, dlogits=None
     logits; returns (prob, loss, dlogits).  A dlogits allocated here gets rows
     padded to a multiple of ``row_pad`` floats (a view of the logical shape is
     returned); with 4 it can feed the tensor-core GEMMs of the backward pass."""
+    _fp32(logits, label, prob, loss, dlogits)
     batch, unit = logits.shape
     logits = logits.contiguous()
     if prob is None:
@@ -384,11 +406,13 @@ def softmax_cross_entropy(ctx, logits, label, prob=None, loss=None, dlogits=None
 
 
 def sgd_update(ctx, z, dz, lr):
+    _fp32(z, dz)
     _ew("sb200_sgd_update", ctx, z.data_ptr(), dz.data_ptr(), float(lr), z.numel())
     return z
 
 
 def scale(ctx, x, factor, out=None):
+    _fp32(x, out)
     out = x if out is None else out
     _ew("sb200_scale", ctx, out.data_ptr(), x.data_ptr(), float(factor), x.numel())
     return out
@@ -618,8 +642,8 @@ def orthogonalize(ctx: Context, g: torch.Tensor, *, steps: int = 5, coefficients
                   eps: float = 1e-7, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The orthogonalised update of a matrix [rows, cols], or of each of a batch of them:
     x = g / (|g| + eps), then ``steps`` Newton-Schulz products
-    x = a x + (b A + c A A) x with A = x x^T.  ``out`` may be ``g``; apply it with
-    ``sgd_update``."""
+    x = a x + (b A + c A A) x with A = x x^T.  ``out`` may be ``g``; a
+    float32 result is applied with ``sgd_update``, which takes float32 only."""
     if g.dim() not in (2, 3):
         raise ValueError("expected [rows, cols] or [batch, rows, cols]")
     code = _type_code(g, "g")

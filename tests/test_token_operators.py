@@ -191,3 +191,39 @@ def test_front_end_refuses_host_tensors():
                  lambda: ops.orthogonalize(Ctx, x), lambda: ops.embedding_backward(Ctx, x, x, torch.zeros(4, dtype=torch.int64))):
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float64])
+def test_fp32_calls_refuse_other_types(dtype):
+    """What takes fp32 addresses refuses the 16-bit tensors that the token operators produce,
+    in every place of its arguments, before the library is called."""
+    from sapphire_b200 import conv, ops
+
+    class Ctx:
+        device, handle = 0, None
+
+    f, h = torch.zeros(4, 4), torch.zeros(4, 4, dtype=dtype)
+    idx = torch.zeros(5, dtype=torch.int32)
+    csr, image = ops.CsrMatrix(idx, idx[:0], h[0, :0], 4, 4), torch.zeros(1, 1, 4, 4)
+    good = ops.CsrMatrix(idx, idx[:0], f[0, :0], 4, 4)
+    for call in (
+            lambda: ops.relu(Ctx, h), lambda: ops.relu(Ctx, f, h),
+            lambda: ops.relu_backward(Ctx, h, f, f), lambda: ops.relu_backward(Ctx, f, h, f), lambda: ops.relu_backward(Ctx, f, f, h),
+            lambda: ops.softmax(Ctx, h), lambda: ops.softmax(Ctx, f, h),
+            lambda: ops.softmax_backward(Ctx, h, f, f), lambda: ops.softmax_backward(Ctx, f, h, f), lambda: ops.softmax_backward(Ctx, f, f, h),
+            lambda: ops.cross_entropy(Ctx, h, f), lambda: ops.cross_entropy(Ctx, f, h), lambda: ops.cross_entropy(Ctx, f, f, h[0]),
+            lambda: ops.cross_entropy_backward(Ctx, h, f, f), lambda: ops.cross_entropy_backward(Ctx, f, h, f),
+            lambda: ops.cross_entropy_backward(Ctx, f, f, h),
+            lambda: ops.softmax_cross_entropy(Ctx, h, f), lambda: ops.softmax_cross_entropy(Ctx, f, h),
+            lambda: ops.softmax_cross_entropy(Ctx, f, f, prob=h), lambda: ops.softmax_cross_entropy(Ctx, f, f, loss=h[0]),
+            lambda: ops.softmax_cross_entropy(Ctx, f, f, dlogits=h),
+            lambda: ops.sgd_update(Ctx, h, f, 0.1), lambda: ops.sgd_update(Ctx, f, h, 0.1),
+            lambda: ops.scale(Ctx, h, 2.0), lambda: ops.scale(Ctx, f, 2.0, h),
+            lambda: ops.sum_blocks(Ctx, h, f[None]), lambda: ops.sum_blocks(Ctx, f, h[None]),
+            lambda: ops.gemm(Ctx, f, f, bias=h[0]), lambda: ops.gemm(Ctx, f, f, colsum_out=h[0]),
+            lambda: ops.dense_to_csr(Ctx, h), lambda: ops.csr_to_dense(Ctx, csr), lambda: ops.csr_to_dense(Ctx, good, h),
+            lambda: ops.spgemm(Ctx, csr, good), lambda: ops.spgemm(Ctx, good, csr), lambda: ops.spgemm_callee_alloc(Ctx, csr, good),
+            lambda: conv.im2col(Ctx, image.to(dtype), 3, 3), lambda: conv.col2im(Ctx, image.to(dtype), image, 3, 3),
+            lambda: conv.col2im(Ctx, image, image.to(dtype), 3, 3)):
+        with pytest.raises(TypeError):
+            call()
