@@ -142,6 +142,25 @@ __device__ __forceinline__ bool wait_bar_cluster(uint64_t* bar, uint32_t parity,
     return true;
 }
 
+// Behind the barrier of a kernel's common exit, by all threads.  After a wait that gave up, tile
+// copies and products that this CTA has issued may still be on their way into its shared
+// memory and TMEM, which the next CTA gets: they take microseconds, so the CTA stays another
+// SETTLE_NS.  (By time and not by their barriers, since a copy that never comes would be
+// waited for in vain.)
+constexpr unsigned long long SETTLE_NS = 200000;
+__device__ __forceinline__ void settle(const Abort& ab)
+{
+    if (*ab.flag == 0)
+        return;
+    ptx::cp_async_wait_all();
+    if (threadIdx.x == 0) {
+        const uint64_t t0 = ptx::globaltimer_ns();
+        while (ptx::globaltimer_ns() - t0 < SETTLE_NS) {
+        }
+    }
+    __syncthreads();
+}
+
 // One thread's 32 consecutive output columns of one row: D = post((C + bias) + acc);
 // mrow is the row of the gate matrix or null.
 __device__ __forceinline__ void store_row_chunk(const uint32_t (&v)[32], float* drow,

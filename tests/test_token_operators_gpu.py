@@ -664,6 +664,31 @@ def test_orthogonalize_bounded_waits(ctx):
     assert torch.equal(ops.orthogonalize(ctx, small), want)
 
 
+def test_expired_waits_leave_what_comes_behind_alone(ctx):
+    """A product that gave up stays on its SMs until what it has issued has landed: the kernels
+    enqueued right behind it, which get its shared memory and tensor memory, are as ever."""
+    g = gen(9)
+    ms = [gradient(g, 130, 300), gradient(g, 2300, 2300), gradient(g, 90, 900), gradient(g, 1024, 1024, dtype=BF16)]
+    x, a = randn(g, 4096, 2048), randn(g, 512, 512)
+    want = [*ops.layer_norm(ctx, x), ops.gemm(ctx, a, a), *(ops.orthogonalize(ctx, m) for m in ms)]
+    ctx.check_device_status()
+    ctx.set_option(L.OPT_WAIT_LIMIT_US, 5000)
+    try:
+        for m in ms:
+            ctx.set_option(L.OPT_TEST_STALL_KBLOCKS, 1)
+            ops.orthogonalize(ctx, m, steps=1)
+            ctx.set_option(L.OPT_TEST_STALL_KBLOCKS, -1)
+            got = [*ops.layer_norm(ctx, x), ops.gemm(ctx, a, a), *(ops.orthogonalize(ctx, m) for m in ms)]
+            with pytest.raises(L.Sb200Error) as e:
+                ctx.check_device_status()
+            assert e.value.status == L.ERR_DEVICE_TIMEOUT
+            ctx.check_device_status()
+            assert all(torch.equal(p, q) for p, q in zip(got, want))
+    finally:
+        ctx.set_option(L.OPT_TEST_STALL_KBLOCKS, -1)
+        ctx.set_option(L.OPT_WAIT_LIMIT_US, 2000000)
+
+
 # ----------------------------------------------------------- streams and graphs
 
 def test_other_streams_and_captured_graphs(ctx):
