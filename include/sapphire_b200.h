@@ -618,6 +618,7 @@ int sb200_embedding_backward(sb200_ctx* ctx, void* dtable, int64_t ldt, const vo
  * SB200_F32; weight NULL is 1, bias NULL is 0.  mean and rstd ([rows], fp32, each may
  * be NULL) are what the backward pass wants.  y may be x itself (same pointer and
  * pitch).  Statistics in fp32 from differences to the mean; y is rounded once.
+ * Limits (SB200_ERR_TOO_LARGE), of the backward pass too: rows <= 2^40, cols <= 2^35.
  */
 int sb200_layer_norm(sb200_ctx* ctx, void* y, int64_t ldy, float* mean, float* rstd,
                      const void* x, int64_t ldx, const void* weight, const void* bias,

@@ -802,6 +802,11 @@ int with_width(int vec, F f)
     return f(Int<1>{});
 }
 
+// Beyond any memory; within them no size and no grid's extent overflows (ln_reduce_kernel has a
+// block for 32 columns).
+constexpr int64_t MAX_ROWS = int64_t(1) << 40;
+constexpr int64_t MAX_COLS = int64_t(1) << 35;
+
 int check_types(int type, int weight_type)
 {
     if (!known_type(type) || !known_type(weight_type)) return SB200_ERR_INVALID_ARG;
@@ -844,6 +849,7 @@ extern "C" int sb200_layer_norm(sb200_ctx* ctx, void* y, int64_t ldy, float* mea
     TraceRange trace("sb200_layer_norm");
     if (!ctx || rows < 0 || cols < 1 || ldx < cols || ldy < cols || !(eps >= 0.0f)) return SB200_ERR_INVALID_ARG;
     if (const int rc = check_types(type, weight_type)) return rc;
+    if (rows > MAX_ROWS || cols > MAX_COLS) return SB200_ERR_TOO_LARGE;
     if (rows == 0) return SB200_OK;
     if (!x || !y || !aligned_to(x, type_bytes(type)) || !aligned_to(y, type_bytes(type)) || !aligned_to(weight, type_bytes(weight_type)) ||
         !aligned_to(bias, type_bytes(weight_type)) || !aligned_to(mean, 4) || !aligned_to(rstd, 4))
@@ -907,7 +913,7 @@ extern "C" int sb200_layer_norm(sb200_ctx* ctx, void* y, int64_t ldy, float* mea
 
 extern "C" int64_t sb200_layer_norm_backward_workspace(const sb200_ctx* ctx, int64_t rows, int64_t cols)
 {
-    if (!ctx || rows < 0 || cols < 1) return -1;
+    if (!ctx || rows < 0 || cols < 1 || rows > MAX_ROWS || cols > MAX_COLS) return -1;
     return backward_parts(ctx->sm_count, rows, cols) * cols * 2 * static_cast<int64_t>(sizeof(float));
 }
 
@@ -920,6 +926,7 @@ extern "C" int sb200_layer_norm_backward(sb200_ctx* ctx, void* dx, int64_t lddx,
     TraceRange trace("sb200_layer_norm_backward");
     if (!ctx || rows < 0 || cols < 1 || ldx < cols || lddy < cols || (dx && lddx < cols)) return SB200_ERR_INVALID_ARG;
     if (const int rc = check_types(type, weight_type)) return rc;
+    if (rows > MAX_ROWS || cols > MAX_COLS) return SB200_ERR_TOO_LARGE;
     if (rows > 0 && (!x || !dy || !mean || !rstd)) return SB200_ERR_INVALID_ARG;
     for (const void* at : {static_cast<const void*>(x), dy, static_cast<const void*>(dx)})
         if (!aligned_to(at, type_bytes(type))) return SB200_ERR_INVALID_ARG;

@@ -146,6 +146,15 @@ def test_empty_calls_touch_nothing(fake):
     assert orthogonalize(fake, batch=0) == L.OK
 
 
+@pytest.mark.parametrize("rows,cols", [(1 << 41, 8), (4, 1 << 36), (1 << 20, 1 << 61), (1 << 62, 1 << 13)])
+def test_layer_norm_sizes_beyond_any_memory(fake, rows, cols):
+    """Refused before a size in bytes or a grid's extent wraps (rows of 2^61 columns would have
+    had a workspace of no bytes)."""
+    assert layer_norm(fake, rows=rows, cols=cols, ldx=cols, ldy=cols) == L.ERR_TOO_LARGE
+    assert layer_norm_backward(fake, rows=rows, cols=cols, ldx=cols, lddx=cols, lddy=cols) == L.ERR_TOO_LARGE
+    assert L.lib().sb200_layer_norm_backward_workspace(fake, rows, cols) == -1
+
+
 def test_workspace_sizes(fake):
     lib = L.lib()
     assert lib.sb200_embedding_backward_workspace(None, 4, 10, 8) == -1
