@@ -656,7 +656,9 @@ int sb200_layer_norm_backward(sb200_ctx* ctx, void* dx, int64_t lddx, void* dwei
  * Coefficients that let a singular value s, or |b s^2 + c s^4| with or without a in
  * front, pass about 7 on the way are refused (SB200_ERR_UNSUPPORTED).  Limits
  * (SB200_ERR_TOO_LARGE): sides <= 2^20, batch <= 65535, steps <= 64.  The waits inside
- * the kernels are bounded like those of the GEMM.
+ * the kernels are bounded like those of the GEMM.  Matrices with a side of at most 128
+ * and the other of at most 2048 need no scratch: their workspace is 4096 bytes, whatever
+ * the batch.
  */
 int64_t sb200_orthogonalize_workspace(int64_t rows, int64_t cols, int64_t batch, int type);
 int sb200_orthogonalize(sb200_ctx* ctx, void* out, int64_t ldo, int64_t stride_out,

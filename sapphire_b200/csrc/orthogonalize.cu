@@ -781,6 +781,10 @@ OrthPlan plan_orth(int64_t rows, int64_t cols, int64_t batch, int type)
     q.R = rows < cols ? rows : cols;
     q.C = rows < cols ? cols : rows;
     q.batch = batch;
+    if (orthogonalize_small_always(rows, cols)) {        // never read: a page, so that every call has a workspace
+        q.total = 4096;
+        return q;
+    }
     q.ldx = (q.C + 63) / 64 * 64;
     q.lda = (q.R + 63) / 64 * 64;
     q.split = type != SB200_BF16 || q.R <= 128;  // whichever kernel a narrow matrix takes, its operands have 22 bits
@@ -964,6 +968,7 @@ extern "C" int sb200_orthogonalize(sb200_ctx* ctx, void* out, int64_t ldo, int64
     cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     const OrthCall call{out, ldo, batch > 1 ? stride_out : 0, g, ldg, batch > 1 ? stride_g : 0, rows, cols, batch, steps, a, b, c, eps, type};
     if (orthogonalize_small_fits(ctx, call)) return launch_orthogonalize_small(ctx, call, stream);
+    if (orthogonalize_small_always(rows, cols)) return SB200_ERR_CUDA;   // (the device did not grant the kernel its shared memory)
     unsigned char* ws = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~uintptr_t(255));
     const int tall = rows > cols;
 

@@ -52,7 +52,10 @@ __device__ __forceinline__ void join_f16(float (&v)[8], const Raw<f16, 8>& part)
     }
 }
 
-// orthogonalize_small.cu: matrices whose shorter side is at most 128, whole in one cluster
+// orthogonalize_small.cu: matrices whose shorter side is at most 128, whole in one cluster.
+// always: as large as a portable cluster holds, so that no other way is taken on any device;
+// fits: as large as the cluster that the context's device grants.
+bool orthogonalize_small_always(int64_t rows, int64_t cols);
 bool orthogonalize_small_fits(const sb200_ctx* ctx, const OrthCall& q);
 int launch_orthogonalize_small(sb200_ctx* ctx, const OrthCall& q, cudaStream_t stream);
 

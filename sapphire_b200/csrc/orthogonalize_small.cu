@@ -31,7 +31,8 @@ namespace {
 constexpr int SMALL_THREADS = 512, SMALL_WARPS = 16;
 constexpr int SMALL_TILE = 128 * 128;            // 128 rows of 64 fp16 elements, in bytes
 constexpr int SMALL_W = 256;                     // columns of a CTA at most
-constexpr int SMALL_CTAS = 16;                   // beyond 8 where the device grants clusters of that size
+constexpr int SMALL_CTAS = 16;                   // beyond PORTABLE_CTAS where the device grants clusters of that size
+constexpr int PORTABLE_CTAS = 8;
 constexpr int SMALL_X_PART = SMALL_W / 64 * SMALL_TILE;
 constexpr int SMALL_A_PART = 2 * SMALL_TILE;
 constexpr int SMALL_SMEM = 2 * SMALL_X_PART + 2 * SMALL_A_PART + 256 + 1024;
@@ -390,7 +391,7 @@ cudaLaunchConfig_t small_config(cudaLaunchAttribute (&attr)[2], int64_t batch, i
     return cfg;
 }
 
-// The largest cluster this kernel can have on the context's device: 16, 8, or 0 (asked once).
+// The largest cluster this kernel can have on the context's device: SMALL_CTAS, PORTABLE_CTAS, or 0 (asked once).
 template <typename T>
 int largest_cluster(const sb200_ctx* ctx)
 {
@@ -399,17 +400,17 @@ int largest_cluster(const sb200_ctx* ctx)
     auto kern = orth_small_kernel<T>;
     int most = 0;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMALL_SMEM) == cudaSuccess) {
-        most = 8;
+        most = PORTABLE_CTAS;
         cudaLaunchAttribute attr[2];
-        cudaLaunchConfig_t cfg = small_config<T>(attr, 1, 16, nullptr);
+        cudaLaunchConfig_t cfg = small_config<T>(attr, 1, SMALL_CTAS, nullptr);
         cfg.numAttrs = 1;
         int fit = 0;
         if (cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
             cudaOccupancyMaxActiveClusters(&fit, kern, &cfg) == cudaSuccess && fit > 0)
-            most = 16;
+            most = SMALL_CTAS;
         cudaGetLastError();
     }
-    if (ctx->device < 16) known[ctx->device] = most + 1;
+    if (ctx->device < 16 && most > 0) known[ctx->device] = most + 1;     // (a refusal is asked about again)
     return most;
 }
 
@@ -421,6 +422,12 @@ int with_small_type(int type, F f)
 }
 
 }  // namespace
+
+bool orthogonalize_small_always(int64_t rows, int64_t cols)
+{
+    const int64_t r = rows < cols ? rows : cols, c = rows < cols ? cols : rows;
+    return r <= 128 && c <= SMALL_W * PORTABLE_CTAS;
+}
 
 bool orthogonalize_small_fits(const sb200_ctx* ctx, const OrthCall& q)
 {

@@ -170,6 +170,18 @@ def test_workspace_sizes(fake):
     assert lib.sb200_orthogonalize_workspace(512, 784, 1, L.F32) >= 2 * (4 * 512 * 784 + 4 * 512 * 512)
 
 
+@pytest.mark.parametrize("t", [L.F32, L.BF16, L.F16])
+def test_workspace_of_matrices_that_need_none(t):
+    """What one cluster of any device holds asks for a page, whatever the batch; the next size
+    up, which another device may take the general way with, for all its matrices."""
+    size = L.lib().sb200_orthogonalize_workspace
+    for rows, cols in ((1, 1), (128, 2048), (2048, 128), (50, 60)):
+        for batch in (0, 1, 65535):
+            assert size(rows, cols, batch, t) == 4096
+    for rows, cols in ((128, 2049), (129, 129)):
+        assert size(rows, cols, 10, t) > 10 * rows * cols * 2 * 4
+
+
 def test_workspace_of_narrow_bf16(fake):
     """With a side of at most 128 every operand has two parts, for bf16 as for fp32; with both
     sides longer A and B have one."""

@@ -664,6 +664,23 @@ def test_orthogonalize_bounded_waits(ctx):
     assert torch.equal(ops.orthogonalize(ctx, small), want)
 
 
+@pytest.mark.parametrize("batch,rows,cols", [(1, 128, 2048), (700, 2000, 100), (3, 40, 50)])
+def test_orthogonalize_reads_and_writes_no_workspace_where_it_needs_none(ctx, batch, rows, cols):
+    """The page such a call asks for stays as it was, and the buffer behind it too."""
+    g = gradient(gen(batch), batch, rows, cols)
+    want = ops.orthogonalize(ctx, g)
+    need = L.lib().sb200_orthogonalize_workspace(rows, cols, batch, L.F32)
+    assert need == 4096
+    ws = torch.full((2 * need,), 0xA5, dtype=torch.uint8, device=DEV)
+    out = torch.full_like(g, float("nan"))
+    torch.cuda.synchronize()
+    status = L.lib().sb200_orthogonalize(ctx.handle, out.data_ptr(), cols, rows * cols, g.data_ptr(), cols, rows * cols, rows, cols,
+                                         batch, 5, *COEF, 1e-7, L.F32, ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
+    assert status == L.OK
+    ctx.check_device_status()
+    assert torch.equal(out, want) and (ws == 0xA5).all()
+
+
 def test_expired_waits_leave_what_comes_behind_alone(ctx):
     """A product that gave up stays on its SMs until what it has issued has landed: the kernels
     enqueued right behind it, which get its shared memory and tensor memory, are as ever."""
