@@ -198,6 +198,38 @@ def test_embedding_backward_long_runs(ctx, n, distinct):
     check(dt, want, (count + 2) * U * size)
 
 
+@pytest.mark.parametrize("tt,ta", [(F32, F32), (F32, BF16), (BF16, BF16), (F16, F32)])
+@pytest.mark.parametrize("n,vocab,cols,index", [(16384, 3000, 24, torch.int64), (16385, 3000, 24, torch.int32), (16385, 300000, 16, torch.int64),
+                                                (20011, 900, 2064, torch.int64), (70001, 5000, 33, torch.int32)])
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_embedding_backward_sorted_by_several_blocks(ctx, tt, ta, n, vocab, cols, index, accumulate):
+    """On both sides of 16384 tokens, from where on several blocks sort: padding and a number
+    beyond the vocabulary among the tokens, rows that no token names, a token number that runs over
+    many pieces, a third pass of the sort (300000 rows), several tiles of columns (2064)."""
+    g = gen(n + cols)
+    ids = token_ids(g, n, vocab // 2, index)
+    ids[torch.randperm(n, generator=g)[: n // 4]] = vocab - 2        # behind the half that the others name
+    ids[n // 3] = vocab
+    dout = randn(g, n, cols, dtype=ta)
+    before = randn(g, vocab, cols, dtype=tt) if accumulate else torch.full((vocab, cols), float("nan"), dtype=tt, device=DEV)
+    dt = ops.embedding_backward(ctx, before.clone(), dout, ids.to(DEV), scale=-0.5, accumulate=accumulate)
+    with pytest.raises(L.Sb200Error) as e:
+        ctx.check_device_status()
+    assert e.value.status == L.ERR_TOKEN_RANGE
+    want, size, count = grad_reference(dout, torch.where(ids < vocab, ids, -1), vocab, -0.5)
+    assert (count == 0).any() and count[vocab - 2] > 3000
+    if accumulate:
+        want = want + before.cpu().double()
+        idle = (count[:, 0] == 0).to(DEV)
+        assert torch.equal(dt[idle], before[idle])
+        size = size + want.abs()
+    check(dt, want, (count + 2) * U * size + half_step(tt) * want.abs() * 1.001 + tiny(tt))
+    again = ops.embedding_backward(ctx, before.clone(), dout, ids.to(DEV), scale=-0.5, accumulate=accumulate)
+    assert torch.equal(again, dt)
+    with pytest.raises(L.Sb200Error):
+        ctx.check_device_status()
+
+
 def test_embedding_backward_all_padding(ctx):
     dt = torch.full((33, 12), float("nan"), device=DEV)
     ids = torch.full((100,), -1, dtype=torch.int32, device=DEV)
