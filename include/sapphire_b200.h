@@ -596,8 +596,8 @@ int sb200_embedding(sb200_ctx* ctx, void* out, int64_t ldo, const void* table, i
 
 /*
  * The table's gradient: dtable[v, :] = scale * sum of dout[t, :] over the tokens t
- * with ids[t] == v, in an order that depends on the token numbers alone; sums in
- * fp32, rounded once.  accumulate = 0: every row of dtable is written, with zeros
+ * with ids[t] == v, in an order that depends on the token numbers, cols and the
+ * device's number of SMs alone; sums in fp32, rounded once.  accumulate = 0: every row of dtable is written, with zeros
  * where no token names it.  accumulate != 0: the sums are added to dtable and the
  * other rows are neither read nor written; with dtable the table itself and scale
  * times -lr this is the SGD step of the rows in use.  Padding and out-of-range

@@ -72,7 +72,7 @@ struct TensorMapKey {
     uint64_t base;
     int64_t contig, rows, ld, batches, batch_stride;
     int64_t box_rows;      // rows (3-D map) or chunks (merged 4-D map) per box
-    int64_t kind;          // 0: K-major 3-D, 1: MN-major 3-D, 2: MN-major merged 4-D
+    int64_t kind;          // fp32: 0 K-major 3-D, 1 MN-major 3-D, 2 MN-major merged 4-D; 3: fp16 3-D (orthogonalize)
 };
 struct alignas(64) TensorMapSlot {
     CUtensorMap map;

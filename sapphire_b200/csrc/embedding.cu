@@ -6,7 +6,7 @@
 // Both are bound by memory: the lookup reads the rows that are named and writes one row
 // a token; the gradient reads one row a token and writes the whole table (or, when it
 // accumulates, reads and writes the rows that are named).  65536 tokens x 4096 bf16: lookup
-// 125 us (5.4 TB/s), gradient into an fp32 table 304 us (5.2 TB/s).
+// 125 us (5.4 TB/s), gradient into an fp32 table 304 us (5.2 TB/s), added to it 229 us.
 //
 // The gradient needs the tokens of one vocabulary row together and in a fixed order, so
 // that the sum is the same run to run.  The token positions are sorted by vocabulary row
@@ -528,7 +528,7 @@ grad_join_kernel(TT* __restrict__ dtable, const GradArgs a, int lanes, int col_t
 
 constexpr int64_t MAX_TOKENS = int64_t(1) << 30;
 constexpr int64_t MAX_VOCAB = (int64_t(1) << 31) - 2;
-constexpr int64_t MAX_COLS = int64_t(1) << 20;           // column tiles are a grid's y extent
+constexpr int64_t MAX_COLS = int64_t(1) << 20;           // pieces of a row are counted in 32 bits
 
 int check_types(int table_type, int type, int index_bits)
 {

@@ -7,15 +7,15 @@
 //
 // Memory bound: the forward pass has to read x and write y, the backward pass to read
 // x and dy and write dx.  A row is read once, held in the registers of the threads that
-// share it (a group of 1 to 32 lanes, or a block of up to 512 threads, 16 elements a
-// thread), and its sums are taken over those registers, so the variance is the mean of
+// share it (a group of 1 to 32 lanes, or a block of up to 512 threads; 16 elements a
+// thread, in the forward pass 32 where rows have more than 512), and its sums are taken over those registers, so the variance is the mean of
 // squared differences from a mean, not a difference of large sums.  All sums are fp32.
 // The blocks walk over rows; each thread keeps its columns' weights in registers and has
 // its pieces of the next rows on the way into shared memory (its own slots, so nothing
 // but the thread itself waits for them): the memory system always has several rows a
 // block to work on, which one row at a time in registers does not give it (65536 x 4096
-// bf16 forward: 291 us, so 180 to 192 or 5.6 to 6.0 TB/s; 32768 x 4096 fp32 backward: 240 us,
-// 6.7 TB/s).  In the backward pass every thread keeps the column sums of its
+// bf16 forward: 291 us, so 180 to 193 or 5.6 to 6.0 TB/s; 32768 x 4096 fp32 backward: 238 to
+// 251 us, 6.4 to 6.8 TB/s).  In the backward pass every thread keeps the column sums of its
 // columns in registers over all the rows its block sees, writes one partial sum a block,
 // and a second kernel adds the partials in block order: no atomics, the same bits run to
 // run.  Rows that 16-byte accesses do not fit take 4-byte ones.  Odd rows of 16-bit elements

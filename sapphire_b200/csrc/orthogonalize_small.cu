@@ -14,9 +14,10 @@
 //     distributed shared memory, splits the sums into parts and stores them in every CTA
 //   B = b A + c A A by every CTA for itself
 //   X = a X + B X on the CTA's columns
-// Products, parts and roundings are those of the general way with two parts, for bf16 too: the
-// products are too short to gain from one.  Five steps take 50 us for 128 x 128 fp32 (135 in
-// launches), 78 for 128 x 1000, 108 for 128 x 4000.
+// Products and parts are those of the general way with two parts, for bf16 too: the products
+// are too short to gain from one.  Accumulation chains have 32 of k (64 in B X where W columns
+// leave room for two accumulators only; the general way's have 64 or 128).  Five steps take 50 us for 128 x 128 fp32 (135 in
+// launches), 77 for 128 x 1000, 86 for 128 x 2000, 108 for 128 x 4000.
 #include <type_traits>
 
 #include "gemm_common.cuh"
@@ -39,7 +40,7 @@ constexpr int SMALL_SMEM = 2 * SMALL_X_PART + 2 * SMALL_A_PART + 256 + 1024;
 
 struct SmallParams {
     OrthCall q;
-    int R, C, W, ctas, tall, final_vec;
+    int R, C, W, ctas, tall;
     unsigned* status;
     unsigned long long wait_limit_ns;
     int test_stall_kb;

@@ -117,8 +117,9 @@ __device__ __forceinline__ void prefetch_tensormap(const CUtensorMap* map)
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
 
-// 16 bytes global -> shared by this thread, asynchronously; the first `bytes` (0 or 16) are
-// read, the rest is zero.
+// 16 bytes global -> shared by this thread, asynchronously; the first `bytes` (0 to 16) are
+// read, the rest is filled with zeros (layer norm's rows with a shift end in such pieces and
+// add the zeros up).  Both addresses are 16-byte aligned, whatever `bytes` is.
 __device__ __forceinline__ void cp_async_16(void* smem_dst, const void* src, int bytes)
 {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(smem_dst)), "l"(src), "r"(bytes)
