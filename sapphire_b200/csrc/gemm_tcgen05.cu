@@ -20,7 +20,8 @@
 //
 // Every wait on an mbarrier is bounded; when one expires the CTA records a code
 // in the status word, raises a CTA-wide abort flag, and every role falls through
-// to the common exit, where the CTA waits for what it has issued and releases TMEM.
+// to the common exit, behind the time that what it has issued needs to land, where TMEM is
+// released.
 #include "gemm_common.cuh"
 
 namespace sb200 {
@@ -579,7 +580,6 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap mapA,
     // common exit: every thread arrives here, also after an abort
     ptx::tc_fence_before_sync();
     __syncthreads();
-    settle(ab);
     if (warp == 1) {
         __syncwarp();
         ptx::tc_fence_after_sync();

@@ -274,7 +274,6 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap mapA,
     // common exit: no CTA may leave while its peer can still touch its barriers or TMEM
     ptx::tc_fence_before_sync();
     __syncthreads();
-    settle(ab);
     ptx::cluster_sync();
     if (warp == 1) {
         __syncwarp();

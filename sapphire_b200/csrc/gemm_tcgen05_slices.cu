@@ -269,7 +269,6 @@ gemm_tcgen05_slices_kernel(const __grid_constant__ CUtensorMap mapA, const __gri
     // common exit: every thread arrives here, also after an abort
     ptx::tc_fence_before_sync();
     __syncthreads();
-    settle(ab);
     if (warp == 1) {
         __syncwarp();
         ptx::tc_fence_after_sync();

@@ -644,7 +644,6 @@ orth_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     // common exit, also after an abort; a CTA of a cluster stays while a peer may touch its memory
     ptx::tc_fence_before_sync();
     __syncthreads();
-    settle(ab);
     ptx::cluster_sync_relaxed();
     if (warp == 1) {
         __syncwarp();

@@ -364,7 +364,6 @@ __global__ void __launch_bounds__(SMALL_THREADS, 1) orth_small_kernel(const Smal
 
     ptx::tc_fence_before_sync();
     __syncthreads();
-    settle(ab);
     if (p.ctas > 1) ptx::cluster_sync_relaxed();         // a peer may still store into this CTA's A
     if (warp == 0) {
         __syncwarp();
