@@ -62,7 +62,7 @@ constexpr int ORTH_PANEL = 8;
 constexpr int MAX_SLICES = 8;
 constexpr int PART_LD = 132;                     // floats per row of a partial tile in shared memory
 
-enum Product { GRAM, POLY, APPLY };
+enum Product { GRAM, POLY, APPLY, LONG_GRAM };   // LONG_GRAM: X X^T in chains of LONG_CHAIN_KB (one part, pairs)
 
 // A matrix of the iteration: [parts][batch][rows][ld] fp16, part 0 = hi, 1 = lo.
 struct Split {
@@ -420,7 +420,7 @@ orth_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
             if constexpr (PAIR && (READS_HI || READS_LO)) {
                 if (blocks > 0) fetch(0);        // travels while the products run
             }
-            if (SPLIT || !PAIR || (WHAT == GRAM && p.chunk_kb < p.num_kb)) {
+            if (SPLIT || !PAIR || WHAT == LONG_GRAM) {
                 // chains of accumulations are added here, rounded to nearest
                 float sum[COLS];
 #pragma unroll
@@ -883,9 +883,15 @@ int product(sb200_ctx* ctx, bool split, const OrthMaps& m, OrthParams p, cudaStr
     // what the chain cuts off goes to one side: 3.0e-3 of a sum over 2^19 columns in a single chain (measured,
     // 0.8 x 2^-23 an accumulation).  The others run over the shorter side; where that is 2^16 (X in its parts
     // and copies then takes 69 GB) a chain loses 4e-4, less than the half step of its fp16 operands.
-    p.chunk_kb = split ? (p.slices == 0 ? CHUNK_KB : 1) : WHAT == GRAM && p.num_kb > LONG_CHAIN_KB ? LONG_CHAIN_KB : p.num_kb;
-    if (p.slices == 0)
+    const bool chains = WHAT == GRAM && !split && p.num_kb > LONG_CHAIN_KB;
+    p.chunk_kb = split ? (p.slices == 0 ? CHUNK_KB : 1) : chains ? LONG_CHAIN_KB : p.num_kb;
+    if (p.slices == 0) {
+        // (a kernel apart from GRAM: with the code for the chains that one has 96 registers instead of 85,
+        // and 4 x 1024 x 4096 takes 497 us instead of 495)
+        if constexpr (WHAT == GRAM)
+            if (chains) return launch_product<LONG_GRAM, true, false>(ctx, m, p, stream);
         return split ? launch_product<WHAT, true, true>(ctx, m, p, stream) : launch_product<WHAT, true, false>(ctx, m, p, stream);
+    }
     return split ? launch_product<WHAT, false, true>(ctx, m, p, stream) : launch_product<WHAT, false, false>(ctx, m, p, stream);
 }
 
