@@ -826,6 +826,44 @@ def test_two_streams_at_once(ctx):
     assert all(torch.equal(p, q) for out in got for p, q in zip(out, want))
 
 
+def test_two_host_threads_with_a_context_each(ctx):
+    """A context per host thread, as documented: the calls of two threads at the same time."""
+    import threading
+    g = gen(16)
+    ms = [gradient(g, 300, 700), gradient(g, 100, 900, dtype=BF16), gradient(g, 1100, 1300, dtype=BF16)]
+    ids, dout = token_ids(g, 20000, 3000, torch.int64).to(DEV), randn(g, 20000, 40)
+    x, w = randn(g, 2001, 999, dtype=BF16), randn(g, 999)
+
+    def work(c):
+        out = [ops.orthogonalize(c, m) for m in ms]
+        out += [ops.embedding_backward(c, torch.empty(3000, 40, device=DEV), dout[:n], ids[:n]) for n in (20000, 5000)]
+        y, mean, rstd = ops.layer_norm(c, x, w)
+        return out + [y, *ops.layer_norm_backward(c, y, x, mean, rstd, w)]
+
+    want = work(ctx)
+    torch.cuda.synchronize()
+    got, failed = [], []
+
+    def thread():
+        try:
+            own = ops.Context(0)
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(10):
+                    got.append(work(own))
+                own.check_device_status()
+        except Exception as e:
+            failed.append(e)
+
+    threads = [threading.Thread(target=thread) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed and len(got) == 20
+    assert all(torch.equal(p, q) for out in got for p, q in zip(out, want))
+
+
 def test_offsets_beyond_32_bits(ctx):
     """Rows so far apart that the last ones start more than 2^32 elements in."""
     g = gen(14)
